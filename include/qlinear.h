@@ -66,6 +66,11 @@ typedef enum {
     QL_KERNEL_GEMV_REGS = 7, /* the register-fed GEMV alone (M <= 8)                     */
 } ql_kernel;
 
+typedef enum {
+    QL_ROPE_HALF = 0,        /* pairs (i, i + rotary_dim / 2)                           */
+    QL_ROPE_INTERLEAVED = 1, /* pairs (2i, 2i + 1)                                      */
+} ql_rope_layout;
+
 /* Fused epilogue and options of ql_quantized_matmul.  Zero-initialise, then set
  * what is needed.  Replaces the ops the reference runs after quantized_matmul:
  * the bias add (src/adapters.rs:318-320), the LoRA residual sum
@@ -192,6 +197,76 @@ int ql_quantized_matmul_noalloc(const void *x, int x_dtype, int64_t M, int64_t K
                                 const uint32_t *wq, const void *scales, const void *biases,
                                 int sb_dtype, int64_t N, int group_size, int bits, int transpose,
                                 const ql_epilogue *ep, void *y, int y_dtype, void *stream);
+
+/* ---- decoder operators: what stands between the quantized linears of a decoder layer or a
+ * DiT block.  Pages: a cache of one layer is [num_pages, Hkv, page_size, D] for the keys and
+ * the same for the values; page p starts page_stride elements after page p - 1 and its
+ * [Hkv, page_size, D] are contiguous.  A sequence's page table row lists its pages in order;
+ * position j is slot table[j / page_size] * page_size + j % page_size. */
+
+/* The norms around a block, fused with its gate and residual scale:
+ *     u = post_weight ? rms(y) * (weight_offset + post_weight) : y
+ *     r_out = residual + alpha * gate * u
+ *     h = rms(r) * (weight_offset + weight) * (1 + scale),   rms(x) = x / sqrt(mean(x^2) + eps)
+ * in fp32, each output rounded once (h is computed from the unrounded r).  y, weights, gate,
+ * scale and h in y_dtype, residual and r_out in r_dtype (y's, or f32).  D in [1, 32768];
+ * y_stride / r_stride: elements between rows of y / residual (h and r_out are contiguous).
+ * gate / scale: [rows, D] with row m / period (period 0: one row for all), or NULL; post_weight
+ * may be NULL.  r_out may be residual itself (same stride), h may be y. */
+int ql_norm_residual(const void *y, int y_dtype, int64_t y_stride, const void *residual, int r_dtype, int64_t r_stride,
+                     int64_t M, int64_t D, const void *weight, float weight_offset, const void *post_weight,
+                     const void *gate, int64_t gate_period, float alpha, const void *scale, int64_t scale_period,
+                     float eps, void *h, void *r_out, void *stream);
+
+/* Rotary positions: q [T, Hq, D] and k [T, Hk, D] (element strides given, D contiguous) ->
+ * contiguous q_out, k_out.  (a, b) -> (a cos - b sin, b cos + a sin) on the pairs of the first
+ * rotary_dim elements of each head, the rest copied; fp32, one rounding.  table: fp32
+ * [table_rows, rotary_dim], row p holds position p's rotary_dim / 2 cosines, then its sines.
+ * A position outside the table gives zeros and sets the device error word.  q_out may be q and
+ * k_out k when those are contiguous.  Hq or Hk may be 0. */
+int ql_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k, int64_t k_token_stride,
+            int64_t k_head_stride, int dtype, int64_t T, int Hq, int Hk, int D, int rotary_dim, int layout,
+            const float *table, int64_t table_rows, const int64_t *positions, void *q_out, void *k_out, void *stream);
+
+/* The same, with the rotated k and v written to the cache at slots[t] (page * page_size +
+ * offset) instead of k_out.  A negative slot: the token is not cached (padding).  A slot past
+ * the cache, or a bad position: not cached, device error word set.  Slots that are written must
+ * be distinct.  page_size: a power of two. */
+int ql_rope_append(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                   int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                   int64_t T, int Hq, int Hkv, int D, int rotary_dim, int layout, const float *table,
+                   int64_t table_rows, const int64_t *positions, const int64_t *slots, void *k_cache, void *v_cache,
+                   int64_t num_pages, int64_t page_stride, int page_size, void *q_out, void *stream);
+
+/* Attention of each sequence's new tokens over its paged cache (the new tokens' keys and
+ * values already appended): out = softmax(scale q k^T) v.  q [T, Hq, D] (strides given), out
+ * [T, Hq, D] contiguous; q head h reads kv head h / (Hq / Hkv).  Sequence b's tokens are
+ * q_starts[b] .. q_starts[b + 1] - 1 (q_starts [B + 1], covering 0 .. T), its cached positions
+ * 0 .. kv_lens[b] - 1, its pages page_table[b * table_stride ..].  Token i of q_len stands at
+ * p = kv_len - q_len + i and sees the positions j < kv_len, with causal j <= p, with window > 0
+ * (needs causal) j > p - window.  A token that sees nothing gets zeros.  max_q / max_kv: upper
+ * bounds of q_len / kv_len known to the host; a sequence beyond them, or a page index outside
+ * the cache, sets the device error word (its output is unspecified).  Entries of the page table
+ * and cache contents that no token of a sequence sees are not used.
+ * dtype bf16 or f16; D 64, 96, 128 or 256; page_size a power of two in [16, 1024]; fp32
+ * softmax, the weights rounded to dtype for the second product.  workspace: see below. */
+int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
+                       int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages,
+                       int64_t page_stride, int page_size, const int32_t *page_table, int64_t table_stride,
+                       const int32_t *q_starts, const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv,
+                       float scale, int causal, int64_t window, void *out, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/* Bytes of device workspace ql_paged_attention needs for these sizes (0: none). */
+size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv);
+
+/* Copies pages inside a pool: page dst[i] := page src[i] in each of `planes` planes (the keys or
+ * values of one layer), plane_stride bytes apart, pages page_stride bytes apart, page_bytes each
+ * (all multiples of 16).  src and dst are HOST arrays of n indices, read before the call
+ * returns.  Every index must be inside num_pages, no page twice a destination, no destination a
+ * source.  For a fork's copy on write and for compaction. */
+int ql_copy_pages(void *pool, int64_t planes, int64_t plane_stride, int64_t num_pages, int64_t page_stride,
+                  int64_t page_bytes, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
 
 #ifdef __cplusplus
 }

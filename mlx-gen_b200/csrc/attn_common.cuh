@@ -1,0 +1,149 @@
+// attn_common.cuh -- what the paged-attention kernels share: the parameter block, the view
+// of one sequence, the division of the work, and the join of partial results.
+//
+//     o_i = sum_j softmax_j(scale q_i . k_j) v_j   over the positions j that token i sees
+//
+// Token i of a sequence with q_len new tokens and kv_len cached positions (the new ones
+// included) stands at position p = kv_len - q_len + i; it sees j < kv_len, with `causal` only
+// j <= p, with a window only j > p - window.  A token that sees nothing gets zeros.
+//
+// The q heads of one kv head are packed: row r of a (sequence, kv head) is token r / G, head
+// r % G of the group (G = Hq / Hkv), so a group's heads read each key and value together.
+#pragma once
+
+#include "ql_common.cuh"
+
+namespace ql {
+namespace attn {
+
+constexpr int kSMs = 148;         // B200; used for planning only
+constexpr int ROWS_TILE = 16;     // rows of the small-row kernel (one m16 tile)
+constexpr float NEG_INF = -INFINITY;
+
+struct Params {
+    const void *q;
+    int64_t q_token, q_head;      // strides of q, elements
+    int64_t T;                    // tokens of all sequences
+    int Hq, Hkv, G;
+    const void *k_cache, *v_cache;  // [pages, Hkv, page_size, D], inner three contiguous
+    int64_t page_stride;          // elements between pages
+    int num_pages, page_shift;
+    const int32_t *table;         // [B, >= ceil(max_kv / page_size)]
+    int64_t table_stride;
+    const int32_t *q_starts, *kv_lens;
+    int max_q, max_kv;
+    float scale_log2;             // scale * log2(e)
+    int causal, window;
+    void *out;                    // [T, Hq, D]
+    float *part_o, *part_lse;     // [T * Hq, nsplit, D], [T * Hq, nsplit]; nsplit > 1 only
+    int nsplit, chunk;            // positions of one split (a multiple of 128)
+    int rows_kernel_most;         // sequences with up to so many rows go to the small-row kernel
+};
+
+struct Seq {
+    int q0, q_len, kv_len, ctx;
+    bool ok;
+};
+
+__device__ __forceinline__ Seq load_seq(const Params &p, int b) {
+    Seq s;
+    s.q0 = p.q_starts[b];
+    const int q1 = p.q_starts[b + 1];
+    s.kv_len = p.kv_lens[b];
+    s.q_len = q1 - s.q0;
+    s.ctx = s.kv_len - s.q_len;
+    // sizes that contradict what the launch was planned for: nothing is read or written
+    s.ok = s.q0 >= 0 && q1 >= s.q0 && q1 <= p.T && s.q_len <= p.max_q && s.kv_len >= 0 && s.kv_len <= p.max_kv;
+    return s;
+}
+
+// [lo, hi): the positions that token `tok` sees
+__device__ __forceinline__ void visible(const Params &p, const Seq &s, int tok, int &lo, int &hi) {
+    hi = p.causal ? min(s.kv_len, max(0, s.ctx + tok + 1)) : s.kv_len;
+    lo = p.window ? max(0, s.ctx + tok + 1 - p.window) : 0;
+}
+
+// The page that holds position pos; an index outside the cache is reported and reads page 0.
+__device__ __forceinline__ int page_of(const Params &p, int b, int pos) {
+    int pg = p.table[b * p.table_stride + (pos >> p.page_shift)];
+    if ((unsigned)pg >= (unsigned)p.num_pages) {
+        raise_dev_error(DEV_ERR_BAD_INDEX);
+        pg = 0;
+    }
+    return pg;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Joins the partial results of the splits: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max)
+// with each o_s normalised and lse_s in base 2.  A split that a row sees nothing of has lse
+// -inf and an unwritten o_s, which is not read.  One warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const float *part_o, const float *part_lse, int64_t rows, int nsplit,
+                                                   T *out) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31;
+    const float *lse = part_lse + row * nsplit;
+    float mx = NEG_INF;
+    for (int s = lane; s < nsplit; s += 32) mx = fmaxf(mx, lse[s]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    constexpr int PER = D / 32;
+    float acc[PER] = {}, total = 0.f;
+    if (mx != NEG_INF) {
+        for (int s = 0; s < nsplit; ++s) {
+            const float l = lse[s];
+            if (l == NEG_INF) continue;
+            const float w = ex2(l - mx);
+            total += w;
+            const float *o = part_o + (row * nsplit + s) * D;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] += w * o[e * 32 + lane];
+        }
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const uint32_t v = pack2<T>(acc[e] * inv, 0.f);
+        reinterpret_cast<uint16_t *>(out)[row * D + e * 32 + lane] = (uint16_t)v;
+    }
+}
+
+template <typename T, int D>
+static int launch_join(const Params &p, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    const int64_t rows = p.T * p.Hq;
+    cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, (const float *)p.part_o, (const float *)p.part_lse, rows,
+                                   p.nsplit, (T *)p.out));
+    return QL_OK;
+}
+
+}  // namespace attn
+}  // namespace ql

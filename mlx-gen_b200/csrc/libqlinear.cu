@@ -12,3 +12,9 @@
 #include "quantize.cu"
 #include "noalloc.cu"
 #include "modulate.cu"
+#include "norm_residual.cu"
+#include "rope.cu"
+#include "pages.cu"
+#include "attn_rows.cu"
+#include "attn_launch.cu"
+#include "api_decoder.cu"

@@ -1,0 +1,62 @@
+// pages.cu -- copies of whole pages inside a paged cache (a fork's copy on write, compaction).
+// dst[i] := src[i] in every plane (a plane: the keys or the values of one layer).
+//
+// Bound: HBM, one read and one write of each page.  The pairs travel in the kernel's
+// parameter block, so a call needs no upload and no device memory; no source is a
+// destination and no destination occurs twice (checked on the host), so the copies are
+// independent and their order does not matter.  Split: CTAs of 256 threads, each moving
+// 16 KB of one page (four 16-byte loads in flight per thread).
+#include <stdlib.h>
+#include <string.h>
+
+#include "ql_common.cuh"
+
+namespace ql {
+namespace pagesk {
+
+constexpr int MAX_PAIRS = 480;  // per launch: 3840 of the parameter block's 4096 bytes
+constexpr int THREADS = 256, UNROLL = 4;
+
+struct Pairs {
+    int src[MAX_PAIRS], dst[MAX_PAIRS];
+};
+
+__global__ void __launch_bounds__(THREADS) copy_pages_kernel(uint4 *pool, int64_t plane, int64_t page, int64_t words,
+                                                             const __grid_constant__ Pairs pr) {
+    // plane, page, words: 16-byte words between planes, between pages, of one page
+    uint4 *base = pool + (int64_t)blockIdx.z * plane;
+    const uint4 *s = base + pr.src[blockIdx.y] * page;
+    uint4 *d = base + pr.dst[blockIdx.y] * page;
+    const int64_t i0 = (int64_t)blockIdx.x * THREADS * UNROLL + threadIdx.x;
+    uint4 v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+        if (i0 + u * THREADS < words) v[u] = s[i0 + u * THREADS];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+        if (i0 + u * THREADS < words) d[i0 + u * THREADS] = v[u];
+}
+
+}  // namespace pagesk
+
+int launch_copy_pages(void *pool, int64_t planes, int64_t plane_stride, int64_t page_stride, int64_t page_bytes,
+                      const int32_t *src, const int32_t *dst, int64_t n, cudaStream_t st) {
+    using namespace pagesk;
+    const int64_t words = page_bytes / 16;
+    const unsigned gx = (unsigned)((words + THREADS * UNROLL - 1) / (THREADS * UNROLL));
+    for (int64_t z0 = 0; z0 < planes; z0 += 65535) {
+        const unsigned gz = (unsigned)(planes - z0 < 65535 ? planes - z0 : 65535);
+        for (int64_t i = 0; i < n; i += MAX_PAIRS) {
+            const int k = (int)(n - i < MAX_PAIRS ? n - i : MAX_PAIRS);
+            Pairs pr;
+            memcpy(pr.src, src + i, k * sizeof(int));
+            memcpy(pr.dst, dst + i, k * sizeof(int));
+            copy_pages_kernel<<<dim3(gx, k, gz), THREADS, 0, st>>>(
+                reinterpret_cast<uint4 *>(pool) + z0 * (plane_stride / 16), plane_stride / 16, page_stride / 16, words, pr);
+            QL_CUDA_TRY(cudaGetLastError());
+        }
+    }
+    return QL_OK;
+}
+
+}  // namespace ql

@@ -19,6 +19,7 @@ QL_OK, QL_EINVAL_SHAPE, QL_EUNSUPPORTED, QL_ECUDA, QL_EINVAL_ARG, QL_ETIMEOUT = 
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF, ACT_SWIGLU = range(4)
 (KERNEL_AUTO, KERNEL_GENERIC, KERNEL_GEMV, KERNEL_GEMM, KERNEL_GEMM_PAIR, KERNEL_GEMV_TC, KERNEL_GEMV_TMA,
  KERNEL_GEMV_REGS) = range(8)
+ROPE_HALF, ROPE_INTERLEAVED = range(2)
 
 STATUS_NAMES = {
     QL_OK: "QL_OK",
@@ -43,6 +44,12 @@ EXPORTS = (
     "ql_quantized_matmul_noalloc",
     "ql_debug_inject",
     "ql_matmul_workspace_size_x",
+    "ql_norm_residual",
+    "ql_rope",
+    "ql_rope_append",
+    "ql_paged_attention",
+    "ql_paged_attention_workspace_size",
+    "ql_copy_pages",
 )
 
 
@@ -110,6 +117,19 @@ def lib():
         L.ql_matmul_workspace_size.restype = C.c_size_t
         L.ql_matmul_workspace_size_x.argtypes = [i64, i64, i64, C.POINTER(Epilogue), i32]
         L.ql_matmul_workspace_size_x.restype = C.c_size_t
+        f32, sz = C.c_float, C.c_size_t
+        L.ql_norm_residual.argtypes = [vp, i32, i64, vp, i32, i64, i64, i64, vp, f32, vp, vp, i64, f32, vp, i64, f32,
+                                       vp, vp, vp]
+        L.ql_rope.argtypes = [vp, i64, i64, vp, i64, i64, i32, i64, i32, i32, i32, i32, i32, vp, i64, vp, vp, vp, vp]
+        L.ql_rope_append.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, i32, i32, i32, i32, i32, vp,
+                                     i64, vp, vp, vp, vp, i64, i64, i32, vp, vp]
+        L.ql_paged_attention.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i64, i64, i32, vp, i64, vp, vp,
+                                         i64, i64, i64, f32, i32, i64, vp, vp, sz, vp]
+        L.ql_paged_attention_workspace_size.argtypes = [i64, i32, i32, i32, i64, i64, i64]
+        L.ql_paged_attention_workspace_size.restype = sz
+        L.ql_copy_pages.argtypes = [vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]
+        for f in ("ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention", "ql_copy_pages"):
+            getattr(L, f).restype = i32
         for f in ("ql_quantize", "ql_dequantize", "ql_dequantize_rows", "ql_layernorm_modulate", "ql_quantized_matmul",
                   "ql_quantized_matmul_noalloc"):
             getattr(L, f).restype = i32

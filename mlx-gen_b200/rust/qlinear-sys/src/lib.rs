@@ -10,6 +10,8 @@
 //! - `ql_quantized_matmul`: `quantized_matmul(x, wq, scales, biases, true, gs, bits)` plus
 //!   bias in `LinearBase::forward` (src/adapters.rs:300-322) and the adapter residuals of
 //!   `AdaptableLinear::forward` (src/adapters.rs:543-549).
+//! - `ql_norm_residual`, `ql_rope`, `ql_rope_append`, `ql_paged_attention`, `ql_copy_pages`: the
+//!   decoder operators between the linears.
 //! - `ql_layernorm_modulate`: `fast::layer_norm` + `nn::modulate`
 //!   (mlx-gen-flux/src/transformer.rs:891-913, src/nn.rs:262-287).
 #![allow(non_camel_case_types)]
@@ -44,6 +46,10 @@ pub const QL_KERNEL_GEMM_PAIR: ql_kernel = 4;
 pub const QL_KERNEL_GEMV_TC: ql_kernel = 5;
 pub const QL_KERNEL_GEMV_TMA: ql_kernel = 6;
 pub const QL_KERNEL_GEMV_REGS: ql_kernel = 7;
+
+pub type ql_rope_layout = c_int;
+pub const QL_ROPE_HALF: ql_rope_layout = 0;
+pub const QL_ROPE_INTERLEAVED: ql_rope_layout = 1;
 
 /// Mirror of `ql_epilogue`: the ops fused into one `ql_quantized_matmul` call.  All
 /// pointers are device pointers; NULL turns the corresponding op off.
@@ -126,4 +132,30 @@ extern "C" {
                                        group_size: c_int, bits: c_int, transpose: c_int,
                                        ep: *const ql_epilogue, y: *mut c_void, y_dtype: c_int,
                                        stream: *mut c_void) -> c_int;
+    pub fn ql_norm_residual(y: *const c_void, y_dtype: c_int, y_stride: i64, residual: *const c_void, r_dtype: c_int,
+                            r_stride: i64, m: i64, d: i64, weight: *const c_void, weight_offset: f32,
+                            post_weight: *const c_void, gate: *const c_void, gate_period: i64, alpha: f32,
+                            scale: *const c_void, scale_period: i64, eps: f32, h: *mut c_void, r_out: *mut c_void,
+                            stream: *mut c_void) -> c_int;
+    pub fn ql_rope(q: *const c_void, q_token_stride: i64, q_head_stride: i64, k: *const c_void, k_token_stride: i64,
+                   k_head_stride: i64, dtype: c_int, t: i64, hq: c_int, hk: c_int, d: c_int, rotary_dim: c_int,
+                   layout: c_int, table: *const f32, table_rows: i64, positions: *const i64, q_out: *mut c_void,
+                   k_out: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn ql_rope_append(q: *const c_void, q_token_stride: i64, q_head_stride: i64, k: *const c_void,
+                          k_token_stride: i64, k_head_stride: i64, v: *const c_void, v_token_stride: i64,
+                          v_head_stride: i64, dtype: c_int, t: i64, hq: c_int, hkv: c_int, d: c_int,
+                          rotary_dim: c_int, layout: c_int, table: *const f32, table_rows: i64,
+                          positions: *const i64, slots: *const i64, k_cache: *mut c_void, v_cache: *mut c_void,
+                          num_pages: i64, page_stride: i64, page_size: c_int, q_out: *mut c_void,
+                          stream: *mut c_void) -> c_int;
+    pub fn ql_paged_attention(q: *const c_void, dtype: c_int, q_token_stride: i64, q_head_stride: i64, t: i64,
+                              hq: c_int, hkv: c_int, d: c_int, k_cache: *const c_void, v_cache: *const c_void,
+                              num_pages: i64, page_stride: i64, page_size: c_int, page_table: *const i32,
+                              table_stride: i64, q_starts: *const i32, kv_lens: *const i32, b: i64, max_q: i64,
+                              max_kv: i64, scale: f32, causal: c_int, window: i64, out: *mut c_void,
+                              workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ql_paged_attention_workspace_size(t: i64, hq: c_int, hkv: c_int, d: c_int, b: i64, max_q: i64,
+                                             max_kv: i64) -> usize;
+    pub fn ql_copy_pages(pool: *mut c_void, planes: i64, plane_stride: i64, num_pages: i64, page_stride: i64,
+                         page_bytes: i64, src: *const i32, dst: *const i32, n: i64, stream: *mut c_void) -> c_int;
 }
