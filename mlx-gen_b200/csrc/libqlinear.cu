@@ -16,5 +16,6 @@
 #include "rope.cu"
 #include "pages.cu"
 #include "attn_rows.cu"
+#include "attn_sm100.cu"
 #include "attn_launch.cu"
 #include "api_decoder.cu"

@@ -482,6 +482,23 @@ def test_attention_refusals(dev):
         call(q=q.float(), k=kc.float(), v=vc.float())
 
 
+@pytest.mark.parametrize("q_len,kv", [(200, 1500), (30, 100)])
+def test_attention_wait_runs_out_and_reports(q_len, kv):
+    """With a loader that issues nothing (a flag that only this sets) and the wait limit at 50 ms,
+    the launch ends by itself, the timeout is reported, and the next call is right."""
+    g = gen(9)
+    q, kc, vc, table, starts, lens = paged(g, [q_len], [kv], 6, 2, 128, 16, BF)
+    assert qlinear.device_error() == 0
+    try:
+        _lib.debug_inject(_lib.INJECT_ATTENTION_PRODUCER_SILENT, 50_000_000)
+        qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=q_len, max_kv=kv)
+        err = qlinear.device_error()
+    finally:
+        _lib.debug_inject(0, 0)
+    assert err & (_lib.DEV_ERR_TIMEOUT_FULL | _lib.DEV_ERR_TIMEOUT_EMPTY | _lib.DEV_ERR_TIMEOUT_ACC)
+    check_attention(gen(10), [q_len], [kv], 6, 2, 128)
+
+
 # ------------------------------------------------------------------------ pages
 
 @pytest.mark.parametrize("shape", [(9, 2, 16, 64), (3, 2, 40, 1, 16, 8), (1, 12, 3, 128, 256), (70000, 3, 1, 8, 1)])
