@@ -8,59 +8,43 @@ ValueError or TypeError here; a QlError comes from the library's own checks.
 """
 from __future__ import annotations
 
-import ctypes as C
+import ctypes
 import math
+import os
 from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import ROPE_HALF, ROPE_INTERLEAVED, check, lib
+from ._lib import ROPE_HALF, ROPE_INTERLEAVED, lib
 
-_DT = {torch.float32: _lib.QL_F32, torch.bfloat16: _lib.QL_BF16, torch.float16: _lib.QL_F16}
 _LAYOUTS = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
 
 
-def _dtype(t: torch.Tensor) -> int:
-    code = _DT.get(t.dtype)
-    if code is None:
-        raise TypeError(f"unsupported dtype {t.dtype}; expected float32, bfloat16 or float16")
-    return code
+class _Native:
+    """qlinear._native (csrc/native.cpp), loaded and given libqlinear's functions on first use."""
+
+    def __getattr__(self, name):
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_native.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} not found; build it first (python -c 'import __graft_entry__ as g; g.build()')")
+        from . import _native as m
+        L = lib()
+        m.init(_lib.QlError, *(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
+            "ql_last_error", "ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention",
+            "ql_paged_attention_workspace_size", "ql_copy_pages")))
+        for f in ("norm_residual", "rope", "rope_append", "paged_attention", "copy_pages"):
+            setattr(self, f, getattr(m, f))
+        return self.__dict__[name]
 
 
-def _call(device: torch.device, fn, *args) -> None:
-    """One library call on `device`'s current stream."""
-    i = device.index
-    if i != torch.cuda.current_device():
-        with torch.cuda.device(i):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
-    else:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(i)))
+_native = _Native()
 
 
-def _on(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
-def _cuda(t: torch.Tensor) -> torch.device:
-    if not t.is_cuda:
-        raise ValueError("libqlinear operates on CUDA tensors only")
-    return t.device
-
-
-def _row(name: str, t: Optional[torch.Tensor], like: torch.Tensor, D: int, rows: int = 1) -> int:
-    """Pointer of a contiguous [rows.., D] operand in `like`'s dtype (0: absent)."""
-    if t is None:
-        return 0
-    if t.dtype != like.dtype or t.device != like.device:
-        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if t.shape[-1] != D or t.numel() < rows * D:
-        raise ValueError(f"{name} must hold {rows} row(s) of {D} elements, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+def _layout(name: str) -> int:
+    if name not in _LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {name!r}")
+    return _LAYOUTS[name]
 
 
 # ------------------------------------------------------------------------ residual norm
@@ -80,31 +64,8 @@ def norm_residual(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     gate / scale ``[D]`` or ``[rows, D]`` with row ``m // period`` for row m of y.  The DiT blocks'
     ``residual + gate * norm(branch)`` is post_weight and gate (src/nn.rs:166-176 for the gated
     sum); a decoder layer uses neither."""
-    device = _cuda(y)
-    D = y.shape[-1]
-    if residual.shape != y.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} must have y's shape {tuple(y.shape)}")
-    if residual.device != device:
-        raise ValueError(f"residual is on {residual.device}, expected {device}")
-    ydt, rdt = _dtype(y), _dtype(residual)
-    M = y.numel() // D if D else 0
-    y2 = y if y.dim() == 2 else y.reshape(-1, D)
-    r2 = residual if residual.dim() == 2 else residual.reshape(-1, D)
-    ys, rs = y2.stride(0), r2.stride(0)
-    if y2.stride(1) != 1 or (M > 1 and ys < D):
-        y2 = y2.contiguous()
-        ys = D
-    if r2.stride(1) != 1 or (M > 1 and rs < D):
-        r2 = r2.contiguous()
-        rs = D
-    rows = lambda period: -(-M // period) if period > 0 else 1  # noqa: E731
-    h = torch.empty(y.shape, dtype=y.dtype, device=device)
-    r = torch.empty(y.shape, dtype=residual.dtype, device=device)
-    _call(device, lib().ql_norm_residual, y2.data_ptr(), ydt, max(ys, D), r2.data_ptr(), rdt, max(rs, D), M, D,
-          _row("weight", weight, y, D), weight_offset, _row("post_weight", post_weight, y, D),
-          _row("gate", gate, y, D, rows(gate_period)), gate_period, alpha,
-          _row("scale", scale, y, D, rows(scale_period)), scale_period, eps, h.data_ptr(), r.data_ptr())
-    return h, r
+    return _native.norm_residual(y, residual, weight, post_weight, gate, gate_period, alpha, scale, scale_period, eps,
+                                 weight_offset)
 
 
 # ------------------------------------------------------------------------ rotary positions
@@ -190,60 +151,13 @@ def rope_table(rotary_dim: int, positions, base: float = 10000.0, scaling: Optio
     return torch.cat([angles.cos() * magnitude, angles.sin() * magnitude], 1).float().to(device)
 
 
-def _heads(name: str, x: torch.Tensor, T: int, D: int, like: torch.Tensor) -> torch.Tensor:
-    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D:
-        raise ValueError(f"{name} must be [{T}, heads, {D}], got {tuple(x.shape)}")
-    if x.dtype != like.dtype or x.device != like.device:
-        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {x.dtype} on {x.device}")
-    return x if x.stride(2) == 1 else x.contiguous()
-
-
-def _rope_args(q, table, positions, layout):
-    device = _cuda(q)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
-    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
-        raise ValueError("table must be a contiguous float32 [positions, rotary_dim] (see rope_table)")
-    if positions.dtype != torch.int64 or positions.shape != q.shape[:1] or not positions.is_contiguous():
-        raise ValueError("positions must be a contiguous int64 [tokens]")
-    _on(device, table=table, positions=positions)
-    if layout not in _LAYOUTS:
-        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-    return device, _LAYOUTS[layout]
-
-
 def rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, *,
          layout: str = "half") -> Tuple[torch.Tensor, torch.Tensor]:
     """Rotary positions on q ``[T, Hq, D]`` and k ``[T, Hk, D]`` (views with any token and head
     stride); returns new contiguous tensors.  The table's width is the rotary dimension (the rest
     of each head is copied); ``positions [T]`` (int64) are its rows.  layout "half" pairs (i, i +
     rotary_dim / 2), "interleaved" (2i, 2i + 1)."""
-    device, lay = _rope_args(q, table, positions, layout)
-    T, Hq, D = q.shape
-    q = _heads("q", q, T, D, q)
-    k = _heads("k", k, T, D, q)
-    Hk = k.shape[1]
-    qo = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-    ko = torch.empty((T, Hk, D), dtype=q.dtype, device=device)
-    _call(device, lib().ql_rope, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-          _dtype(q), T, Hq, Hk, D, table.shape[1], lay, table.data_ptr(), table.shape[0], positions.data_ptr(),
-          qo.data_ptr(), ko.data_ptr())
-    return qo, ko
-
-
-def _cache_shape(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor):
-    """(pages, heads, page size, head dim, page stride) of a layer's two caches."""
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.dtype != like.dtype or c.device != like.device:
-            raise ValueError(f"{name} must be [pages, heads, page_size, head_dim] in {like.dtype} on {like.device}, got "
-                             f"{tuple(c.shape)} {c.dtype} on {c.device}")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
-        raise ValueError("k_cache and v_cache must have the same shape and strides")
-    P, H, ps, D = k_cache.shape
-    sp, sh, st, sd = k_cache.stride()
-    if sd != 1 or st != D or (H > 1 and sh != ps * D) or (P > 1 and sp < H * ps * D):
-        raise ValueError("the [heads, page_size, head_dim] of a page must be contiguous")
-    return P, H, ps, D, sp if P > 1 else H * ps * D
+    return _native.rope(q, k, table, positions, _layout(layout))
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
@@ -251,21 +165,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
                 layout: str = "half") -> torch.Tensor:
     """``rope`` with the rotated k and v written to the paged cache ``[pages, Hkv, page_size, D]`` at
     ``slots [T]`` (int64, page * page_size + offset; negative: not cached); returns the rotated q."""
-    device, lay = _rope_args(q, table, positions, layout)
-    T, Hq, D = q.shape
-    q = _heads("q", q, T, D, q)
-    k, v = _heads("k", k, T, D, q), _heads("v", v, T, D, q)
-    P, H, ps, cd, stride = _cache_shape(k_cache, v_cache, q)
-    if k.shape[1] != H or v.shape[1] != H or cd != D:
-        raise ValueError(f"k and v must have the cache's {H} heads of {cd}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    if slots.dtype != torch.int64 or slots.shape != positions.shape or not slots.is_contiguous() or slots.device != device:
-        raise ValueError(f"slots must be a contiguous int64 [tokens] on {device}")
-    qo = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-    _call(device, lib().ql_rope_append, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-          v.data_ptr(), v.stride(0), v.stride(1), _dtype(q), T, Hq, H, D, table.shape[1], lay, table.data_ptr(),
-          table.shape[0], positions.data_ptr(), slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), P, stride, ps,
-          qo.data_ptr())
-    return qo
+    return _native.rope_append(q, k, v, table, positions, k_cache, v_cache, slots, _layout(layout))
 
 
 # ------------------------------------------------------------------------ paged attention
@@ -287,38 +187,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     captured with).  scale: ``1 / sqrt(D)`` by default.  Token i of q_len stands at ``p = kv_len -
     q_len + i`` and sees the positions up to p (all, without ``causal``), with a window only the
     last ``window`` of them.  Returns ``[T, Hq, D]``; a token that sees nothing gets zeros."""
-    device = _cuda(q)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
-    T, Hq, D = q.shape
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-    P, Hkv, ps, cd, stride = _cache_shape(k_cache, v_cache, q)
-    if cd != D:
-        raise ValueError(f"q's head dimension {D} differs from the cache's {cd}")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if (B < 0 or page_table.dim() != 2 or page_table.shape[0] != B or q_starts.shape != (B + 1,)):
-        raise ValueError("expected kv_lens [B], q_starts [B + 1] and page_table [B, pages], got "
-                         f"{tuple(kv_lens.shape)}, {tuple(q_starts.shape)}, {tuple(page_table.shape)}")
-    for name, t in (("page_table", page_table), ("q_starts", q_starts), ("kv_lens", kv_lens)):
-        if t.dtype != torch.int32 or t.device != device or (t.numel() and t.stride(-1) != 1):
-            raise ValueError(f"{name} must be int32 on {device} with a contiguous last axis")
-    if page_table.shape[1] * ps < max_kv:
-        raise ValueError(f"page_table's {page_table.shape[1]} pages of {ps} do not hold max_kv={max_kv} positions")
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape, dtype and device")
-    L = lib()
-    need = L.ql_paged_attention_workspace_size(T, Hq, Hkv, D, B, max_q, max_kv)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(device, L.ql_paged_attention, q.data_ptr(), _dtype(q), q.stride(0), q.stride(1), T, Hq, Hkv, D,
-          k_cache.data_ptr(), v_cache.data_ptr(), P, stride, ps, page_table.data_ptr(),
-          page_table.stride(0) if B > 1 else page_table.shape[1], q_starts.data_ptr(), kv_lens.data_ptr(), B, max_q, max_kv,
-          1.0 / math.sqrt(D) if scale is None else scale, causal, window, out.data_ptr(),
-          workspace.data_ptr() if need else 0, need)
-    return out
+    return _native.paged_attention(q, k_cache, v_cache, page_table, q_starts, kv_lens, max_q, max_kv, scale, causal, window,
+                                   out, workspace)
 
 
 # ------------------------------------------------------------------------ pages
@@ -327,17 +197,4 @@ def copy_pages(pool: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> No
     """Page ``dst[i] := src[i]`` in every plane of a pool ``[..., pages, heads, page_size, head_dim]``
     (leading axes: layers, keys and values).  src and dst are host sequences; every page may be a
     destination once and no destination may be a source."""
-    device = _cuda(pool)
-    if pool.dim() < 4 or not pool.is_contiguous():
-        raise ValueError("pool must be a contiguous [.., pages, heads, page_size, head_dim]")
-    n = len(src)
-    if len(dst) != n:
-        raise ValueError(f"{n} sources for {len(dst)} destinations")
-    pages = pool.shape[-4]
-    if any(not -0x80000000 <= i <= 0x7fffffff for x in (src, dst) for i in (min(x, default=0), max(x, default=0))):
-        raise ValueError("page index out of range")
-    arr = C.c_int32 * n
-    page_bytes = pool.shape[-3] * pool.shape[-2] * pool.shape[-1] * pool.element_size()
-    planes = pool.numel() * pool.element_size() // (pages * page_bytes) if pages and page_bytes else 0
-    _call(device, lib().ql_copy_pages, pool.data_ptr(), planes, pages * page_bytes, pages, page_bytes, page_bytes,
-          arr(*src), arr(*dst), n)
+    _native.copy_pages(pool, src, dst)
