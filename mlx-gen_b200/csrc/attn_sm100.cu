@@ -42,7 +42,7 @@ struct Sm100Cfg {
     static constexpr int STAGES = D == 128 ? 5 : 8;
     static constexpr int SMEM_Q = 0, SMEM_KV = 2 * TILE_BYTES;
     static constexpr int SMEM_BAR = SMEM_KV + STAGES * TILE_BYTES;
-    static constexpr int NBAR = 2 * STAGES + 2 * 6 + 2;
+    static constexpr int NBAR = 2 * STAGES + 2 * 7 + 2;
     static constexpr int SMEM = SMEM_BAR + NBAR * 8 + 16 + 1024;
 };
 
@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint64_t *pfull = sfull + 2;       // [2][2] halves of P_t written
     uint64_t *ofull = pfull + 4;       // [2] O_t complete
     uint64_t *drain = ofull + 2;       // [2] an aborted tile's MMAs are done
-    uint64_t *vfix = drain + 2;        // [2] V of the first / last step cleared outside [vlo, vhi)
+    uint64_t *turn = drain + 2;        // [2] the other tile's exponentials of the step are done
+    uint64_t *vfix = turn + 2;         // [2] V of the first / last step cleared outside [vlo, vhi)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             mbar_init(&pfull[2 * t + 1], 4);
             mbar_init(&ofull[t], 1);
             mbar_init(&drain[t], 1);
+            mbar_init(&turn[t], 4);
             mbar_init(&vfix[t], 1);
         }
         *abort_flag = 0;
@@ -212,15 +214,20 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 for (int i = 0; i < TKV / 32; ++i) tmem_ld32(s_col + i * 32, reinterpret_cast<uint32_t *>(sc) + i * 32);
                 tmem_ld_wait();
                 const int kv0 = (t0 + j) * TKV;
-                if (kv0 < max_lo || kv0 + TKV > min_hi || r >= rows) {
+                // a step that some row of the tile does not see whole (the same for all its threads)
+                if (kv0 < max_lo || kv0 + TKV > min_hi) {
                     const int a = rlo - kv0, e = rhi - kv0;
 #pragma unroll
                     for (int i = 0; i < TKV; ++i) sc[i] = (i >= a && i < e) ? sc[i] : NEG_INF;
                 }
                 float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-                for (int i = 4; i < TKV; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[i]);
-                const float nm = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+                for (int i = 4; i < 124; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], sc[i + 2 * k], sc[i + 2 * k + 1]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], sc[124 + k]);
+                const float nm = max3(max3(mx[0], mx[1], mx[2]), mx[3], m);
                 const bool grow = (nm - m) * c > 8.f;  // also from -inf; false while nothing is seen (nan)
                 if (__any_sync(0xffffffffu, grow)) {
                     const float f = grow ? ex2((m - nm) * c) : 1.f;
@@ -239,15 +246,22 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     }
                 }
                 const float base = m == NEG_INF ? 0.f : m * c;
-                float sum[2] = {0.f, 0.f};
+                // the tiles take turns: tile 1 follows tile 0's step, tile 0 tile 1's step before
+                if (ntiles == 2 && (t == 1 || j > 0)) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&turn[t], (t == 1 ? j : j - 1) & 1, abort_flag, DEV_ERR_TIMEOUT_ACC));
+                    if (!ok) break;
+                }
+                const uint64_t c2 = f2_make(c, c), nb2 = f2_make(-base, -base);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pk[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float x = ex2(fmaf(sc[h * 64 + 2 * i], c, -base)), y = ex2(fmaf(sc[h * 64 + 2 * i + 1], c, -base));
-                        sum[0] += x;
-                        sum[1] += y;
+                        float x, y;
+                        f2_split(f2_fma(f2_make(sc[h * 64 + 2 * i], sc[h * 64 + 2 * i + 1]), c2, nb2), x, y);
+                        x = ex2(x), y = ex2(y);
+                        sum[i & 1] = f2_add(sum[i & 1], f2_make(x, y));
                         pk[i] = pack2<T>(x, y);
                     }
                     tmem_st32(s_col + h * 32, pk);
@@ -256,7 +270,10 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&pfull[2 * t + h]);
                 }
-                l += sum[0] + sum[1];
+                if (lane == 0 && ntiles == 2) mbar_arrive(&turn[t ^ 1]);
+                float sx, sy;
+                f2_split(f2_add(sum[0], sum[1]), sx, sy);
+                l += sx + sy;
             }
             // ------------------------------------------------------------ epilogue of tile t
             if (ok && __all_sync(0xffffffffu, mbar_wait(&ofull[t], 0, abort_flag, DEV_ERR_TIMEOUT_ACC))) {
