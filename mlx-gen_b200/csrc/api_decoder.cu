@@ -18,6 +18,7 @@ int launch_paged_attention(attn::Params &, int, int, int64_t, void *, cudaStream
 
 static int elem_bytes(int dt) { return dt == QL_F32 ? 4 : 2; }
 static bool elem_aligned(const void *p, int dt) { return (reinterpret_cast<uintptr_t>(p) % elem_bytes(dt)) == 0; }
+static bool aligned32(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 static bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 static int log2i(int64_t v) {
     int s = 0;
@@ -160,12 +161,12 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
     if (T == 0 || B == 0 || max_q == 0) return QL_OK;
     if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
         return fail(QL_EINVAL_ARG, "ql_paged_attention: NULL pointer");
-    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || q_token_stride % 8 ||
+    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned32(out) || q_token_stride % 8 ||
         q_head_stride % 8)
-        return fail(QL_EINVAL_ARG, "q, the caches and out must be 16-byte aligned, q's strides multiples of 8");
+        return fail(QL_EINVAL_ARG, "q and the caches must be 16-byte aligned, out 32-byte, q's strides multiples of 8");
     const size_t need = paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv);
-    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-        return fail(QL_EINVAL_ARG, "ql_paged_attention needs a 16-byte aligned workspace of %zu bytes (got %zu)", need,
+    if (need && (!workspace || workspace_bytes < need || !aligned32(workspace)))
+        return fail(QL_EINVAL_ARG, "ql_paged_attention needs a 32-byte aligned workspace of %zu bytes (got %zu)", need,
                     workspace_bytes);
     ql::attn::Params p{};
     p.q = q, p.q_token = q_token_stride, p.q_head = q_head_stride, p.T = T;

@@ -65,6 +65,13 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 
+// 32 bytes in one store: a whole DRAM sector of a thread's own row
+__device__ __forceinline__ void st_global_32(void *dst, const uint32_t v[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // V as stored is [position][element]: for O = P V its N axis (elements) is the contiguous one.
 // Swizzled MN-major operand: 64-element atoms along N are HALF_BYTES apart (leading offset),
 // groups of 8 positions 1024 bytes apart (stride offset).
@@ -167,20 +174,22 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             // ------------------------------------------------------------ softmax of tile t
             const int tid = threadIdx.x & 127;  // == row of the tile == TMEM lane
             {
-                // Q_t, 16 bytes a lane, rows past the end as zeros
-                constexpr int CPR = D / 8;
-                uint8_t *qs = smem + C::SMEM_Q + t * C::TILE_BYTES;
-#pragma unroll 4
+                // Q_t by asynchronous copies of 16 bytes, rows past the end as zeros; a thread's rows
+                // are 128 / CPR apart, so token and head advance without a division
+                constexpr int CPR = D / 8, STEP = 128 / CPR;
+                const uint32_t qs = smem_u32(smem + C::SMEM_Q + t * C::TILE_BYTES);
+                const int c = tid % CPR, step_tok = STEP / p.G, step_g = STEP % p.G;
+                int rr = tid / CPR, gr = row0 + t * TQ + rr, tok = gr / p.G, g = gr % p.G;
+#pragma unroll
                 for (int i = 0; i < CPR; ++i) {
-                    const int idx = i * 128 + tid, r = idx / CPR, c = idx % CPR, gr = row0 + t * TQ + r;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (gr < rows) {
-                        const int tok = gr / p.G, hd = kvh * p.G + gr % p.G;
-                        v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p.q) +
-                                                             (s.q0 + (int64_t)tok) * p.q_token + hd * p.q_head + c * 8);
-                    }
-                    *reinterpret_cast<uint4 *>(qs + (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                    const bool in = gr < rows;
+                    const uint16_t *src = reinterpret_cast<const uint16_t *>(p.q) +
+                                          (in ? (s.q0 + (int64_t)tok) * p.q_token + (kvh * p.G + g) * p.q_head + c * 8 : 0);
+                    cp_async16(qs + (c >> 3) * C::HALF_BYTES + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src, in);
+                    rr += STEP, gr += STEP, tok += step_tok, g += step_g;
+                    if (g >= p.G) g -= p.G, ++tok;
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&qfull[t]);
             }
@@ -289,23 +298,21 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     tmem_ld32(o_col + i * 32, o);
                     tmem_ld_wait();
                     if (p.nsplit > 1) {
-                        float4 *dst = reinterpret_cast<float4 *>(p.part_o + (row * p.nsplit + split) * D) + i * 8;
+                        float *dst = p.part_o + (row * p.nsplit + split) * D + i * 32;
                         if (seen && r < rows) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                                     __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) st_global_32(dst + e, o + e);
                         }
                     } else if (r < rows) {  // (a row that saw nothing has O = 0 and inv = 0)
-                        uint4 *dst = reinterpret_cast<uint4 *>(p.out) + row * (D / 8) + i * 4;
+                        uint32_t w[16];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = pack2<T>(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
-                            dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int e = 0; e < 16; ++e)
+                            w[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                        uint16_t *dst = reinterpret_cast<uint16_t *>(p.out) + row * D + i * 32;
+                        st_global_32(dst, w);
+                        st_global_32(dst + 16, w + 8);
                     }
                     __syncwarp();
                 }
