@@ -31,6 +31,7 @@ namespace ql {
 namespace attn {
 
 constexpr int TQ = 128, TKV = 128;
+constexpr int PFIRST = 96;  // positions of P_t handed over first: O_t's product starts under the last weights
 constexpr int SM100_THREADS = 384;
 constexpr int SM100_ROWS = 2 * TQ;  // rows of a CTA
 
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint64_t *empty = full + STAGES;   // stage read by every tile's MMAs
     uint64_t *qfull = empty + STAGES;  // [2] Q_t written
     uint64_t *sfull = qfull + 2;       // [2] S_t of the step computed (and O_t of the step before)
-    uint64_t *pfull = sfull + 2;       // [2][2] halves of P_t written
+    uint64_t *pfull = sfull + 2;       // [2][2] P_t written: its first PFIRST positions, the rest
     uint64_t *ofull = pfull + 4;       // [2] O_t complete
     uint64_t *drain = ofull + 2;       // [2] an aborted tile's MMAs are done
     uint64_t *turn = drain + 2;        // [2] the other tile's exponentials of the step are done
@@ -263,17 +264,21 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 const uint64_t c2 = f2_make(c, c), nb2 = f2_make(-base, -base);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t pk[32];
+                for (int h = 0; h < 2; ++h) {  // the first PFIRST positions, then the rest
+                    const int from = h ? PFIRST : 0, to = h ? TKV : PFIRST;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float x, y;
-                        f2_split(f2_fma(f2_make(sc[h * 64 + 2 * i], sc[h * 64 + 2 * i + 1]), c2, nb2), x, y);
-                        x = ex2(x), y = ex2(y);
-                        sum[i & 1] = f2_add(sum[i & 1], f2_make(x, y));
-                        pk[i] = pack2<T>(x, y);
+                    for (int q = from; q < to; q += 32) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float x, y;
+                            f2_split(f2_fma(f2_make(sc[q + 2 * i], sc[q + 2 * i + 1]), c2, nb2), x, y);
+                            x = ex2(x), y = ex2(y);
+                            sum[i & 1] = f2_add(sum[i & 1], f2_make(x, y));
+                            pk[i] = pack2<T>(x, y);
+                        }
+                        tmem_st16(s_col + q / 2, pk);
                     }
-                    tmem_st32(s_col + h * 32, pk);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int k = 4 * h; k < 4 * h + 4; ++k)
+                    for (int k = h ? PFIRST / 16 : 0; k < (h ? TKV : PFIRST) / 16; ++k)
                         tc_mma_ts(o_col, s_col + k * 8, umma_desc_mn_sw128(vs + k * 2048, C::HALF_BYTES), pv, (j | k) != 0);
                 }
                 if (!ok) break;

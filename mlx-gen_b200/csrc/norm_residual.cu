@@ -10,6 +10,8 @@
 // Split: one CTA per row; a thread owns NCH chunks of VEC consecutive elements, so the row
 // is held in registers whatever D is (up to 32 elements for each of 1024 threads).  The two
 // sums of squares are block reductions.
+#include <string.h>
+
 #include "ql_common.cuh"
 
 namespace ql {
@@ -29,6 +31,24 @@ __device__ __forceinline__ void from_f(float &d, float v) { d = v; }
 __device__ __forceinline__ void from_f(__nv_bfloat16 &d, float v) { d = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f(__half &d, float v) { d = __float2half_rn(v); }
 
+// v[e] = x[e] rounded to T (two at a time where T is 16 bits wide)
+template <typename T, int V>
+__device__ __forceinline__ void round_to_pack(Pack<T, V> &o, const float (&x)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+            if constexpr (__is_same(T, __half))
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(x[2 * e + 1]), "f"(x[2 * e]));
+            else w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+        }
+        memcpy(&o, w, sizeof(o));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) from_f(o.v[e], x[e]);
+    }
+}
+
 struct Params {
     const void *y, *residual;
     int64_t y_stride, r_stride;  // elements between rows
@@ -39,12 +59,14 @@ struct Params {
     void *h, *r_out;
 };
 
-// Sum over the block; `red` holds one float per warp and is not reused within a row.
-__device__ __forceinline__ float block_sum(float v, float *red) {
+// Sum over the threads of a row (a warp or the block); `red` holds one float per warp and is
+// not reused within a row.
+template <bool WARP_ROW>
+__device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (WARP_ROW) return v;
     const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (nw == 1) return v;
     if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = lane < nw ? red[lane] : 0.f;
@@ -53,12 +75,14 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return v;
 }
 
-template <typename Y, typename R, int VEC, int NCH>
-__global__ void __launch_bounds__(1024) norm_residual_kernel(const Params p) {
+template <typename Y, typename R, int VEC, int NCH, bool WARP_ROW>
+__global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_residual_kernel(const Params p, int64_t M) {
     __shared__ float red[2][32];
     using PY = Pack<Y, VEC>;
     using PR = Pack<R, VEC>;
-    const int64_t m = blockIdx.x;
+    const int nt = WARP_ROW ? 32 : blockDim.x, tid = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t m = WARP_ROW ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP_ROW && m >= M) return;
     const int n = p.D / VEC;
     const PY *yp = reinterpret_cast<const PY *>(reinterpret_cast<const Y *>(p.y) + m * p.y_stride);
     const PR *rp = reinterpret_cast<const PR *>(reinterpret_cast<const R *>(p.residual) + m * p.r_stride);
@@ -73,89 +97,105 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(const Params p) {
     PR rv[NCH];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int i = c * blockDim.x + threadIdx.x;
+        const int i = c * nt + tid;
         if (i < n) {
             yv[c] = yp[i];
             rv[c] = rp[i];
         }
     }
-    float inv_post = 1.f;
+    // the sums first touch, then the weights: their loads overlap the reductions
+    float post_factor = p.alpha;  // of y: alpha, and 1 / rms(y) with a post norm
     if (postp) {
         float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
-            if (c * blockDim.x + threadIdx.x < n)
+            if (c * nt + tid < n)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) ss += to_f(yv[c].v[e]) * to_f(yv[c].v[e]);
-        inv_post = rsqrtf(block_sum(ss, red[0]) * p.inv_d + p.eps);
+        post_factor *= rsqrtf(row_sum<WARP_ROW>(ss, red[0]) * p.inv_d + p.eps);
     }
     float r[NCH][VEC], ss = 0.f;
     PR *ro = reinterpret_cast<PR *>(reinterpret_cast<R *>(p.r_out) + m * p.D);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int i = c * blockDim.x + threadIdx.x;
+        const int i = c * nt + tid;
         if (i >= n) continue;
         float u[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) u[e] = to_f(yv[c].v[e]);
+        for (int e = 0; e < VEC; ++e) u[e] = to_f(yv[c].v[e]) * post_factor;
         if (postp) {
             const PY w = postp[i];
+            if (p.offset != 0.f) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) u[e] = u[e] * inv_post * (p.offset + to_f(w.v[e]));
+                for (int e = 0; e < VEC; ++e) u[e] *= p.offset + to_f(w.v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) u[e] *= to_f(w.v[e]);
+            }
         }
         if (gp) {
             const PY g = gp[i];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) u[e] *= to_f(g.v[e]);
-        }
-        PR o;
+            for (int e = 0; e < VEC; ++e) r[c][e] = fmaf(u[e], to_f(g.v[e]), to_f(rv[c].v[e]));
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            r[c][e] = fmaf(p.alpha, u[e], to_f(rv[c].v[e]));
-            ss += r[c][e] * r[c][e];
-            from_f(o.v[e], r[c][e]);
+            for (int e = 0; e < VEC; ++e) r[c][e] = u[e] + to_f(rv[c].v[e]);
         }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) ss += r[c][e] * r[c][e];
+        PR o;
+        round_to_pack(o, r[c]);
         ro[i] = o;
     }
-    const float inv = rsqrtf(block_sum(ss, red[1]) * p.inv_d + p.eps);
+    const float inv = rsqrtf(row_sum<WARP_ROW>(ss, red[1]) * p.inv_d + p.eps);
     PY *ho = reinterpret_cast<PY *>(reinterpret_cast<Y *>(p.h) + m * p.D);
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const int i = c * blockDim.x + threadIdx.x;
+        const int i = c * nt + tid;
         if (i >= n) continue;
         const PY w = wp[i];
-        PY o;
-        float f[VEC];
+        if (p.offset != 0.f) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = inv * (p.offset + to_f(w.v[e]));
+            for (int e = 0; e < VEC; ++e) r[c][e] *= inv * (p.offset + to_f(w.v[e]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) r[c][e] *= inv * to_f(w.v[e]);
+        }
         if (sp) {
             const PY s = sp[i];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] *= 1.f + to_f(s.v[e]);
+            for (int e = 0; e < VEC; ++e) r[c][e] = fmaf(r[c][e], to_f(s.v[e]), r[c][e]);
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) from_f(o.v[e], r[c][e] * f[e]);
+        PY o;
+        round_to_pack(o, r[c]);
         ho[i] = o;
     }
+}
+
+template <typename Y, typename R, int VEC, int NCH>
+static void launch_n(const Params &p, int64_t M, int nt, cudaStream_t st) {
+    if (NCH == 1 && nt == 32) norm_residual_kernel<Y, R, VEC, 1, true><<<(unsigned)((M + 7) / 8), 256, 0, st>>>(p, M);
+    else norm_residual_kernel<Y, R, VEC, NCH, false><<<(unsigned)M, nt, 0, st>>>(p, M);
 }
 
 template <typename Y, typename R, int VEC>
 static int launch(const Params &p, int64_t M, cudaStream_t st) {
     const int n = p.D / VEC;  // vectors of a row
-    // chunks of a thread: the fewest that a block of 1024 threads needs
+    // chunks of a thread: the fewest that a block of 1024 threads needs.  Rows of one warp's
+    // width (up to 32 vectors) run eight to a CTA.
     constexpr int MAXC = 32 / VEC;
     int nch = 1;
     while (nch < MAXC && (int64_t)nch * 1024 < n) nch *= 2;
     const int nt = ((n + nch - 1) / nch + 31) / 32 * 32;
     switch (nch) {
-        case 1: norm_residual_kernel<Y, R, VEC, 1><<<(unsigned)M, nt, 0, st>>>(p); break;
-        case 2: norm_residual_kernel<Y, R, VEC, 2><<<(unsigned)M, nt, 0, st>>>(p); break;
-        case 4: norm_residual_kernel<Y, R, VEC, 4><<<(unsigned)M, nt, 0, st>>>(p); break;
+        case 1: launch_n<Y, R, VEC, 1>(p, M, nt, st); break;
+        case 2: launch_n<Y, R, VEC, 2>(p, M, nt, st); break;
+        case 4: launch_n<Y, R, VEC, 4>(p, M, nt, st); break;
         default:
             if constexpr (VEC == 1) {
-                if (nch == 8) norm_residual_kernel<Y, R, VEC, 8><<<(unsigned)M, nt, 0, st>>>(p);
-                else if (nch == 16) norm_residual_kernel<Y, R, VEC, 16><<<(unsigned)M, nt, 0, st>>>(p);
-                else norm_residual_kernel<Y, R, VEC, 32><<<(unsigned)M, nt, 0, st>>>(p);
+                if (nch == 8) launch_n<Y, R, VEC, 8>(p, M, nt, st);
+                else if (nch == 16) launch_n<Y, R, VEC, 16>(p, M, nt, st);
+                else launch_n<Y, R, VEC, 32>(p, M, nt, st);
             }
     }
     QL_CUDA_TRY(cudaGetLastError());

@@ -32,59 +32,60 @@ struct Params {
 };
 
 template <typename T, int VEC, bool HALF>
-__global__ void __launch_bounds__(1024) rope_kernel(const Params p) {
+__global__ void __launch_bounds__(VEC == 8 ? 256 : 1024) rope_kernel(const Params p) {
     using PT = Pack<T, VEC>;
     using PF = Pack<float, VEC>;
     const int64_t t = blockIdx.x;
+    const int half = p.rot / 2;
+    const int U = half / VEC, C = U + (p.D - p.rot) / VEC;  // pair chunks, then copied chunks
+    const int c = threadIdx.x % C, h0 = threadIdx.x / C, HG = blockDim.x / C, heads = p.Hq + p.Hk;
+    const bool pair = c < U;
+    // elements of the thread's first and second access within a head
+    const int e0 = !pair ? p.rot + (c - U) * VEC : HALF ? c * VEC : 2 * c * VEC;
+    const int e1 = HALF ? half + c * VEC : 2 * c * VEC + VEC;
+    auto load = [&](int h, PT &a, PT &b) {
+        const T *src = h < p.Hq ? reinterpret_cast<const T *>(p.q) + t * p.q_token + h * p.q_head
+                                : reinterpret_cast<const T *>(p.k) + t * p.k_token + (h - p.Hq) * p.k_head;
+        a = *reinterpret_cast<const PT *>(src + e0);
+        if (pair) b = *reinterpret_cast<const PT *>(src + e1);
+    };
+    const int v_per = p.D / VEC, v_all = p.k_cache ? p.Hk * v_per : 0;
+    auto load_v = [&](int i) {
+        const int h = i / v_per;
+        return *reinterpret_cast<const PT *>(reinterpret_cast<const T *>(p.v) + t * p.v_token + h * p.v_head + (i - h * v_per) * VEC);
+    };
+    // the first chunks are in flight while the position and its table row are fetched
+    const bool busy = h0 < HG && h0 < heads;
+    PT a, b, w;
+    if (busy) load(h0, a, b);
+    if ((int)threadIdx.x < v_all) w = load_v(threadIdx.x);
+
     const int64_t pos = p.positions[t];
+    int64_t slot = p.k_cache ? p.slots[t] : -1;
     const bool bad = pos < 0 || pos >= p.P;
-    int64_t slot = -1;
-    if (p.k_cache) {
-        slot = p.slots[t];
-        if (slot >= p.num_slots || bad) {
-            if (slot >= p.num_slots && threadIdx.x == 0) raise_dev_error(DEV_ERR_BAD_INDEX);
-            slot = -1;  // the token is not cached
-        }
-    }
-    if (bad && threadIdx.x == 0) raise_dev_error(DEV_ERR_BAD_INDEX);
+    if ((bad || slot >= p.num_slots) && threadIdx.x == 0 && (bad || p.k_cache)) raise_dev_error(DEV_ERR_BAD_INDEX);
+    if (bad || slot >= p.num_slots) slot = -1;  // the token is not cached
     const int64_t ps = (int64_t)1 << p.page_shift;
     const int64_t cache_at = slot < 0 ? 0 : (slot >> p.page_shift) * p.page_stride + (slot & (ps - 1)) * p.D;
     const int64_t cache_head = ps * p.D;
 
-    const int half = p.rot / 2;
-    const int U = half / VEC, C = U + (p.D - p.rot) / VEC;  // pair chunks, then copied chunks
-    const int c = threadIdx.x % C, h0 = threadIdx.x / C, HG = blockDim.x / C;
-    if (h0 < HG) {
-        const bool pair = c < U;
-        // elements of the thread's first and second access within a head
-        const int e0 = !pair ? p.rot + (c - U) * VEC : HALF ? c * VEC : 2 * c * VEC;
-        const int e1 = !pair ? e0 : HALF ? half + c * VEC : 2 * c * VEC + VEC;
+    if (busy) {
         PF cs, sn;
         if (pair && !bad) {
             cs = *reinterpret_cast<const PF *>(p.table + pos * p.rot + c * VEC);
             sn = *reinterpret_cast<const PF *>(p.table + pos * p.rot + half + c * VEC);
         }
-        for (int h = h0; h < p.Hq + p.Hk; h += HG) {
-            const bool isq = h < p.Hq;
-            const T *src = isq ? reinterpret_cast<const T *>(p.q) + t * p.q_token + h * p.q_head
-                               : reinterpret_cast<const T *>(p.k) + t * p.k_token + (h - p.Hq) * p.k_head;
-            T *dst;
-            if (isq) dst = reinterpret_cast<T *>(p.q_out) + (t * p.Hq + h) * p.D;
-            else if (p.k_cache) dst = reinterpret_cast<T *>(p.k_cache) + cache_at + (h - p.Hq) * cache_head;
-            else dst = reinterpret_cast<T *>(p.k_out) + (t * p.Hk + (h - p.Hq)) * p.D;
-            if (!isq && p.k_cache && slot < 0) continue;
-            PT a, b;
+        for (int h = h0;;) {
+            const int next = h + HG;
+            PT na, nb;
+            if (next < heads) load(next, na, nb);
             if (bad) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     from_f(a.v[e], 0.f);
                     from_f(b.v[e], 0.f);
                 }
-            } else {
-                a = *reinterpret_cast<const PT *>(src + e0);
-                if (pair) b = *reinterpret_cast<const PT *>(src + e1);
-            }
-            if (pair && !bad) {
+            } else if (pair) {
                 if (HALF || VEC == 1) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
@@ -95,25 +96,30 @@ __global__ void __launch_bounds__(1024) rope_kernel(const Params p) {
                 } else {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        PT &w = e < VEC / 2 ? a : b;
+                        PT &z = e < VEC / 2 ? a : b;
                         const int i = 2 * e % VEC;
-                        const float x = to_f(w.v[i]), y = to_f(w.v[i + 1]);
-                        from_f(w.v[i], x * cs.v[e] - y * sn.v[e]);
-                        from_f(w.v[i + 1], y * cs.v[e] + x * sn.v[e]);
+                        const float x = to_f(z.v[i]), y = to_f(z.v[i + 1]);
+                        from_f(z.v[i], x * cs.v[e] - y * sn.v[e]);
+                        from_f(z.v[i + 1], y * cs.v[e] + x * sn.v[e]);
                     }
                 }
             }
-            *reinterpret_cast<PT *>(dst + e0) = a;
-            if (pair) *reinterpret_cast<PT *>(dst + e1) = b;
+            T *dst;
+            if (h < p.Hq) dst = reinterpret_cast<T *>(p.q_out) + (t * p.Hq + h) * p.D;
+            else if (p.k_cache) dst = reinterpret_cast<T *>(p.k_cache) + cache_at + (h - p.Hq) * cache_head;
+            else dst = reinterpret_cast<T *>(p.k_out) + (t * p.Hk + (h - p.Hq)) * p.D;
+            if (h < p.Hq || !p.k_cache || slot >= 0) {
+                *reinterpret_cast<PT *>(dst + e0) = a;
+                if (pair) *reinterpret_cast<PT *>(dst + e1) = b;
+            }
+            if (next >= heads) break;
+            h = next, a = na, b = nb;
         }
     }
-    if (slot >= 0) {
-        const int per = p.D / VEC;
-        for (int i = threadIdx.x; i < p.Hk * per; i += blockDim.x) {
-            const int h = i / per, e = (i - h * per) * VEC;
-            *reinterpret_cast<PT *>(reinterpret_cast<T *>(p.v_cache) + cache_at + h * cache_head + e) =
-                *reinterpret_cast<const PT *>(reinterpret_cast<const T *>(p.v) + t * p.v_token + h * p.v_head + e);
-        }
+    for (int i = threadIdx.x; i < v_all && slot >= 0; i += blockDim.x) {
+        if (i != (int)threadIdx.x) w = load_v(i);
+        const int h = i / v_per;
+        *reinterpret_cast<PT *>(reinterpret_cast<T *>(p.v_cache) + cache_at + h * cache_head + (i - h * v_per) * VEC) = w;
     }
 }
 
@@ -122,7 +128,7 @@ static int launch(const Params &p, int64_t tokens, bool half, bool vec, cudaStre
     const int VEC = vec ? 8 : 1;
     const int C = p.rot / 2 / VEC + (p.D - p.rot) / VEC;
     int nt = C * (p.Hq + p.Hk);
-    if (nt > 256) nt = 256;
+    if (nt > 128) nt = 128;
     if (nt < C) nt = C;
     nt = (nt + 31) / 32 * 32;
     const unsigned grid = (unsigned)tokens;
