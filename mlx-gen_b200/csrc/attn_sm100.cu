@@ -262,28 +262,40 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     if (!ok) break;
                 }
                 const uint64_t c2 = f2_make(c, c), nb2 = f2_make(-base, -base);
-                uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // the first PFIRST positions, then the rest
-                    const int from = h ? PFIRST : 0, to = h ? TKV : PFIRST;
-#pragma unroll
-                    for (int q = from; q < to; q += 32) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float x, y;
-                            f2_split(f2_fma(f2_make(sc[q + 2 * i], sc[q + 2 * i + 1]), c2, nb2), x, y);
-                            x = ex2(x), y = ex2(y);
-                            sum[i & 1] = f2_add(sum[i & 1], f2_make(x, y));
-                            pk[i] = pack2<T>(x, y);
-                        }
-                        tmem_st16(s_col + q / 2, pk);
-                    }
+                auto hand_over = [&](int h) {  // P_t's positions so far are in TMEM
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&pfull[2 * t + h]);
+                };
+                uint64_t sum[2] = {0ull, 0ull};
+                // pairs of scores in flight: x2 of pair i + AHEAD is made while pair i is in the
+                // special-function unit, so that unit, which bounds the loop, does not wait
+                constexpr int AHEAD = 2;
+                uint64_t x2[AHEAD];
+                uint32_t pk[16];
+                auto pair = [&](int i) { return f2_fma(f2_make(sc[2 * i], sc[2 * i + 1]), c2, nb2); };
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) x2[i] = pair(i);
+                float px, py;
+#pragma unroll
+                for (int i = 0; i < TKV / 2; ++i) {
+                    float x, y;
+                    f2_split(x2[i % AHEAD], x, y);
+                    x = ex2(x), y = ex2(y);
+                    if (i + AHEAD < TKV / 2) x2[i % AHEAD] = pair(i + AHEAD);
+                    if (i > 0) {
+                        sum[i & 1] = f2_add(sum[i & 1], f2_make(px, py));
+                        pk[(i - 1) & 15] = pack2<T>(px, py);
+                        if (((i - 1) & 15) == 15) tmem_st16(s_col + (i - 16), pk);
+                    }
+                    if (i == PFIRST / 2) hand_over(0);
+                    px = x, py = y;
                 }
+                sum[0] = f2_add(sum[0], f2_make(px, py));
+                pk[15] = pack2<T>(px, py);
+                tmem_st16(s_col + TKV / 2 - 16, pk);
+                hand_over(1);
                 if (lane == 0 && ntiles == 2) mbar_arrive(&turn[t ^ 1]);
                 float sx, sy;
                 f2_split(f2_add(sum[0], sum[1]), sx, sy);
