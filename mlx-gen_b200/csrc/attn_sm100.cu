@@ -41,9 +41,12 @@ struct Sm100Cfg {
     static constexpr int HALF_BYTES = 128 * 128;           // 128 rows of 64 elements
     static constexpr int TILE_BYTES = HALVES * HALF_BYTES;  // of Q, K or V
     static constexpr int STAGES = D == 128 ? 5 : 8;
+    // TMEM columns: S_t at 128 t, O_t next, and for D = 64 what is left is enough for P_t beside S_t
+    static constexpr bool P_APART = D == 64;
+    static constexpr int COL_O = 256, COL_P = P_APART ? 256 + 2 * D : 0, P_STEP = P_APART ? TKV / 2 : TKV;
     static constexpr int SMEM_Q = 0, SMEM_KV = 2 * TILE_BYTES;
     static constexpr int SMEM_BAR = SMEM_KV + STAGES * TILE_BYTES;
-    static constexpr int NBAR = 2 * STAGES + 2 * 7 + 2;
+    static constexpr int NBAR = 2 * STAGES + 2 * 8 + 2;
     static constexpr int SMEM = SMEM_BAR + NBAR * 8 + 16 + 1024;
 };
 
@@ -65,6 +68,9 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+
+// the n lowest bits (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // 32 bytes in one store: a whole DRAM sector of a thread's own row
 __device__ __forceinline__ void st_global_32(void *dst, const uint32_t v[8]) {
@@ -92,6 +98,10 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
     using C = Sm100Cfg<D>;
     constexpr int STAGES = C::STAGES;
+#ifndef V_TURNS64
+#define V_TURNS64 0
+#endif
+    constexpr bool TURNS = !C::P_APART || V_TURNS64;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::SMEM_BAR);  // K / V stage landed
@@ -99,10 +109,11 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint64_t *qfull = empty + STAGES;  // [2] Q_t written
     uint64_t *sfull = qfull + 2;       // [2] S_t of the step computed (and O_t of the step before)
     uint64_t *pfull = sfull + 2;       // [2][2] P_t written: its first PFIRST positions, the rest
-    uint64_t *ofull = pfull + 4;       // [2] O_t complete
+    uint64_t *ofull = pfull + 4;       // [2] O_t complete (P_APART: of the step)
     uint64_t *drain = ofull + 2;       // [2] an aborted tile's MMAs are done
     uint64_t *turn = drain + 2;        // [2] the other tile's exponentials of the step are done
-    uint64_t *vfix = turn + 2;         // [2] V of the first / last step cleared outside [vlo, vhi)
+    uint64_t *sread = turn + 2;        // [2] S_t of the step is in registers (P_APART)
+    uint64_t *vfix = sread + 2;        // [2] V of the first / last step cleared outside [vlo, vhi)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -154,6 +165,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             mbar_init(&ofull[t], 1);
             mbar_init(&drain[t], 1);
             mbar_init(&turn[t], 4);
+            mbar_init(&sread[t], 4);
             mbar_init(&vfix[t], 1);
         }
         *abort_flag = 0;
@@ -206,7 +218,8 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             rhi = min(rhi, vhi);
 
             const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t s_col = lane_base + t * 128, o_col = lane_base + 256 + t * 128;
+            const uint32_t s_col = lane_base + t * TKV, o_col = lane_base + C::COL_O + t * D;
+            const uint32_t p_col = lane_base + C::COL_P + t * C::P_STEP;
             const float c = p.scale_log2;
             float m = NEG_INF, l = 0.f;  // reference maximum (of unscaled scores) in use, sum
             bool ok = true;
@@ -216,19 +229,27 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 tc_fence_after();
                 if (tid == 0) {  // K of this step and V of the step before have been read
                     mbar_arrive(&empty[(2 * j) % STAGES]);
-                    if (j > 0) mbar_arrive(&empty[(2 * j - 1) % STAGES]);
+                    if (!C::P_APART && j > 0) mbar_arrive(&empty[(2 * j - 1) % STAGES]);
                 }
                 __syncwarp();
                 float sc[TKV];
 #pragma unroll
                 for (int i = 0; i < TKV / 32; ++i) tmem_ld32(s_col + i * 32, reinterpret_cast<uint32_t *>(sc) + i * 32);
                 tmem_ld_wait();
+                if constexpr (C::P_APART) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sread[t]);
+                }
                 const int kv0 = (t0 + j) * TKV;
                 // a step that some row of the tile does not see whole (the same for all its threads)
                 if (kv0 < max_lo || kv0 + TKV > min_hi) {
-                    const int a = rlo - kv0, e = rhi - kv0;
 #pragma unroll
-                    for (int i = 0; i < TKV; ++i) sc[i] = (i >= a && i < e) ? sc[i] : NEG_INF;
+                    for (int w = 0; w < TKV / 32; ++w) {  // one bit per position: two instructions a score
+                        const uint32_t see = bits_below(rhi - kv0 - w * 32) & ~bits_below(rlo - kv0 - w * 32);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sc[w * 32 + i] = (see & (1u << i)) ? sc[w * 32 + i] : NEG_INF;
+                    }
                 }
                 float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
@@ -237,6 +258,13 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], sc[i + 2 * k], sc[i + 2 * k + 1]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], sc[124 + k]);
+                if (C::P_APART && j > 0) {  // O_t of the step before: P_t and its V stage are free, O_t is at rest
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ofull[t], (j - 1) & 1, abort_flag, DEV_ERR_TIMEOUT_ACC));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (tid == 0) mbar_arrive(&empty[(2 * j - 1) % STAGES]);
+                    __syncwarp();
+                }
                 const float nm = max3(max3(mx[0], mx[1], mx[2]), mx[3], m);
                 const bool grow = (nm - m) * c > 8.f;  // also from -inf; false while nothing is seen (nan)
                 if (__any_sync(0xffffffffu, grow)) {
@@ -257,7 +285,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
                 const float base = m == NEG_INF ? 0.f : m * c;
                 // the tiles take turns: tile 1 follows tile 0's step, tile 0 tile 1's step before
-                if (ntiles == 2 && (t == 1 || j > 0)) {
+                if (TURNS && ntiles == 2 && (t == 1 || j > 0)) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&turn[t], (t == 1 ? j : j - 1) & 1, abort_flag, DEV_ERR_TIMEOUT_ACC));
                     if (!ok) break;
                 }
@@ -287,22 +315,22 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     if (i > 0) {
                         sum[i & 1] = f2_add(sum[i & 1], f2_make(px, py));
                         pk[(i - 1) & 15] = pack2<T>(px, py);
-                        if (((i - 1) & 15) == 15) tmem_st16(s_col + (i - 16), pk);
+                        if (((i - 1) & 15) == 15) tmem_st16(p_col + (i - 16), pk);
                     }
                     if (i == PFIRST / 2) hand_over(0);
                     px = x, py = y;
                 }
                 sum[0] = f2_add(sum[0], f2_make(px, py));
                 pk[15] = pack2<T>(px, py);
-                tmem_st16(s_col + TKV / 2 - 16, pk);
+                tmem_st16(p_col + TKV / 2 - 16, pk);
                 hand_over(1);
-                if (lane == 0 && ntiles == 2) mbar_arrive(&turn[t ^ 1]);
+                if (TURNS && lane == 0 && ntiles == 2) mbar_arrive(&turn[t ^ 1]);
                 float sx, sy;
                 f2_split(f2_add(sum[0], sum[1]), sx, sy);
                 l += sx + sy;
             }
             // ------------------------------------------------------------ epilogue of tile t
-            if (ok && __all_sync(0xffffffffu, mbar_wait(&ofull[t], 0, abort_flag, DEV_ERR_TIMEOUT_ACC))) {
+            if (ok && __all_sync(0xffffffffu, mbar_wait(&ofull[t], C::P_APART ? (n - 1) & 1 : 0, abort_flag, DEV_ERR_TIMEOUT_ACC))) {
                 tc_fence_after();
                 const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
                 const int64_t row = (s.q0 + (int64_t)(r / p.G)) * p.Hq + kvh * p.G + r % p.G;
@@ -399,7 +427,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
         const int t = warp - 9;
         if (t < ntiles && lane == 0) {
             constexpr uint32_t qk = attn_idesc<T>(TKV, false), pv = attn_idesc<T>(D, true);
-            const uint32_t s_col = tmem + t * 128, o_col = tmem + 256 + t * 128;
+            const uint32_t s_col = tmem + t * TKV, o_col = tmem + C::COL_O + t * D, p_col = tmem + C::COL_P + t * C::P_STEP;
             const uint32_t qs = smem_u32(smem + C::SMEM_Q + t * C::TILE_BYTES), ring = smem_u32(smem + C::SMEM_KV);
             auto scores = [&](int j) {  // S_t = Q_t K^T of step j
                 const int st = (2 * j) % STAGES;
@@ -416,6 +444,11 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             bool ok = mbar_wait(&qfull[t], 0, abort_flag, DEV_ERR_TIMEOUT_FULL) && scores(0);
             if (ok) tc_commit(&sfull[t]);
             for (int j = 0; ok && j < n; ++j) {
+                if (C::P_APART && j + 1 < n) {  // the next step's scores before this step's weights
+                    ok = mbar_wait(&sread[t], j & 1, abort_flag, DEV_ERR_TIMEOUT_ACC) && scores(j + 1);
+                    if (!ok) break;
+                    tc_commit(&sfull[t]);
+                }
                 const int it = 2 * j + 1, st = it % STAGES;
                 ok = mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, DEV_ERR_TIMEOUT_FULL);
                 if (ok && j == 0 && (fix_first || (n == 1 && fix_last))) ok = mbar_wait(&vfix[0], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
@@ -428,14 +461,14 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     tc_fence_after();
 #pragma unroll
                     for (int k = h ? PFIRST / 16 : 0; k < (h ? TKV : PFIRST) / 16; ++k)
-                        tc_mma_ts(o_col, s_col + k * 8, umma_desc_mn_sw128(vs + k * 2048, C::HALF_BYTES), pv, (j | k) != 0);
+                        tc_mma_ts(o_col, p_col + k * 8, umma_desc_mn_sw128(vs + k * 2048, C::HALF_BYTES), pv, (j | k) != 0);
                 }
                 if (!ok) break;
-                if (j + 1 < n) {
+                if (C::P_APART || j + 1 == n) {
+                    tc_commit(&ofull[t]);
+                } else {
                     ok = scores(j + 1);
                     if (ok) tc_commit(&sfull[t]);
-                } else {
-                    tc_commit(&ofull[t]);
                 }
             }
             if (!ok) {  // aborted: the MMAs issued so far finish before TMEM is freed
