@@ -386,14 +386,27 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(done);
             };
-            int it = 0;
-            int page = 0;
+            // this lane's page of step j, where there is something to see; indices are fetched four
+            // steps ahead
+            auto page_index = [&](int j) {
+                const int pos = (t0 + j) * TKV + lane * box;
+                return j < n && lane < nb && pos < vhi && pos + box > vlo ? p.table[b * p.table_stride + (pos >> p.page_shift)] : 0;
+            };
+            int it = 0, page = 0, ahead[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ahead[j] = page_index(j);
             for (; it < 2 * n; ++it) {
-                if (it == STAGES && fix_first) clear_v(0, &vfix[0]);
-                const int st = it % STAGES, kv0 = (t0 + (it >> 1)) * TKV;
-                const int pos = kv0 + lane * box;
-                const bool in = lane < nb && pos < vhi && pos + box > vlo;  // pages that hold something to see
-                if (!(it & 1) && in) page = page_of(p, b, pos);
+                if (it == min(STAGES, 2 * n - 1) && fix_first && n > 1) clear_v(0, &vfix[0]);
+                const int st = it % STAGES, pos = (t0 + (it >> 1)) * TKV + lane * box;
+                const bool in = lane < nb && pos < vhi && pos + box > vlo;
+                if (!(it & 1)) {
+                    page = ahead[0], ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
+                    ahead[3] = page_index((it >> 1) + 4);
+                    if (in && (unsigned)page >= (unsigned)p.num_pages) {
+                        raise_dev_error(DEV_ERR_BAD_INDEX);
+                        page = 0;
+                    }
+                }
                 if (it >= STAGES &&
                     !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((it / STAGES) & 1) ^ 1, abort_flag, DEV_ERR_TIMEOUT_EMPTY)))
                     break;
@@ -409,7 +422,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
             }
             if (it == 2 * n) {
-                if ((fix_first && 2 * n <= STAGES) || (fix_last && n == 1)) clear_v(0, &vfix[0]);
+                if (n == 1 && (fix_first || fix_last)) clear_v(0, &vfix[0]);
                 if (fix_last && n > 1) clear_v(n - 1, &vfix[1]);
             }
             if (*abort_flag) {  // let the copies in flight land before the CTA's memory is given up
