@@ -259,7 +259,8 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
                        void *stream);
 
 /* Bytes of device workspace ql_paged_attention needs for these sizes (0: none). */
-size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv);
+size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv,
+                                         int64_t window);
 
 /* Copies pages inside a pool: page dst[i] := page src[i] in each of `planes` planes (the keys or
  * values of one layer), plane_stride bytes apart, pages page_stride bytes apart, page_bytes each

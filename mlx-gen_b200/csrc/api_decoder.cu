@@ -13,7 +13,7 @@ int launch_norm_residual(const normres::Params &, int, int, int64_t, bool, cudaS
 int launch_rope(const ropek::Params &, int, int64_t, bool, bool, cudaStream_t);
 int launch_copy_pages(void *, int64_t, int64_t, int64_t, int64_t, const int32_t *, const int32_t *, int64_t,
                       cudaStream_t);
-size_t paged_attention_workspace(int64_t, int, int, int, int64_t, int64_t, int64_t);
+size_t paged_attention_workspace(int64_t, int, int, int, int64_t, int64_t, int64_t, int64_t);
 int launch_paged_attention(attn::Params &, int, int, int64_t, void *, cudaStream_t);
 
 static int elem_bytes(int dt) { return dt == QL_F32 ? 4 : 2; }
@@ -134,9 +134,12 @@ int ql_rope_append(const void *q, int64_t q_token_stride, int64_t q_head_stride,
     return rope_common(p, dtype, T, page_size, layout, stream);
 }
 
-size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv) {
+static int64_t effective_window(int64_t window, int64_t max_kv) { return window <= 0 || window >= max_kv ? 0 : window; }
+
+size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv,
+                                         int64_t window) {
     if (check_attention(T, Hq, Hkv, D, B, max_q, max_kv) || T == 0 || B == 0) return 0;
-    return paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv);
+    return paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv, effective_window(window, max_kv));
 }
 
 int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
@@ -164,7 +167,8 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned32(out) || q_token_stride % 8 ||
         q_head_stride % 8)
         return fail(QL_EINVAL_ARG, "q and the caches must be 16-byte aligned, out 32-byte, q's strides multiples of 8");
-    const size_t need = paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv);
+    window = effective_window(window, max_kv);
+    const size_t need = paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv, window);
     if (need && (!workspace || workspace_bytes < need || !aligned32(workspace)))
         return fail(QL_EINVAL_ARG, "ql_paged_attention needs a 32-byte aligned workspace of %zu bytes (got %zu)", need,
                     workspace_bytes);
@@ -176,7 +180,7 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
     p.table = page_table, p.table_stride = table_stride, p.q_starts = q_starts, p.kv_lens = kv_lens;
     p.max_q = (int)max_q, p.max_kv = (int)max_kv;
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.causal = causal != 0, p.window = (int)(window > max_kv ? 0 : window);
+    p.causal = causal != 0, p.window = (int)window;
     p.out = out;
     return launch_paged_attention(p, dtype, D, B, workspace, (cudaStream_t)stream);
 }

@@ -18,6 +18,7 @@ namespace attn {
 
 constexpr int kSMs = 148;         // B200; used for planning only
 constexpr int ROWS_TILE = 16;     // rows of the small-row kernel (one m16 tile)
+constexpr int MAX_CLUSTER = 8;    // splits of the small-row kernel that can join inside a cluster
 constexpr float NEG_INF = -INFINITY;
 
 struct Params {
@@ -36,7 +37,9 @@ struct Params {
     int causal, window;
     void *out;                    // [T, Hq, D]
     float *part_o, *part_lse;     // [T * Hq, nsplit, D], [T * Hq, nsplit]; nsplit > 1 only
-    int nsplit, chunk;            // positions of one split (a multiple of 128)
+    int nsplit, chunk;            // most splits of a row's positions; positions of one (tile kernel: whole steps)
+    bool adapt;                   // small-row kernel: the chunk follows from the sequences' lengths (adapted_chunk)
+    bool cluster;                 // small-row kernel: the splits join inside a cluster, part_* unused
     int rows_kernel_most;         // sequences with up to so many rows go to the small-row kernel
 };
 
@@ -61,6 +64,21 @@ __device__ __forceinline__ Seq load_seq(const Params &p, int b) {
 __device__ __forceinline__ void visible(const Params &p, const Seq &s, int tok, int &lo, int &hi) {
     hi = p.causal ? min(s.kv_len, max(0, s.ctx + tok + 1)) : s.kv_len;
     lo = p.window ? max(0, s.ctx + tok + 1 - p.window) : 0;
+}
+
+// [lo, hi): the positions that some of the packed rows [r0, r1) sees
+__device__ __forceinline__ void visible_rows(const Params &p, const Seq &s, int r0, int r1, int &lo, int &hi) {
+    int unused;
+    visible(p, s, r0 / p.G, lo, unused);
+    visible(p, s, (r1 - 1) / p.G, unused, hi);
+}
+
+// The splits divide what the CTA's rows see, [lo, hi), from lo's 128-boundary on.
+__device__ __forceinline__ void take_split(const Params &p, int split, int chunk, int &lo, int &hi) {
+    if (p.nsplit == 1) return;
+    const int64_t from = (lo & ~127) + (int64_t)split * chunk;
+    lo = (int)max((int64_t)lo, min(from, (int64_t)hi));
+    hi = (int)min((int64_t)hi, from + chunk);
 }
 
 // The page that holds position pos; an index outside the cache is reported and reads page 0.

@@ -29,9 +29,25 @@ struct RowsCfg {
     static constexpr int STAGES = D == 64 ? 6 : D == 96 ? 4 : 3;
     static constexpr int WARP_BYTES = STAGES * 2 * TILE_BYTES;
     static constexpr int SMEM = RW * WARP_BYTES;
-    static_assert(RW * ROWS_TILE * D * 4 + RW * ROWS_TILE * 8 <= SMEM, "the warps' results fit in the ring");
+    // more than half of an SM's: one CTA per SM.  Without it two of a wave that would fit one to an
+    // SM share one while others idle (2 x 131k positions in 144 pieces: 221 us instead of 177)
+    static constexpr int SMEM_ALONE = SMEM > 120000 ? SMEM : 120000;
+    static_assert((RW + 1) * ROWS_TILE * (D + 2) * 4 <= SMEM, "the warps' and the CTA's results fit in the ring");
 };
 
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t r[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -63,31 +79,14 @@ __device__ __forceinline__ void mma16816<__half>(float c[4], const uint32_t a[4]
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// grid: x = split, y = kv head * rowblocks + row block, z = sequence
-template <typename T, int D>
-__global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowblocks) {
+// One stretch of positions [lo, hi) for one row block of a (sequence, kv head).  Its result is
+// partial result number `slot` of `slots`, or the output itself where slots is 1 (and not CLUSTER).
+template <typename T, int D, bool CLUSTER>
+__device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int b, int kvh, int rb, int lo, int hi, int slot,
+                                             int slots, uint8_t *smem) {
     using C = RowsCfg<D>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int b = blockIdx.z, kvh = blockIdx.y / rowblocks, rb = blockIdx.y % rowblocks, split = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Seq s = load_seq(p, b);
-    if (!s.ok) {
-        if (threadIdx.x == 0) raise_dev_error(DEV_ERR_BAD_INDEX);
-        return;
-    }
-    const int rows = s.q_len * p.G, r0 = rb * ROWS_TILE;
-    if (r0 >= rows || rows > p.rows_kernel_most) return;
-    const int nrows = min(ROWS_TILE, rows - r0);
-
-    // positions that some row of this CTA sees, within its split
-    int lo, hi, unused;
-    visible(p, s, r0 / p.G, lo, unused);
-    visible(p, s, (r0 + nrows - 1) / p.G, unused, hi);
-    if (p.nsplit > 1) {
-        lo = max(lo, split * p.chunk);
-        hi = (int)min((int64_t)hi, (int64_t)(split + 1) * p.chunk);
-    }
+    const int rows = s.q_len * p.G, r0 = rb * ROWS_TILE, nrows = min(ROWS_TILE, rows - r0);
 
     // this thread's two rows, g and g + 8, and what they see
     const int g = lane >> 2, t4 = lane & 3;
@@ -242,6 +241,9 @@ __global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowbl
         }
     }
     __syncthreads();
+    const int64_t row0 = s.q0 * (int64_t)p.Hq + kvh * p.G;
+    auto row_at = [&](int r) { return row0 + (int64_t)((r0 + r) / p.G) * p.Hq + (r0 + r) % p.G; };
+    float *jo = sl + RW * ROWS_TILE, *jl = jo + ROWS_TILE * D;  // CLUSTER: this CTA's [16][D] and its lse
     for (int idx = threadIdx.x; idx < nrows * (D / 4); idx += RW * 32) {
         const int r = idx / (D / 4), e = idx % (D / 4) * 4;
         float mx = NEG_INF;
@@ -261,33 +263,152 @@ __global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowbl
                 a.w += f * v.w;
             }
         }
-        const float inv = total > 0.f ? 1.f / total : 0.f;
-        const int64_t row = (s.q0 + (int64_t)((r0 + r) / p.G)) * p.Hq + kvh * p.G + (r0 + r) % p.G;
-        if (p.nsplit > 1) {
-            if (e == 0) p.part_lse[row * p.nsplit + split] = mx == NEG_INF ? NEG_INF : mx + log2f(total);
-            if (mx != NEG_INF)
-                *reinterpret_cast<float4 *>(p.part_o + (row * p.nsplit + split) * D + e) =
-                    make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+        a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        const float lse = total > 0.f || total != total ? mx + log2f(total) : NEG_INF;
+        if (CLUSTER) {
+            if (e == 0) jl[r] = lse;
+            *reinterpret_cast<float4 *>(jo + r * D + e) = a;
+        } else if (slots > 1) {
+            const int64_t row = row_at(r);
+            if (e == 0) p.part_lse[row * p.nsplit + slot] = lse;
+            if (lse != NEG_INF) *reinterpret_cast<float4 *>(p.part_o + (row * p.nsplit + slot) * D + e) = a;
         } else {
-            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.out) + row * D + e) =
-                make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.out) + row_at(r) * D + e) =
+                make_uint2(pack2<T>(a.x, a.y), pack2<T>(a.z, a.w));
         }
     }
+    if constexpr (CLUSTER) {
+        cluster_sync_all();
+        // every CTA joins its share of the rows' elements, in the order of the splits
+        for (int idx = slot * RW * 32 + threadIdx.x; idx < nrows * (D / 4); idx += slots * RW * 32) {
+            const int r = idx / (D / 4), e = idx % (D / 4) * 4;
+            float mx = NEG_INF, lse[MAX_CLUSTER];
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c) {
+                lse[c] = c < slots ? ld_cluster(mapa_shared(smem_u32(jl + r), c)) : NEG_INF;
+                mx = fmaxf(mx, lse[c]);
+            }
+            float total = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float base = mx == NEG_INF ? 0.f : mx;
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; ++c) {
+                if (lse[c] == NEG_INF) continue;
+                const float f = ex2(lse[c] - base);
+                const float4 v = ld_cluster4(mapa_shared(smem_u32(jo + r * D + e), c));
+                total += f;
+                a.x += f * v.x;
+                a.y += f * v.y;
+                a.z += f * v.z;
+                a.w += f * v.w;
+            }
+            const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(p.out) + row_at(r) * D + e) =
+                make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+        }
+        cluster_sync_all();  // no CTA leaves while another reads its shared memory
+    }
+}
+
+// The positions of one split when a few sequences (up to 32) are to fill the SMs, whatever their
+// lengths: of the candidates n = 1 .. nsplit pieces for the longest, the one whose waves of CTAs
+// (one per SM, see SMEM_ALONE) take the least time, a piece costing its positions and about 500
+// more.  Lane by lane, two candidates each.
+// (2 x 131k positions: 9 pieces in one wave 177 us, 64 of whatever placement 203.)
+__device__ __forceinline__ int adapted_chunk(const Params &p, int B) {
+    const int lane = threadIdx.x & 31;
+    int len = 0;
+    if (lane < B) {
+        const Seq s = load_seq(p, lane);
+        if (s.ok && s.q_len > 0) {
+            int lo, hi;
+            visible_rows(p, s, 0, s.q_len * p.G, lo, hi);
+            len = hi - (lo & ~127);
+        }
+    }
+    int most = len;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    float best = INFINITY;
+    int chunk = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int n = k * 32 + lane + 1;
+        const int c = ((most + n - 1) / n + 63) & ~63;
+        int pieces = 0;
+        for (int b = 0; b < B; ++b) pieces += (__shfl_sync(0xffffffffu, len, b) + c - 1) / max(c, 1);
+        const float cost = (float)((pieces * p.Hkv + kSMs - 1) / kSMs) * (float)(c + 500);
+        if (n <= p.nsplit && cost < best) best = cost, chunk = c;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float ob = __shfl_xor_sync(0xffffffffu, best, o);
+        const int oc = __shfl_xor_sync(0xffffffffu, chunk, o);
+        if (ob < best || (ob == best && oc > chunk)) best = ob, chunk = oc;
+    }
+    return max(chunk, 64);
+}
+
+// CLUSTER: the splits of a (sequence, kv head, row block) are one thread-block cluster and join
+// through distributed shared memory: no partial results in global memory, no second launch.
+// grid: kv head * rowblocks + row block, sequence and split; the split runs fastest (x) with
+// CLUSTER and slowest (z) without, so that pieces which hold something come before empty ones and
+// the first of them go one to an SM.
+template <typename T, int D, bool CLUSTER>
+__global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowblocks) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int b = CLUSTER ? blockIdx.z : blockIdx.y, split = CLUSTER ? blockIdx.x : blockIdx.z;
+    const int item = CLUSTER ? blockIdx.y : blockIdx.x, kvh = item / rowblocks, rb = item % rowblocks;
+    const Seq s = load_seq(p, b);
+    if (!s.ok) {
+        if (threadIdx.x == 0) raise_dev_error(DEV_ERR_BAD_INDEX);
+        return;
+    }
+    const int rows = s.q_len * p.G, r0 = rb * ROWS_TILE;
+    if (r0 >= rows || rows > p.rows_kernel_most) return;
+    int lo, hi;
+    visible_rows(p, s, r0, min(rows, r0 + ROWS_TILE), lo, hi);
+    take_split(p, split, p.adapt ? adapted_chunk(p, gridDim.y) : p.chunk, lo, hi);
+    if (!CLUSTER && p.nsplit > 1 && lo >= hi) {  // nothing in this split
+        const int r = threadIdx.x;
+        if (r < min(ROWS_TILE, rows - r0))
+            p.part_lse[((s.q0 + (int64_t)((r0 + r) / p.G)) * p.Hq + kvh * p.G + (r0 + r) % p.G) * p.nsplit + split] = NEG_INF;
+        return;
+    }
+    rows_stretch<T, D, CLUSTER>(p, s, b, kvh, rb, lo, hi, split, p.nsplit, smem);
+}
+
+template <typename T, int D, bool CLUSTER>
+static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
+    using C = RowsCfg<D>;
+    auto kernel = rows_kernel<T, D, CLUSTER>;
+    static PerDeviceFlag configured;
+    const int dev = current_device();
+    if (!configured.test(dev)) {
+        QL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_ALONE));
+        configured.set(dev);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = CLUSTER ? dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B) : dim3(p.Hkv * rowblocks, (unsigned)B, p.nsplit);
+    cfg.blockDim = dim3(RW * 32);
+    cfg.dynamicSmemBytes = p.adapt ? C::SMEM_ALONE : C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.nsplit;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = CLUSTER ? 1 : 0;
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, rowblocks));
+    return QL_OK;
 }
 
 template <typename T, int D>
 static int launch_rows_t(const Params &p, int64_t B, int64_t most_rows, cudaStream_t st) {
-    using C = RowsCfg<D>;
-    static PerDeviceFlag configured;
-    const int dev = current_device();
-    if (!configured.test(dev)) {
-        QL_CUDA_TRY(cudaFuncSetAttribute(rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-        configured.set(dev);
-    }
     const int rowblocks = (int)((most_rows + ROWS_TILE - 1) / ROWS_TILE);
-    rows_kernel<T, D><<<dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B), RW * 32, C::SMEM, st>>>(p, rowblocks);
-    QL_CUDA_TRY(cudaGetLastError());
-    return QL_OK;
+    return p.cluster ? launch_rows_c<T, D, true>(p, B, rowblocks, st) : launch_rows_c<T, D, false>(p, B, rowblocks, st);
 }
 
 }  // namespace attn

@@ -135,10 +135,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     int vlo, vhi, unused;
     visible(p, s, row0 / p.G, vlo, unused);
     visible(p, s, (row0 + nrows - 1) / p.G, unused, vhi);
-    if (p.nsplit > 1) {
-        vlo = max(vlo, split * p.chunk);
-        vhi = (int)min((int64_t)vhi, (int64_t)(split + 1) * p.chunk);
-    }
+    take_split(p, split, p.chunk, vlo, vhi);
     if (vhi <= vlo) {  // nothing to see: no partial result, or zeros
         for (int idx = threadIdx.x; idx < nrows; idx += SM100_THREADS) {
             const int r = row0 + idx;

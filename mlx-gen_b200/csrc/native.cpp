@@ -236,7 +236,7 @@ PyObject *paged_attention(PyObject *const *a) {
     at::Tensor q = tensor(a[0], "q");
     const at::Tensor &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &table = tensor(a[3], "page_table");
     const at::Tensor &starts = tensor(a[4], "q_starts"), &lens = tensor(a[5], "kv_lens");
-    const int64_t max_q = integer(a[6]), max_kv = integer(a[7]);
+    const int64_t max_q = integer(a[6]), max_kv = integer(a[7]), window = integer(a[10]);
     const c10::Device dev = on_cuda(q);
     VALUE(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", q.sizes());
     const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
@@ -262,7 +262,7 @@ PyObject *paged_attention(PyObject *const *a) {
               "out must be contiguous, of q's shape, dtype and device");
     }
     const int hq = head_count(Hq), hkv = (int)c.heads, d = (int)D;
-    const size_t need = p_paged_attention_workspace_size(T, hq, hkv, d, B, max_q, max_kv);
+    const size_t need = p_paged_attention_workspace_size(T, hq, hkv, d, B, max_q, max_kv, window);
     at::Tensor ws;
     if (need) {
         if (a[12] != Py_None) {
@@ -275,7 +275,7 @@ PyObject *paged_attention(PyObject *const *a) {
     check(p_paged_attention(q.const_data_ptr(), dtype_code(q), q.stride(0), q.stride(1), T, hq, hkv, d, kc.const_data_ptr(),
                             vc.const_data_ptr(), c.pages, c.stride, (int)c.page_size, tp,
                             B > 1 ? table.stride(0) : table.size(1), sp, lp, B, max_q, max_kv, scale, truth(a[9]),
-                            integer(a[10]), out.mutable_data_ptr(), need ? ws.mutable_data_ptr() : nullptr, need,
+                            window, out.mutable_data_ptr(), need ? ws.mutable_data_ptr() : nullptr, need,
                             stream_of(dev)));
     return THPVariable_Wrap(std::move(out));
 }

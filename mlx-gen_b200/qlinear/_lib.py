@@ -125,7 +125,7 @@ def lib():
                                      i64, vp, vp, vp, vp, i64, i64, i32, vp, vp]
         L.ql_paged_attention.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i64, i64, i32, vp, i64, vp, vp,
                                          i64, i64, i64, f32, i32, i64, vp, vp, sz, vp]
-        L.ql_paged_attention_workspace_size.argtypes = [i64, i32, i32, i32, i64, i64, i64]
+        L.ql_paged_attention_workspace_size.argtypes = [i64, i32, i32, i32, i64, i64, i64, i64]
         L.ql_paged_attention_workspace_size.restype = sz
         L.ql_copy_pages.argtypes = [vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]
         for f in ("ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention", "ql_copy_pages"):

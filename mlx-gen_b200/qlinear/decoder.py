@@ -170,9 +170,10 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
 
 # ------------------------------------------------------------------------ paged attention
 
-def paged_attention_workspace_size(T: int, Hq: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int) -> int:
+def paged_attention_workspace_size(T: int, Hq: int, Hkv: int, D: int, B: int, max_q: int, max_kv: int,
+                                   window: int = 0) -> int:
     """Bytes of workspace ``paged_attention`` needs for these sizes (0: none)."""
-    return int(lib().ql_paged_attention_workspace_size(T, Hq, Hkv, D, B, max_q, max_kv))
+    return int(lib().ql_paged_attention_workspace_size(T, Hq, Hkv, D, B, max_q, max_kv, window))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

@@ -155,7 +155,7 @@ extern "C" {
                               max_kv: i64, scale: f32, causal: c_int, window: i64, out: *mut c_void,
                               workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn ql_paged_attention_workspace_size(t: i64, hq: c_int, hkv: c_int, d: c_int, b: i64, max_q: i64,
-                                             max_kv: i64) -> usize;
+                                             max_kv: i64, window: i64) -> usize;
     pub fn ql_copy_pages(pool: *mut c_void, planes: i64, plane_stride: i64, num_pages: i64, page_stride: i64,
                          page_bytes: i64, src: *const i32, dst: *const i32, n: i64, stream: *mut c_void) -> c_int;
 }

@@ -125,10 +125,10 @@ def test_library_checks_need_no_gpu():
                    (dict(mk=1 << 31, tst=1 << 30), 1), (dict(T=1 << 20, mq=1 << 20, Hq=128, Hkv=2), 2)):
         assert _attention(L, **kw) == rc, kw
     assert _attention(L, T=0, mq=0) == 0 and _attention(L, B=0) == 0
-    need = L.ql_paged_attention_workspace_size(4, 4, 2, 64, 2, 2, 100000)
+    need = L.ql_paged_attention_workspace_size(4, 4, 2, 64, 2, 2, 100000, 0)
     assert need > 0
     assert _attention(L, mk=100000, tst=6250, ws=p, wb=need - 1) == _lib.QL_EINVAL_ARG and b"workspace" in L.ql_last_error()
-    assert L.ql_paged_attention_workspace_size(4, 4, 2, 80, 2, 2, 100000) == 0
+    assert L.ql_paged_attention_workspace_size(4, 4, 2, 80, 2, 2, 100000, 0) == 0
 
     copy = lambda src, dst, **kw: L.ql_copy_pages(*{**dict(pool=p, planes=1, ps=0, P=8, st=64, pb=64), **kw}.values(),  # noqa: E731
                                                   (C.c_int32 * len(src))(*src), (C.c_int32 * len(dst))(*dst), len(src), None)
