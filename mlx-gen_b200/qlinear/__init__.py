@@ -8,6 +8,7 @@ include/qlinear.h.  All arithmetic runs in libqlinear.so (CUDA, sm_100a).
 from ._lib import (ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, ACT_SWIGLU, KERNEL_AUTO, KERNEL_GEMM, KERNEL_GEMM_PAIR,
                    KERNEL_GEMV, KERNEL_GEMV_REGS, KERNEL_GEMV_TC, KERNEL_GEMV_TMA, KERNEL_GENERIC, QlError,
                    device_error)
+from .cache import OutOfPages, PagedCache
 from .decoder import (copy_pages, norm_residual, paged_attention, paged_attention_workspace_size, rope, rope_append,
                       rope_table)
 from .nn import (DEFAULT_GROUP_SIZE, AdaptableLinear, Linear, Lokr, Lora, QuantizedLinear,
@@ -23,5 +24,5 @@ __all__ = [
     "dequantize_rows", "layernorm_modulate", "quantize", "quantized_matmul", "workspace_size", "embedding", "lin",
     "packed_bits", "PackedShapeError", "quantize_map", "reconstruct_lokr_delta", "reconstruct_lokr_delta_scaled",
     "reconstruct_loha_delta", "copy_pages", "norm_residual", "paged_attention", "paged_attention_workspace_size",
-    "rope", "rope_append", "rope_table",
+    "rope", "rope_append", "rope_table", "OutOfPages", "PagedCache",
 ]
