@@ -11,7 +11,7 @@
 // r % G of the group (G = Hq / Hkv), so a group's heads read each key and value together.
 #pragma once
 
-#include "ql_common.cuh"
+#include "pdl.cuh"
 
 namespace ql {
 namespace attn {
@@ -145,7 +145,8 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const float *part_o, const float *part_lse, int64_t rows, int nsplit,
                                                    T *out) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_trigger();
+    pdl_wait();
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= rows) return;
     const int lane = threadIdx.x & 31;
@@ -177,18 +178,9 @@ __global__ void __launch_bounds__(128) join_kernel(const float *part_o, const fl
 
 template <typename T, int D>
 static int launch_join(const Params &p, cudaStream_t st) {
-    cudaLaunchConfig_t cfg{};
     const int64_t rows = p.T * p.Hq;
-    cfg.gridDim = dim3((unsigned)((rows + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, (const float *)p.part_o, (const float *)p.part_lse, rows,
-                                   p.nsplit, (T *)p.out));
+    QL_CUDA_TRY(launch_pdl(join_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, 1, (const float *)p.part_o,
+                           (const float *)p.part_lse, rows, p.nsplit, (T *)p.out));
     return QL_OK;
 }
 

@@ -358,7 +358,8 @@ __device__ __forceinline__ int adapted_chunk(const Params &p, int B) {
 template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowblocks) {
     extern __shared__ __align__(16) uint8_t smem[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    pdl_trigger();
+    pdl_wait();
     const int b = CLUSTER ? blockIdx.z : blockIdx.y, split = CLUSTER ? blockIdx.x : blockIdx.z;
     const int item = CLUSTER ? blockIdx.y : blockIdx.x, kvh = item / rowblocks, rb = item % rowblocks;
     const Seq s = load_seq(p, b);
@@ -390,18 +391,8 @@ static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t
         QL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_ALONE));
         configured.set(dev);
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = CLUSTER ? dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B) : dim3(p.Hkv * rowblocks, (unsigned)B, p.nsplit);
-    cfg.blockDim = dim3(RW * 32);
-    cfg.dynamicSmemBytes = p.adapt ? C::SMEM_ALONE : C::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = p.nsplit;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = CLUSTER ? 1 : 0;
-    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, rowblocks));
+    const dim3 grid = CLUSTER ? dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B) : dim3(p.Hkv * rowblocks, (unsigned)B, p.nsplit);
+    QL_CUDA_TRY(launch_pdl(kernel, grid, dim3(RW * 32), p.adapt ? C::SMEM_ALONE : C::SMEM, st, CLUSTER ? p.nsplit : 1, p, rowblocks));
     return QL_OK;
 }
 

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     const Seq s = load_seq(p, blockIdx.z);
@@ -175,6 +175,9 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // only now: a dependent kernel that allocates tensor memory before its own wait must not take
+    // it from a CTA of this one
+    pdl_trigger();
 
     // registers: 3 warpgroups x 168 at launch = 2 x 216 + 72 (a softmax thread holds 128 scores)
     if (warp < 8) {
@@ -524,8 +527,8 @@ static int launch_sm100_t(const Params &p, int64_t B, cudaStream_t st) {
     if (int rc = cache_map<T>(&mk, p.k_cache, p, D)) return rc;
     if (int rc = cache_map<T>(&mv, p.v_cache, p, D)) return rc;
     const int tiles = (int)(((int64_t)p.max_q * p.G + SM100_ROWS - 1) / SM100_ROWS);
-    sm100_kernel<T, D><<<dim3(p.Hkv * p.nsplit, tiles, (unsigned)B), SM100_THREADS, C::SMEM, st>>>(mk, mv, p);
-    QL_CUDA_TRY(cudaGetLastError());
+    QL_CUDA_TRY(launch_pdl(sm100_kernel<T, D>, dim3(p.Hkv * p.nsplit, tiles, (unsigned)B), dim3(SM100_THREADS), C::SMEM, st, 1,
+                           mk, mv, p));
     return QL_OK;
 }
 

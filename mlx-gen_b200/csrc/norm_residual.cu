@@ -12,7 +12,7 @@
 // sums of squares are block reductions.
 #include <string.h>
 
-#include "ql_common.cuh"
+#include "pdl.cuh"
 
 namespace ql {
 namespace normres {
@@ -78,6 +78,8 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
 template <typename Y, typename R, int VEC, int NCH, bool WARP_ROW>
 __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_residual_kernel(const Params p, int64_t M) {
     __shared__ float red[2][32];
+    pdl_trigger();
+    pdl_wait();
     using PY = Pack<Y, VEC>;
     using PR = Pack<R, VEC>;
     const int nt = WARP_ROW ? 32 : blockDim.x, tid = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
@@ -173,9 +175,10 @@ __global__ void __launch_bounds__(WARP_ROW ? 256 : 1024) norm_residual_kernel(co
 }
 
 template <typename Y, typename R, int VEC, int NCH>
-static void launch_n(const Params &p, int64_t M, int nt, cudaStream_t st) {
-    if (NCH == 1 && nt == 32) norm_residual_kernel<Y, R, VEC, 1, true><<<(unsigned)((M + 7) / 8), 256, 0, st>>>(p, M);
-    else norm_residual_kernel<Y, R, VEC, NCH, false><<<(unsigned)M, nt, 0, st>>>(p, M);
+static cudaError_t launch_n(const Params &p, int64_t M, int nt, cudaStream_t st) {
+    if (NCH == 1 && nt == 32)
+        return launch_pdl(norm_residual_kernel<Y, R, VEC, 1, true>, dim3((unsigned)((M + 7) / 8)), dim3(256), 0, st, 1, p, M);
+    return launch_pdl(norm_residual_kernel<Y, R, VEC, NCH, false>, dim3((unsigned)M), dim3(nt), 0, st, 1, p, M);
 }
 
 template <typename Y, typename R, int VEC>
@@ -187,18 +190,19 @@ static int launch(const Params &p, int64_t M, cudaStream_t st) {
     int nch = 1;
     while (nch < MAXC && (int64_t)nch * 1024 < n) nch *= 2;
     const int nt = ((n + nch - 1) / nch + 31) / 32 * 32;
+    cudaError_t rc = cudaErrorInvalidValue;
     switch (nch) {
-        case 1: launch_n<Y, R, VEC, 1>(p, M, nt, st); break;
-        case 2: launch_n<Y, R, VEC, 2>(p, M, nt, st); break;
-        case 4: launch_n<Y, R, VEC, 4>(p, M, nt, st); break;
+        case 1: rc = launch_n<Y, R, VEC, 1>(p, M, nt, st); break;
+        case 2: rc = launch_n<Y, R, VEC, 2>(p, M, nt, st); break;
+        case 4: rc = launch_n<Y, R, VEC, 4>(p, M, nt, st); break;
         default:
             if constexpr (VEC == 1) {
-                if (nch == 8) launch_n<Y, R, VEC, 8>(p, M, nt, st);
-                else if (nch == 16) launch_n<Y, R, VEC, 16>(p, M, nt, st);
-                else launch_n<Y, R, VEC, 32>(p, M, nt, st);
+                if (nch == 8) rc = launch_n<Y, R, VEC, 8>(p, M, nt, st);
+                else if (nch == 16) rc = launch_n<Y, R, VEC, 16>(p, M, nt, st);
+                else rc = launch_n<Y, R, VEC, 32>(p, M, nt, st);
             }
     }
-    QL_CUDA_TRY(cudaGetLastError());
+    QL_CUDA_TRY(rc);
     return QL_OK;
 }
 

@@ -9,7 +9,7 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include "ql_common.cuh"
+#include "pdl.cuh"
 
 namespace ql {
 namespace pagesk {
@@ -23,6 +23,8 @@ struct Pairs {
 
 __global__ void __launch_bounds__(THREADS) copy_pages_kernel(uint4 *pool, int64_t plane, int64_t page, int64_t words,
                                                              const __grid_constant__ Pairs pr) {
+    pdl_trigger();
+    pdl_wait();
     // plane, page, words: 16-byte words between planes, between pages, of one page
     uint4 *base = pool + (int64_t)blockIdx.z * plane;
     const uint4 *s = base + pr.src[blockIdx.y] * page;
@@ -51,9 +53,9 @@ int launch_copy_pages(void *pool, int64_t planes, int64_t plane_stride, int64_t 
             Pairs pr;
             memcpy(pr.src, src + i, k * sizeof(int));
             memcpy(pr.dst, dst + i, k * sizeof(int));
-            copy_pages_kernel<<<dim3(gx, k, gz), THREADS, 0, st>>>(
-                reinterpret_cast<uint4 *>(pool) + z0 * (plane_stride / 16), plane_stride / 16, page_stride / 16, words, pr);
-            QL_CUDA_TRY(cudaGetLastError());
+            QL_CUDA_TRY(launch_pdl(copy_pages_kernel, dim3(gx, k, gz), dim3(THREADS), 0, st, 1,
+                                   reinterpret_cast<uint4 *>(pool) + z0 * (plane_stride / 16), plane_stride / 16,
+                                   page_stride / 16, words, pr));
         }
     }
     return QL_OK;

@@ -9,7 +9,7 @@
 // token; a thread owns one chunk of pairs and walks over the heads with it, so it reads its
 // cosines and sines once.  VEC = 8 moves 16 or 32 bytes per access; VEC = 1 takes any
 // alignment and any even rot.
-#include "ql_common.cuh"
+#include "pdl.cuh"
 
 namespace ql {
 namespace ropek {
@@ -35,6 +35,8 @@ template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(VEC == 8 ? 256 : 1024) rope_kernel(const Params p) {
     using PT = Pack<T, VEC>;
     using PF = Pack<float, VEC>;
+    pdl_trigger();
+    pdl_wait();
     const int64_t t = blockIdx.x;
     const int half = p.rot / 2;
     const int U = half / VEC, C = U + (p.D - p.rot) / VEC;  // pair chunks, then copied chunks
@@ -132,11 +134,9 @@ static int launch(const Params &p, int64_t tokens, bool half, bool vec, cudaStre
     if (nt < C) nt = C;
     nt = (nt + 31) / 32 * 32;
     const unsigned grid = (unsigned)tokens;
-    if (vec && half) rope_kernel<T, 8, true><<<grid, nt, 0, st>>>(p);
-    else if (vec) rope_kernel<T, 8, false><<<grid, nt, 0, st>>>(p);
-    else if (half) rope_kernel<T, 1, true><<<grid, nt, 0, st>>>(p);
-    else rope_kernel<T, 1, false><<<grid, nt, 0, st>>>(p);
-    QL_CUDA_TRY(cudaGetLastError());
+    auto kernel = vec ? (half ? rope_kernel<T, 8, true> : rope_kernel<T, 8, false>)
+                      : (half ? rope_kernel<T, 1, true> : rope_kernel<T, 1, false>);
+    QL_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(nt), 0, st, 1, p));
     return QL_OK;
 }
 
