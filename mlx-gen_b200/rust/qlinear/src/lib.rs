@@ -229,6 +229,96 @@ pub fn layernorm_modulate(x: DevicePtr, m: i64, d: i64, eps: f32, scale: Option<
     check(unsafe { sys::ql_layernorm_modulate(x.0, m, d, eps, p(scale), p(shift), period, y.0, y_dtype.raw(), stream.0) })
 }
 
+/// Geometry of a layer's key and value caches: `[num_pages, kv_heads, page_size, head_dim]` each,
+/// pages `page_stride` elements apart.
+#[derive(Debug, Clone, Copy)]
+pub struct PagedKv {
+    pub k: DevicePtr,
+    pub v: DevicePtr,
+    pub num_pages: i64,
+    pub page_stride: i64,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+}
+
+/// A `[tokens, heads, head_dim]` operand with its token and head strides in elements.
+#[derive(Debug, Clone, Copy)]
+pub struct Heads {
+    pub ptr: DevicePtr,
+    pub token_stride: i64,
+    pub head_stride: i64,
+}
+
+/// The norms around a decoder block without gate and modulation: `r = residual + alpha * y`,
+/// `h = rms(r) * weight` (contiguous rows; y, weight and h in `dtype`, residual and r in `r_dtype`).
+pub fn norm_residual(y: DevicePtr, dtype: Dtype, residual: DevicePtr, r_dtype: Dtype, m: i64, d: i64, weight: DevicePtr,
+                     alpha: f32, eps: f32, h: DevicePtr, r: DevicePtr, stream: Stream) -> Result<()> {
+    let null = std::ptr::null();
+    check(unsafe {
+        sys::ql_norm_residual(y.0, dtype.raw(), d, residual.0, r_dtype.raw(), d, m, d, weight.0, 0.0, null, null, 0, alpha,
+                              null, 0, eps, h.0, r.0, stream.0)
+    })
+}
+
+/// Rotary positions on q and k; k and v go to the cache at `slots`.  `layout`: `QL_ROPE_HALF` or
+/// `QL_ROPE_INTERLEAVED`; `table` `[table_rows, rotary_dim]` cosines, then sines, in f32.
+#[allow(clippy::too_many_arguments)]
+pub fn rope_append(q: Heads, k: Heads, v: Heads, dtype: Dtype, t: i64, q_heads: i32, kv: &PagedKv, rotary_dim: i32,
+                   layout: i32, table: DevicePtr, table_rows: i64, positions: DevicePtr, slots: DevicePtr,
+                   q_out: DevicePtr, stream: Stream) -> Result<()> {
+    check(unsafe {
+        sys::ql_rope_append(q.ptr.0, q.token_stride, q.head_stride, k.ptr.0, k.token_stride, k.head_stride, v.ptr.0,
+                            v.token_stride, v.head_stride, dtype.raw(), t, q_heads, kv.kv_heads, kv.head_dim, rotary_dim,
+                            layout, table.0 as *const f32, table_rows, positions.0 as *const i64, slots.0 as *const i64,
+                            kv.k.0, kv.v.0, kv.num_pages, kv.page_stride, kv.page_size, q_out.0, stream.0)
+    })
+}
+
+/// The sequences of an attention call: `page_table [b, table_stride]`, `q_starts [b + 1]`, `kv_lens [b]`
+/// (i32, on the device) and the host's bounds of the chunk and sequence lengths.
+#[derive(Debug, Clone, Copy)]
+pub struct Sequences {
+    pub page_table: DevicePtr,
+    pub table_stride: i64,
+    pub q_starts: DevicePtr,
+    pub kv_lens: DevicePtr,
+    pub b: i64,
+    pub max_q: i64,
+    pub max_kv: i64,
+}
+
+/// Bytes of workspace [`paged_attention`] needs (0: none).
+pub fn paged_attention_workspace(t: i64, q_heads: i32, kv: &PagedKv, s: &Sequences, window: i64) -> usize {
+    unsafe {
+        sys::ql_paged_attention_workspace_size(t, q_heads, kv.kv_heads, kv.head_dim, s.b, s.max_q, s.max_kv, window)
+    }
+}
+
+/// Attention of the sequences' new tokens over their pages; `out` `[t, q_heads, head_dim]`.
+#[allow(clippy::too_many_arguments)]
+pub fn paged_attention(q: Heads, dtype: Dtype, t: i64, q_heads: i32, kv: &PagedKv, s: &Sequences, scale: f32, causal: bool,
+                       window: i64, out: DevicePtr, workspace: DevicePtr, workspace_bytes: usize, stream: Stream) -> Result<()> {
+    check(unsafe {
+        sys::ql_paged_attention(q.ptr.0, dtype.raw(), q.token_stride, q.head_stride, t, q_heads, kv.kv_heads, kv.head_dim,
+                                kv.k.0, kv.v.0, kv.num_pages, kv.page_stride, kv.page_size, s.page_table.0 as *const i32,
+                                s.table_stride, s.q_starts.0 as *const i32, s.kv_lens.0 as *const i32, s.b, s.max_q,
+                                s.max_kv, scale, causal as i32, window, out.0, workspace.0, workspace_bytes, stream.0)
+    })
+}
+
+/// Copies pages `src[i]` to `dst[i]` in each of `planes` planes of a pool.
+pub fn copy_pages(pool: DevicePtr, planes: i64, plane_stride: i64, num_pages: i64, page_bytes: i64, src: &[i32],
+                  dst: &[i32], stream: Stream) -> Result<()> {
+    if src.len() != dst.len() {
+        return Err(Error::Msg { status: sys::QL_EINVAL_ARG, message: format!("{} sources for {} destinations", src.len(), dst.len()) });
+    }
+    check(unsafe {
+        sys::ql_copy_pages(pool.0, planes, plane_stride, num_pages, page_bytes, page_bytes, src.as_ptr(), dst.as_ptr(),
+                           src.len() as i64, stream.0)
+    })
+}
+
 /// Reads and clears the device error word (bounded-wait timeouts, bad gather ids).
 pub fn device_error() -> i32 {
     unsafe { sys::ql_device_error(1) }
