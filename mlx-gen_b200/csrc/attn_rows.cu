@@ -10,6 +10,9 @@
 // Softmax: running maximum and sum per row in fp32, weights 2^(s - max) <= 1 rounded to the
 // cache's type for the second product, the sum taken before that rounding.
 //
+// Measured: 64 sequences of 311 - 8003 positions (24 / 8 heads of 128) 179 us = 6.08 TB/s, 2 x 131k
+// positions 177 us = 6.04 TB/s (a copy: 6.56 TB/s), one sequence of 777 positions 6.2 us.
+//
 // Positions that no row of the CTA sees are zero-filled in shared memory, whatever the cache
 // holds there (a page's unused tail may hold anything); scores of positions that a row does
 // not see are replaced by -inf.
