@@ -2,7 +2,7 @@
 // (rows = new tokens x heads of a group, up to 16 at a time; more rows run as more CTAs).
 //
 // Bound: HBM -- every cached key and value is read once per kv head and 16 rows.  So the
-// kernel is built around the loads: each of a CTA's four warps walks its own blocks of 16
+// kernel is built around the loads: each of a CTA's four or eight warps walks its own blocks of 16
 // positions with its own ring of cp.async stages, with no barrier between the warps until the
 // end, and CTAs split a long axis (joined by join_kernel).  16 rows are one m16 tile of
 // mma.sync, whose operand layouts let the scores become the second product's operand in
@@ -11,7 +11,7 @@
 // cache's type for the second product, the sum taken before that rounding.
 //
 // Measured: 64 sequences of 311 - 8003 positions (24 / 8 heads of 128) 179 us = 6.08 TB/s, 2 x 131k
-// positions 177 us = 6.04 TB/s (a copy: 6.56 TB/s), one sequence of 777 positions 6.2 us.
+// positions 180 us = 5.95 TB/s (a copy: 6.56 TB/s), one sequence of 777 positions 6.2 us.
 //
 // Positions that no row of the CTA sees are zero-filled in shared memory, whatever the cache
 // holds there (a page's unused tail may hold anything); scores of positions that a row does
@@ -21,20 +21,21 @@
 namespace ql {
 namespace attn {
 
-constexpr int RW = 4;    // warps
 constexpr int RKV = 16;  // positions of one warp step
 
-template <int D>
+// ALONE: a CTA of eight warps that takes an SM's shared memory by itself (D = 256: four warps in
+// both cases), for one wave of CTAs.  Of four warps, two that would fit one to an SM each share
+// one while another SM idles (2 x 131k positions in 144 pieces: 221 us); kept apart by padding
+// they take 177 us, and 198 where the power cap lowers the clock; of eight warps 180 in both.
+template <int D, bool ALONE>
 struct RowsCfg {
+    static constexpr int RW = ALONE && D < 256 ? 8 : 4;  // warps
     static constexpr int ROW_BYTES = D * 2 + 16;  // padded: ldmatrix reads 8 rows free of bank conflicts
     static constexpr int TILE_BYTES = RKV * ROW_BYTES;
-    // stages so that two CTAs (one for D = 256) fill an SM's shared memory
+    // stages so that two CTAs of four warps (one for D = 256) fill an SM's shared memory
     static constexpr int STAGES = D == 64 ? 6 : D == 96 ? 4 : 3;
     static constexpr int WARP_BYTES = STAGES * 2 * TILE_BYTES;
     static constexpr int SMEM = RW * WARP_BYTES;
-    // more than half of an SM's: one CTA per SM.  Without it two of a wave that would fit one to an
-    // SM share one while others idle (2 x 131k positions in 144 pieces: 221 us instead of 177)
-    static constexpr int SMEM_ALONE = SMEM > 120000 ? SMEM : 120000;
     static_assert((RW + 1) * ROWS_TILE * (D + 2) * 4 <= SMEM, "the warps' and the CTA's results fit in the ring");
 };
 
@@ -84,10 +85,11 @@ __device__ __forceinline__ void mma16816<__half>(float c[4], const uint32_t a[4]
 
 // One stretch of positions [lo, hi) for one row block of a (sequence, kv head).  Its result is
 // partial result number `slot` of `slots`, or the output itself where slots is 1 (and not CLUSTER).
-template <typename T, int D, bool CLUSTER>
+template <typename T, int D, bool CLUSTER, bool ALONE>
 __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int b, int kvh, int rb, int lo, int hi, int slot,
                                              int slots, uint8_t *smem) {
-    using C = RowsCfg<D>;
+    using C = RowsCfg<D, ALONE>;
+    constexpr int RW = C::RW;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = s.q_len * p.G, r0 = rb * ROWS_TILE, nrows = min(ROWS_TILE, rows - r0);
 
@@ -227,7 +229,7 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
 
-    // the four warps' results meet in the ring's memory
+    // the warps' results meet in the ring's memory
     __syncthreads();
     float *so = reinterpret_cast<float *>(smem);        // [RW][16][D]
     float *sm = so + RW * ROWS_TILE * D, *sl = sm + RW * ROWS_TILE;
@@ -316,9 +318,8 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
 
 // The positions of one split when a few sequences (up to 32) are to fill the SMs, whatever their
 // lengths: of the candidates n = 1 .. nsplit pieces for the longest, the one whose waves of CTAs
-// (one per SM, see SMEM_ALONE) take the least time, a piece costing its positions and about 500
-// more.  Lane by lane, two candidates each.
-// (2 x 131k positions: 9 pieces in one wave 177 us, 64 of whatever placement 203.)
+// (one per SM) take the least time, a piece costing its positions and about 500 more.  Lane by
+// lane, two candidates each.  (2 x 131k positions: 9 pieces in one wave 180 us, 64 fixed 203.)
 __device__ __forceinline__ int adapted_chunk(const Params &p, int B) {
     const int lane = threadIdx.x & 31;
     int len = 0;
@@ -358,8 +359,8 @@ __device__ __forceinline__ int adapted_chunk(const Params &p, int B) {
 // grid: kv head * rowblocks + row block, sequence and split; the split runs fastest (x) with
 // CLUSTER and slowest (z) without, so that pieces which hold something come before empty ones and
 // the first of them go one to an SM.
-template <typename T, int D, bool CLUSTER>
-__global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowblocks) {
+template <typename T, int D, bool CLUSTER, bool ALONE>
+__global__ void __launch_bounds__(RowsCfg<D, ALONE>::RW * 32) rows_kernel(const Params p, int rowblocks) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_trigger();
     pdl_wait();
@@ -374,35 +375,37 @@ __global__ void __launch_bounds__(RW * 32) rows_kernel(const Params p, int rowbl
     if (r0 >= rows || rows > p.rows_kernel_most) return;
     int lo, hi;
     visible_rows(p, s, r0, min(rows, r0 + ROWS_TILE), lo, hi);
-    take_split(p, split, p.adapt ? adapted_chunk(p, gridDim.y) : p.chunk, lo, hi);
+    take_split(p, split, ALONE ? adapted_chunk(p, gridDim.y) : p.chunk, lo, hi);
     if (!CLUSTER && p.nsplit > 1 && lo >= hi) {  // nothing in this split
         const int r = threadIdx.x;
         if (r < min(ROWS_TILE, rows - r0))
             p.part_lse[((s.q0 + (int64_t)((r0 + r) / p.G)) * p.Hq + kvh * p.G + (r0 + r) % p.G) * p.nsplit + split] = NEG_INF;
         return;
     }
-    rows_stretch<T, D, CLUSTER>(p, s, b, kvh, rb, lo, hi, split, p.nsplit, smem);
+    rows_stretch<T, D, CLUSTER, ALONE>(p, s, b, kvh, rb, lo, hi, split, p.nsplit, smem);
 }
 
-template <typename T, int D, bool CLUSTER>
+template <typename T, int D, bool CLUSTER, bool ALONE>
 static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
-    using C = RowsCfg<D>;
-    auto kernel = rows_kernel<T, D, CLUSTER>;
+    using C = RowsCfg<D, ALONE>;
+    auto kernel = rows_kernel<T, D, CLUSTER, ALONE>;
     static PerDeviceFlag configured;
     const int dev = current_device();
     if (!configured.test(dev)) {
-        QL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_ALONE));
+        QL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         configured.set(dev);
     }
     const dim3 grid = CLUSTER ? dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B) : dim3(p.Hkv * rowblocks, (unsigned)B, p.nsplit);
-    QL_CUDA_TRY(launch_pdl(kernel, grid, dim3(RW * 32), p.adapt ? C::SMEM_ALONE : C::SMEM, st, CLUSTER ? p.nsplit : 1, p, rowblocks));
+    QL_CUDA_TRY(launch_pdl(kernel, grid, dim3(C::RW * 32), C::SMEM, st, CLUSTER ? p.nsplit : 1, p, rowblocks));
     return QL_OK;
 }
 
 template <typename T, int D>
 static int launch_rows_t(const Params &p, int64_t B, int64_t most_rows, cudaStream_t st) {
     const int rowblocks = (int)((most_rows + ROWS_TILE - 1) / ROWS_TILE);
-    return p.cluster ? launch_rows_c<T, D, true>(p, B, rowblocks, st) : launch_rows_c<T, D, false>(p, B, rowblocks, st);
+    if (p.cluster) return launch_rows_c<T, D, true, false>(p, B, rowblocks, st);
+    return p.adapt ? launch_rows_c<T, D, false, true>(p, B, rowblocks, st)
+                   : launch_rows_c<T, D, false, false>(p, B, rowblocks, st);
 }
 
 }  // namespace attn
