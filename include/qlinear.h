@@ -244,7 +244,8 @@ int ql_rope_append(const void *q, int64_t q_token_stride, int64_t q_head_stride,
  * q_starts[b] .. q_starts[b + 1] - 1 (q_starts [B + 1], covering 0 .. T), its cached positions
  * 0 .. kv_lens[b] - 1, its pages page_table[b * table_stride ..].  Token i of q_len stands at
  * p = kv_len - q_len + i and sees the positions j < kv_len, with causal j <= p, with window > 0
- * (needs causal) j > p - window.  A token that sees nothing gets zeros.  max_q / max_kv: upper
+ * (needs causal) j > p - window.  A token that sees nothing gets zeros (so does one all of whose
+ * scores are -inf); a NaN among a row's scores, or a score of +inf, makes the row NaN.  max_q / max_kv: upper
  * bounds of q_len / kv_len known to the host; a sequence beyond them, or a page index outside
  * the cache, sets the device error word (its output is unspecified).  Entries of the page table
  * and cache contents that no token of a sequence sees are not used.

@@ -141,7 +141,8 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 
 // Joins the partial results of the splits: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max)
 // with each o_s normalised and lse_s in base 2.  A split that a row sees nothing of has lse
-// -inf and an unwritten o_s, which is not read.  One warp per row.
+// -inf and an unwritten o_s, which is not read; one whose scores hold a NaN has lse NaN (which the
+// maximum leaves out) and makes the row NaN.  One warp per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const float *part_o, const float *part_lse, int64_t rows, int nsplit,
                                                    T *out) {
@@ -157,18 +158,17 @@ __global__ void __launch_bounds__(128) join_kernel(const float *part_o, const fl
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     constexpr int PER = D / 32;
     float acc[PER] = {}, total = 0.f;
-    if (mx != NEG_INF) {
-        for (int s = 0; s < nsplit; ++s) {
-            const float l = lse[s];
-            if (l == NEG_INF) continue;
-            const float w = ex2(l - mx);
-            total += w;
-            const float *o = part_o + (row * nsplit + s) * D;
+    const float base = mx == NEG_INF ? 0.f : mx;
+    for (int s = 0; s < nsplit; ++s) {
+        const float l = lse[s];
+        if (l == NEG_INF) continue;
+        const float w = ex2(l - base);
+        total += w;
+        const float *o = part_o + (row * nsplit + s) * D;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) acc[e] += w * o[e * 32 + lane];
-        }
+        for (int e = 0; e < PER; ++e) acc[e] += w * o[e * 32 + lane];
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const uint32_t v = pack2<T>(acc[e] * inv, 0.f);

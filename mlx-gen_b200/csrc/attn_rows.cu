@@ -254,19 +254,20 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
         float mx = NEG_INF;
 #pragma unroll
         for (int w = 0; w < RW; ++w) mx = fmaxf(mx, sm[w * ROWS_TILE + r]);
+        // (a maximum leaves NaN out: a warp whose scores are all NaN has -inf and a NaN sum, and 0 * NaN
+        // carries it on; one that saw nothing adds zeros)
+        const float base = mx == NEG_INF ? 0.f : mx;
         float total = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (mx != NEG_INF) {
 #pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                const float f = ex2(sm[w * ROWS_TILE + r] - mx);
-                const float4 v = *reinterpret_cast<const float4 *>(so + (w * ROWS_TILE + r) * D + e);
-                total += f * sl[w * ROWS_TILE + r];
-                a.x += f * v.x;
-                a.y += f * v.y;
-                a.z += f * v.z;
-                a.w += f * v.w;
-            }
+        for (int w = 0; w < RW; ++w) {
+            const float f = ex2(sm[w * ROWS_TILE + r] - base);
+            const float4 v = *reinterpret_cast<const float4 *>(so + (w * ROWS_TILE + r) * D + e);
+            total += f * sl[w * ROWS_TILE + r];
+            a.x += f * v.x;
+            a.y += f * v.y;
+            a.z += f * v.z;
+            a.w += f * v.w;
         }
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
         a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);

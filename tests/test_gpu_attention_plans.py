@@ -1,0 +1,81 @@
+"""GPU: paged attention under every division of the work -- one piece, splits joined in a cluster,
+pieces sized by the lengths, pieces of 2048 joined by a second launch, the tensor-core kernel whole
+and split, and batches that mix the two kernels."""
+import math
+
+import pytest
+import torch
+
+import qlinear
+from test_gpu_decoder import BF, HF, U, attention_reference, gen, paged, within
+
+pytestmark = pytest.mark.gpu
+
+# new tokens, lengths, q heads, kv heads, head size, whether partial results go through memory
+PLANS = {
+    "one piece": ([1, 1], [100, 20], 4, 2, 128, False),
+    "cluster": ([1, 2], [900, 300], 6, 2, 64, False),
+    "cluster, 256": ([40], [300], 4, 2, 256, False),
+    "by lengths": ([1, 1], [9000, 7000], 4, 2, 128, True),
+    "by lengths, 96": ([80], [7000], 4, 2, 96, True),
+    "pieces": ([1] * 40, [5000, 1, 3000, 20] * 10, 4, 2, 64, True),
+    "tiles": ([200], [300], 6, 2, 128, False),
+    "tiles, 64": ([200], [300], 6, 2, 64, False),
+    "tiles, split": ([200], [9000], 6, 2, 128, True),
+    "tiles, 64, split": ([200], [9000], 6, 2, 64, True),
+    "mixed": ([1, 200, 1], [9000, 300, 20], 6, 2, 128, True),
+}
+
+
+def planned(plan):
+    q_lens, kv_lens, Hq, Hkv, D, split = PLANS[plan]
+    need = qlinear.paged_attention_workspace_size(sum(q_lens), Hq, Hkv, D, len(q_lens), max(q_lens), max(kv_lens))
+    assert (need > 0) == split, plan
+    return q_lens, kv_lens, Hq, Hkv, D
+
+
+# ------------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_query_that_is_not_finite(plan, dtype, value):
+    """A query with a NaN (or an infinity, whose scores have a maximum of infinity) gives NaN and
+    not the zeros of a token that sees nothing; every other row is as before."""
+    q_lens, kv_lens, Hq, Hkv, D = planned(plan)
+    g = gen(len(plan))
+    q, kc, vc, table, starts, lens = paged(g, q_lens, kv_lens, Hq, Hkv, D, 16, dtype)
+    o, a = attention_reference(q, kc, vc, table, q_lens, kv_lens, D ** -0.5, True, 0)
+    hit = [(0, Hq - 1)] + ([(sum(q_lens) - 1, 0)] if sum(q_lens) > 1 else [])  # each sees 20 positions at least
+    q = q.clone()
+    for t, h in hit:
+        q[t, h, D // 3] = value
+    got = qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=max(q_lens), max_kv=max(kv_lens))
+    ok = torch.ones(got.shape[:2], dtype=torch.bool, device="cuda")
+    for t, h in hit:
+        assert got[t, h].isnan().all(), (t, h)
+        ok[t, h] = False
+    # weights and output rounded once to the dtype; scores below 2^7, so their fp32 rounding moves
+    # an exponent by 2^-24 * 64 * 2^7 at most; f16 weights under 2^-14 lose 2^-25 each
+    e = 2.0 ** -24 * 64 * 2 ** 7
+    low = max(kv_lens) * 2.0 ** -25 * 8 if dtype == HF else 0.0
+    within(got[ok], o[ok], (U[dtype] * (a + o.abs()) + 2 * e * a + low)[ok])
+    assert qlinear.device_error() == 0
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_key_that_is_not_a_number(plan):
+    """A NaN key reaches exactly the rows that see its position: all heads of its group, from its
+    token on."""
+    q_lens, kv_lens, Hq, Hkv, D = planned(plan)
+    g = gen(len(plan))
+    q, kc, vc, table, starts, lens = paged(g, q_lens, kv_lens, Hq, Hkv, D, 16, BF)
+    o, a = attention_reference(q, kc, vc, table, q_lens, kv_lens, D ** -0.5, True, 0)
+    at = max(0, kv_lens[0] - (q_lens[0] + 1) // 2)  # within the first sequence's new tokens
+    kc[table[0, at // 16].long(), Hkv - 1, at % 16, 5] = math.nan
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    first = at - (kv_lens[0] - q_lens[0])
+    bad[first:q_lens[0], Hq - Hq // Hkv:] = True
+    got = qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=max(q_lens), max_kv=max(kv_lens))
+    assert bad.any() and got[bad].isnan().all()
+    within(got[~bad], o[~bad], (U[BF] * (a + o.abs()) + 2 * 2.0 ** -24 * 64 * 2 ** 7 * a)[~bad])
