@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import heapq
 from dataclasses import dataclass
-from typing import Dict, List, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -32,6 +32,7 @@ class Step:
     kv_lens: torch.Tensor     # int32 [B], the new tokens included
     max_q: int
     max_kv: int
+    new_tokens: Optional[Tuple[int, ...]] = None  # of each sequence, on the host
 
 
 class PagedCache:
@@ -151,7 +152,7 @@ class PagedCache:
         small = torch.tensor(flat, dtype=torch.int32).to(dev, non_blocking=True)
         B = len(seqs)
         return Step(wide[0], wide[1], small[:B * width].view(B, width), small[B * width:B * width + B + 1],
-                    small[B * width + B + 1:], max(new_tokens), max(lens))
+                    small[B * width + B + 1:], max(new_tokens), max(lens), tuple(new_tokens))
 
     # ---- the pool
     def compact(self) -> int:

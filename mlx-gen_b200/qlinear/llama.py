@@ -76,8 +76,12 @@ class Decoder:
         return PagedCache(c.layers, c.kv_heads, c.head_dim, pages, page_size, device=self.norm.device)
 
     def forward(self, tokens: torch.Tensor, cache: PagedCache, step: Step) -> torch.Tensor:
-        """Logits of each sequence's last new token, [B, vocab]; the cache gets the new tokens."""
+        """Logits of each sequence's last new token, [B, vocab]; the cache gets the new tokens.  Every
+        sequence of the step needs one at least (ValueError; the cache counts the step's tokens all the
+        same, until they are truncated)."""
         c = self.config
+        if step.new_tokens is not None and min(step.new_tokens) == 0:
+            raise ValueError(f"a step with sequences without new tokens {step.new_tokens} has no logits for them")
         x = self.embedding(tokens).to(torch.bfloat16)
         T = x.shape[0]
         h, x = decoder.norm_residual(x, torch.zeros_like(x), self.layers[0].attn_norm, eps=c.eps)
