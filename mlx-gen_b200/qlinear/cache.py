@@ -32,7 +32,9 @@ class Step:
     kv_lens: torch.Tensor     # int32 [B], the new tokens included
     max_q: int
     max_kv: int
-    new_tokens: Optional[Tuple[int, ...]] = None  # of each sequence, on the host
+    # the same of each sequence on the host (max_q and max_kv may be replaced by upper bounds)
+    new_tokens: Optional[Tuple[int, ...]] = None
+    lengths: Optional[Tuple[int, ...]] = None
 
 
 class PagedCache:
@@ -152,7 +154,7 @@ class PagedCache:
         small = torch.tensor(flat, dtype=torch.int32).to(dev, non_blocking=True)
         B = len(seqs)
         return Step(wide[0], wide[1], small[:B * width].view(B, width), small[B * width:B * width + B + 1],
-                    small[B * width + B + 1:], max(new_tokens), max(lens), tuple(new_tokens))
+                    small[B * width + B + 1:], max(new_tokens), max(lens), tuple(new_tokens), tuple(lens))
 
     # ---- the pool
     def compact(self) -> int:

@@ -77,11 +77,13 @@ class Decoder:
 
     def forward(self, tokens: torch.Tensor, cache: PagedCache, step: Step) -> torch.Tensor:
         """Logits of each sequence's last new token, [B, vocab]; the cache gets the new tokens.  Every
-        sequence of the step needs one at least (ValueError; the cache counts the step's tokens all the
-        same, until they are truncated)."""
+        sequence of the step needs one at least, and none may pass the table's positions (ValueError;
+        the cache counts the step's tokens all the same, until they are truncated)."""
         c = self.config
         if step.new_tokens is not None and min(step.new_tokens) == 0:
             raise ValueError(f"a step with sequences without new tokens {step.new_tokens} has no logits for them")
+        if step.lengths is not None:
+            self._fits(max(step.lengths))
         x = self.embedding(tokens).to(torch.bfloat16)
         T = x.shape[0]
         h, x = decoder.norm_residual(x, torch.zeros_like(x), self.layers[0].attn_norm, eps=c.eps)
@@ -99,8 +101,14 @@ class Decoder:
         last = (step.q_starts[1:] - 1).long()
         return self.head.forward(h[last])
 
+    def _fits(self, length: int) -> None:
+        """The rotary table's end is known here; past it the kernels would give zeros and report it."""
+        if length > self.config.positions:
+            raise ValueError(f"a sequence of {length} tokens: the decoder's table holds {self.config.positions} positions")
+
     def generate(self, cache: PagedCache, seqs: Sequence[int], tokens: torch.Tensor, new: int) -> torch.Tensor:
         """Greedy continuation of sequences from their next tokens [B]: [B, new] token ids."""
+        self._fits(max(cache.length(s) for s in seqs) + new)
         out = []
         for _ in range(new):
             logits = self.forward(tokens, cache, cache.step(seqs, [1] * len(seqs)))
@@ -110,6 +118,7 @@ class Decoder:
 
     def prompt(self, cache: PagedCache, seq: int, tokens: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         """Appends a prompt [n] in chunks; returns the last token's logits [1, vocab]."""
+        self._fits(cache.length(seq) + tokens.shape[0])
         for at in range(0, tokens.shape[0], chunk):
             part = tokens[at:at + chunk]
             logits = self.forward(part, cache, cache.step([seq], [part.shape[0]]))

@@ -24,3 +24,17 @@ def test_forward_refuses_sequences_without_new_tokens(model, counts):
     step = c.step([c.new() for _ in counts], counts)
     with pytest.raises(ValueError, match="without new tokens"):
         model.forward(torch.zeros(sum(counts), dtype=torch.int64), c, step)
+
+
+def test_positions_past_the_table_are_refused(model):
+    c = cache()
+    a = c.new()
+    step = c.step([a], [41])
+    with pytest.raises(ValueError, match="40 positions"):
+        model.forward(torch.zeros(41, dtype=torch.int64), c, step)
+    c.truncate(a, 38)
+    with pytest.raises(ValueError, match="40 positions"):
+        model.prompt(c, a, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="40 positions"):
+        model.generate(c, [a], torch.zeros(1, dtype=torch.int64), 3)
+    assert c.length(a) == 38 and c.free_pages == 5  # refused before the cache changed
