@@ -114,10 +114,12 @@ class Decoder:
             logits = self.forward(tokens, cache, cache.step(seqs, [1] * len(seqs)))
             tokens = logits.argmax(-1)
             out.append(tokens)
-        return torch.stack(out, 1)
+        return torch.stack(out, 1) if out else tokens.new_empty((len(seqs), 0))
 
     def prompt(self, cache: PagedCache, seq: int, tokens: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         """Appends a prompt [n] in chunks; returns the last token's logits [1, vocab]."""
+        if tokens.shape[0] < 1 or chunk < 1:
+            raise ValueError(f"a prompt needs at least one token and a chunk of one (got {tokens.shape[0]} tokens, chunk {chunk})")
         self._fits(cache.length(seq) + tokens.shape[0])
         for at in range(0, tokens.shape[0], chunk):
             part = tokens[at:at + chunk]

@@ -38,3 +38,13 @@ def test_positions_past_the_table_are_refused(model):
     with pytest.raises(ValueError, match="40 positions"):
         model.generate(c, [a], torch.zeros(1, dtype=torch.int64), 3)
     assert c.length(a) == 38 and c.free_pages == 5  # refused before the cache changed
+
+
+def test_empty_prompts_and_continuations(model):
+    c = cache()
+    a = c.new()
+    with pytest.raises(ValueError, match="at least one token"):
+        model.prompt(c, a, torch.zeros(0, dtype=torch.int64))
+    with pytest.raises(ValueError, match="chunk"):
+        model.prompt(c, a, torch.zeros(3, dtype=torch.int64), chunk=0)
+    assert model.generate(c, [a], torch.zeros(1, dtype=torch.int64), 0).shape == (1, 0)
