@@ -10,7 +10,7 @@ the prompt's and the decode step's times.
 from __future__ import annotations
 
 import argparse
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
 import torch
@@ -22,6 +22,8 @@ from .nn import Linear, QuantizedLinear, TokenEmbedding
 
 @dataclass
 class Config:
+    """Llama-3.2-3B's sizes and rotary scaling (None: plain frequencies)."""
+
     hidden: int = 3072
     layers: int = 28
     heads: int = 24
@@ -31,7 +33,8 @@ class Config:
     vocab: int = 128256
     positions: int = 131072
     rope_base: float = 500000.0
-    rope_scaling: Optional[dict] = None
+    rope_scaling: Optional[dict] = field(default_factory=lambda: {
+        "type": "llama3", "factor": 32.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_positions": 8192})
     eps: float = 1e-5
     bits: int = 4
     group_size: int = 64

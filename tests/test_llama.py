@@ -48,3 +48,16 @@ def test_empty_prompts_and_continuations(model):
     with pytest.raises(ValueError, match="chunk"):
         model.prompt(c, a, torch.zeros(3, dtype=torch.int64), chunk=0)
     assert model.generate(c, [a], torch.zeros(1, dtype=torch.int64), 0).shape == (1, 0)
+
+
+def test_default_table_has_the_models_scaling():
+    """Llama-3.2-3B stretches a context of 8192: wavelengths above 8192 by 32, below 2048 not at all,
+    a linear blend (in turns) between."""
+    n, c = 64, Config()
+    f = c.rope_base ** (-torch.arange(n, dtype=torch.float64) / n)
+    turns = 8192 * f / (2 * torch.pi)
+    keep = ((turns - 1) / 3).clamp(0, 1)
+    a = (f * keep + f / 32 * (1 - keep)) * 1000
+    table = Decoder(Config(layers=0, positions=1001), None, [], torch.ones(1), None).table[1000].double()
+    # the angle in fp64, its cosine and sine rounded to fp32
+    assert float((table - torch.cat([a.cos(), a.sin()])).abs().max()) < 1e-6
