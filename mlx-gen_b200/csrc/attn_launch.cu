@@ -6,14 +6,16 @@
 namespace ql {
 namespace attn {
 
+constexpr double kMostPartial = 128 << 20;  // bytes of partial results of the small-row kernel's pieces
+
 struct Plan {
     int nsplit, chunk;
     bool adapt, cluster;
 };
 
 // The small-row kernel, for `items` (sequence, kv head, row block)s of up to `span` visible
-// positions each.
-static Plan plan_rows(int64_t B, int64_t items, int64_t span, bool window) {
+// positions each; `split_bytes`: the partial results of one split of every row.
+static Plan plan_rows(int64_t B, int64_t items, int64_t span, bool window, double split_bytes) {
     const int64_t pieces = (span + 127) / 128;  // at least 128 positions each
     if (pieces <= 1) return {1, 128, false, false};
     // Few items of moderate length: up to 8 splits in a cluster, one launch and no workspace.
@@ -41,9 +43,15 @@ static Plan plan_rows(int64_t B, int64_t items, int64_t span, bool window) {
     // sequences of 311 - 8003 positions whole 218 us, in pieces of 4096 / 2048 / 1024 positions 189
     // / 180 / 189; 10 of 20000 159 / 141 / 152; 16 of 4000 62 / 52 / 54).
     if (span <= 2048) return {1, 2048, false, false};
-    int64_t ns = (most + 2047) / 2048, chunk = 2048;
-    if (ns > 64) ns = 64, chunk = ((most + 63) / 64 + 127) / 128 * 128;
-    return {(int)ns, (int)chunk, false, false};
+    // Chunks of heads of 96 and 256 run here too, with row blocks that fill the SMs by themselves and
+    // gigabytes of partial results in such pieces: those are held to 128 MiB, by fewer, longer pieces
+    // (16 / 8 heads of 256, 4096 tokens over 32768 positions: 17 pieces 17.2 ms and 1092 MB, 2 pieces
+    // 13.8 ms; 512 over 131072: 64 pieces 9.0 ms, 16 pieces 7.7 ms; decode batches stay below it).
+    int64_t ns = (most + 2047) / 2048, fit = (int64_t)(kMostPartial / split_bytes);
+    fit = fit < 64 ? fit : 64;
+    if (fit <= 1) return {1, 128, false, false};
+    if (ns <= fit) return {(int)ns, 2048, false, false};
+    return {(int)fit, (int)(((most + fit - 1) / fit + 127) / 128 * 128), false, false};
 }
 
 // The tensor-core kernel runs one CTA per SM, so its splits fill whole waves: of all counts, the
@@ -92,7 +100,7 @@ static Kernels kernels_of(int Hq, int Hkv, int D, int64_t T, int64_t B, int64_t 
 static Plan make_plan(int Hq, int Hkv, int D, int64_t T, int64_t B, int64_t max_q, int64_t max_kv, int64_t window) {
     if (kernels_of(Hq, Hkv, D, T, B, max_q).tiles) return plan_tiles(T, Hq, Hkv, D, B, max_q, max_kv, window);
     const int64_t rowblocks = (max_q * (Hq / Hkv) + ROWS_TILE - 1) / ROWS_TILE, windowed = window ? window + max_q : max_kv;
-    return plan_rows(B, B * Hkv * rowblocks, windowed < max_kv ? windowed : max_kv, window != 0);
+    return plan_rows(B, B * Hkv * rowblocks, windowed < max_kv ? windowed : max_kv, window != 0, 4.0 * T * Hq * D);
 }
 
 static size_t lse_bytes(int64_t T, int Hq, int nsplit) { return ((size_t)T * Hq * nsplit * 4 + 255) / 256 * 256; }
