@@ -126,6 +126,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// log2 of the factor on the softmax's weights, which are at most 2^BOUND without it.  f16 holds 2^15 at
+// most and loses bits below 2^-14: with the factor that is 2^-(14 + shift), so a long tail that the sum
+// (fp32) counts in full is not rounded away before the second product (half a million weights of
+// 2^-24.9: the result 0.5 % off without it).  Sums and products carry the factor, which the division
+// cancels.  bf16 has fp32's range.
+template <typename T, int BOUND>
+constexpr float kWeightShift = __is_same(T, __half) ? 15.f - BOUND : 0.f;
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>

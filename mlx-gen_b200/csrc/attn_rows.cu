@@ -7,8 +7,8 @@
 // end, and CTAs split a long axis (joined by join_kernel).  16 rows are one m16 tile of
 // mma.sync, whose operand layouts let the scores become the second product's operand in
 // registers; a 128-row tcgen05 tile would spend its softmax on rows that do not exist.
-// Softmax: running maximum and sum per row in fp32, weights 2^(s - max) <= 1 rounded to the
-// cache's type for the second product, the sum taken before that rounding.
+// Softmax: running maximum and sum per row in fp32, weights 2^(s - max) <= 1 (in f16 times 2^15:
+// kWeightShift) rounded to the cache's type for the second product, the sum taken before that rounding.
 //
 // Measured: 64 sequences of 311 - 8003 positions (24 / 8 heads of 128) 179 us = 6.08 TB/s, 2 x 131k
 // positions 180 us = 5.95 TB/s (a copy: 6.56 TB/s), one sequence of 777 positions 6.2 us.
@@ -90,6 +90,7 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
                                              int slots, uint8_t *smem) {
     using C = RowsCfg<D, ALONE>;
     constexpr int RW = C::RW;
+    constexpr float SHIFT = kWeightShift<T, 0>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = s.q_len * p.G, r0 = rb * ROWS_TILE, nrows = min(ROWS_TILE, rows - r0);
 
@@ -192,6 +193,7 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
             moved |= nm != m[r];
             base[r] = nm == NEG_INF ? 0.f : nm;  // nothing seen yet: every weight is 2^-inf = 0
             f[r] = ex2(m[r] - base[r]);
+            base[r] -= SHIFT;
             m[r] = nm;
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -271,7 +273,7 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
         }
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
         a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-        const float lse = total > 0.f || total != total ? mx + log2f(total) : NEG_INF;
+        const float lse = total > 0.f || total != total ? mx + (log2f(total) - SHIFT) : NEG_INF;
         if (CLUSTER) {
             if (e == 0) jl[r] = lse;
             *reinterpret_cast<float4 *>(jo + r * D + e) = a;

@@ -21,8 +21,9 @@
 // K / V stages in 128-byte swizzled rows of 64 elements.
 //
 // The running maximum is lazy: O and l are rescaled only when a row's maximum rises by more
-// than 2^8 over the one in use; until then the weights may exceed 1 (by up to 2^8: exact in
-// every format's range), which the final division by l cancels.  O is rescaled by the softmax
+// than 2^8 over the one in use; until then the weights may exceed 1 (by up to 2^8, for which every
+// format has room; f16 takes the rest of its range for small weights, kWeightShift), which the
+// final division by l cancels.  O is rescaled by the softmax
 // threads: S_t of step j is committed after O_t of step j - 1, so seeing it means O_t is at
 // rest.  The same order lets S_t of step j + 1 overwrite P_t of step j: both products are
 // issued by one thread and execute in order.
@@ -108,6 +109,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     // with P_t beside S_t the next scores are ready early and the tiles' softmaxes overlap freely
     // (with turns the same: 89 us on the mixed batch either way)
     constexpr bool TURNS = !C::P_APART;
+    constexpr float SHIFT = kWeightShift<T, 8>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::SMEM_BAR);  // K / V stage landed
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     ok = __all_sync(0xffffffffu, mbar_wait(&turn[t], (t == 1 ? j : j - 1) & 1, abort_flag, DEV_ERR_TIMEOUT_ACC));
                     if (!ok) break;
                 }
-                const uint64_t c2 = f2_make(c, c), nb2 = f2_make(-base, -base);
+                const uint64_t c2 = f2_make(c, c), nb2 = f2_make(SHIFT - base, SHIFT - base);
                 auto hand_over = [&](int h) {  // P_t's positions so far are in TMEM
                     tmem_st_wait();
                     tc_fence_before();
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 const int64_t row = (s.q0 + (int64_t)(r / p.G)) * p.Hq + kvh * p.G + r % p.G;
                 const bool seen = m != NEG_INF || l != l;
                 if (p.nsplit > 1 && r < rows)
-                    p.part_lse[row * p.nsplit + split] = seen ? fmaf(m, c, log2f(l)) : NEG_INF;
+                    p.part_lse[row * p.nsplit + split] = seen ? fmaf(m, c, log2f(l) - SHIFT) : NEG_INF;
 #pragma unroll 1
                 for (int i = 0; i < D / 32; ++i) {
                     uint32_t o[32];

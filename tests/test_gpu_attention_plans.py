@@ -79,3 +79,24 @@ def test_key_that_is_not_a_number(plan):
     got = qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=max(q_lens), max_kv=max(kv_lens))
     assert bad.any() and got[bad].isnan().all()
     within(got[~bad], o[~bad], (U[BF] * (a + o.abs()) + 2 * 2.0 ** -24 * 64 * 2 ** 7 * a)[~bad])
+
+
+# ------------------------------------------------------------------------ f16 weights
+
+@pytest.mark.parametrize("D,Hkv,T", [(64, 8, 16384), (128, 8, 16384), (256, 8, 16384), (128, 1, 1)])
+def test_f16_keeps_the_weight_of_a_long_tail(D, Hkv, T):
+    """One score above 524287 others by so much that each of them weighs 2^-24.9 of it: together 1.7 %
+    of the sum, each half a step of f16's smallest numbers.  With every value 1 the result is 1."""
+    n, ps = 524288, 128
+    kc = torch.zeros(n // ps, Hkv, ps, D, dtype=HF, device="cuda")
+    vc = torch.ones_like(kc)
+    kc[0, :, 0, 0] = 24.91 * math.log(2)
+    q = torch.zeros(T, Hkv, D, dtype=HF, device="cuda")
+    q[..., 0] = 1
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = qlinear.paged_attention(q, kc, vc, torch.arange(n // ps, **i32)[None], torch.tensor([0, T], **i32), torch.tensor([n], **i32),
+                                  max_q=T, max_kv=n, scale=1.0, causal=False)
+    # the output's rounding (2^-11), and at most 2^-23 of the fp32 accumulator in each product of 16
+    # positions, of which a piece with the high score has up to 131072 for a warp or tile
+    assert float((got.double() - 1).abs().max()) <= 2.0 ** -11 + 131072 / 16 * 2.0 ** -23
+    assert qlinear.device_error() == 0
