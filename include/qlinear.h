@@ -249,7 +249,8 @@ int ql_rope_append(const void *q, int64_t q_token_stride, int64_t q_head_stride,
  * bounds of q_len / kv_len known to the host; a sequence beyond them, or a page index outside
  * the cache, sets the device error word (its output is unspecified).  Entries of the page table
  * and cache contents that no token of a sequence sees are not used.
- * dtype bf16 or f16; D 64, 96, 128 or 256; page_size a power of two in [16, 1024]; fp32
+ * dtype bf16 or f16; D 64, 96, 128 or 256; page_size a power of two in [16, 1024]; at most 65535
+ * sequences; max_q * Hq / Hkv at most 16776960 (D 64, 128) or 2^30, max_kv at most 2^30; fp32
  * softmax, the weights rounded to dtype for the second product.  q and the caches 16-byte
  * aligned, q's strides multiples of 8; out and workspace (see below) 32-byte aligned. */
 int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,

@@ -35,8 +35,11 @@ static int check_attention(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t
         return fail(QL_EUNSUPPORTED, "head dimension must be 64, 96, 128 or 256 (got %d)", D);
     if (max_q < 0 || max_q > T || max_kv < 0 || max_kv > (1 << 30))
         return fail(QL_EINVAL_SHAPE, "max_q=%lld must be in [0, T], max_kv=%lld in [0, 2^30]", (long long)max_q, (long long)max_kv);
-    if (max_q * (Hq / Hkv) > (1 << 30) || (max_q * (Hq / Hkv) + 15) / 16 * Hkv > 65535)
-        return fail(QL_EUNSUPPORTED, "max_q * Hq = %lld is too large for one call; split the chunk", (long long)(max_q * Hq));
+    // rows of a kv head: ints in the kernels; row blocks of 16 times Hkv are a grid's x, tiles of 256
+    // (heads of 64 and 128) its y
+    const int64_t rows = max_q * (Hq / Hkv);
+    if (rows > (1 << 30) || (rows + 15) / 16 * Hkv > INT32_MAX || ((D == 64 || D == 128) && rows > (int64_t)65535 * attn::SM100_ROWS))
+        return fail(QL_EUNSUPPORTED, "max_q * Hq / Hkv = %lld is too large for one call; split the chunk", (long long)rows);
     return QL_OK;
 }
 

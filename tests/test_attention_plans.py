@@ -2,6 +2,8 @@
 import pytest
 
 import qlinear
+from qlinear import _lib
+from test_decoder import _attention
 
 MB = 1 << 20
 
@@ -21,3 +23,18 @@ def test_decode_batches_keep_their_pieces():
     lse = lambda n: -(-64 * 24 * n * 4 // 256) * 256  # noqa: E731
     for span, pieces in ((8003, 4), (65536, 33), (131071, 64)):
         assert qlinear.paged_attention_workspace_size(64, 24, 8, 128, 64, 1, span) == lse(pieces) + 64 * 24 * pieces * 128 * 4
+
+
+def test_long_chunks_are_refused_only_where_a_grid_ends():
+    """scale=-1 is refused after the sizes: a call that gets there has sizes that can run."""
+    call = lambda **kw: _attention(_lib.lib(), **{**dict(scale=-1.0, pst=1 << 40, P=1 << 20, tst=1 << 20), **kw})  # noqa: E731
+    for D in (64, 96, 128, 256):
+        for Hq, Hkv in ((24, 8), (16, 1), (8, 8)):
+            n = 1 << 20
+            assert call(T=n, mq=n, mk=n, Hq=Hq, Hkv=Hkv, D=D) == (_lib.QL_EUNSUPPORTED if D in (64, 128) and Hq == 16 else _lib.QL_EINVAL_ARG)
+            n = 65535 * 256 * Hkv // Hq  # rows of a kv head in 65535 tiles of 256
+            assert call(T=n, mq=n, mk=n, Hq=Hq, Hkv=Hkv, D=D) == _lib.QL_EINVAL_ARG
+    n = 65535 * 256 + 1
+    assert call(T=n, mq=n, mk=n, Hq=4, Hkv=4, D=128) == _lib.QL_EUNSUPPORTED and call(T=n, mq=n, mk=n, Hq=4, Hkv=4, D=96) == _lib.QL_EINVAL_ARG
+    n = (1 << 30) + 1
+    assert call(T=n, mq=n, mk=100, Hq=4, Hkv=4, D=96) == _lib.QL_EUNSUPPORTED

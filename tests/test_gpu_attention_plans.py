@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import qlinear
-from test_gpu_decoder import BF, HF, U, attention_reference, gen, paged, within
+from test_gpu_decoder import BF, HF, U, attention_reference, gen, paged, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -99,4 +99,26 @@ def test_f16_keeps_the_weight_of_a_long_tail(D, Hkv, T):
     # the output's rounding (2^-11), and at most 2^-23 of the fp32 accumulator in each product of 16
     # positions, of which a piece with the high score has up to 131072 for a warp or tile
     assert float((got.double() - 1).abs().max()) <= 2.0 ** -11 + 131072 / 16 * 2.0 ** -23
+    assert qlinear.device_error() == 0
+
+
+# ------------------------------------------------------------------------ long chunks
+
+@pytest.mark.parametrize("D", [64, 96, 128])
+def test_chunk_of_more_than_a_million_rows(D):
+    """70000 tokens of 16 heads on one kv head, each seeing 50 positions."""
+    n, H, W, ps = 70000, 16, 50, 64
+    g = gen(D)
+    q, cache = rnd(g, n, H, D), rnd(g, -(-n // ps), 2, ps, D)
+    kc, vc = cache[:, :1], cache[:, 1:]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = qlinear.paged_attention(q, kc, vc, torch.arange(-(-n // ps), **i32)[None], torch.tensor([0, n], **i32), torch.tensor([n], **i32),
+                                  max_q=n, max_kv=n, window=W)
+    at = torch.cat([torch.arange(64), torch.arange(64, n, 61), torch.arange(n - 64, n)]).cuda()
+    pos = at[:, None] - W + 1 + torch.arange(W, device="cuda")
+    k, v = (c.reshape(-1, D)[pos.clamp(min=0)].double() for c in (kc, vc))
+    s = torch.einsum("ihd,ijd->ihj", q[at].double(), k) * D ** -0.5
+    p = s.masked_fill((pos < 0)[:, None], -math.inf).softmax(-1)
+    o, a = torch.einsum("ihj,ijd->ihd", p, v), torch.einsum("ihj,ijd->ihd", p, v.abs())
+    within(got[at], o, U[BF] * (a + o.abs()) + 2 * 2.0 ** -24 * 64 * 2 ** 7 * a)
     assert qlinear.device_error() == 0
