@@ -126,7 +126,8 @@ int ql_device_error(int clear);
  * device error word (read with ql_device_error), every role drains, TMEM is freed and the
  * kernel returns; the context stays usable.  wait_limit_ns replaces the 2 s limit on the
  * current device (0 restores it); flags bit 0 makes the tcgen05 GEMM's TMA producer issue
- * nothing, bit 1 the tcgen05 attention's, so their consumers' waits run out.  Synchronises the current device.  Not for
+ * nothing, bit 1 the tcgen05 attention's, bit 2 makes that one stop half-way, so their consumers'
+ * waits run out.  Synchronises the current device.  Not for
  * production use: set flags back to 0 afterwards. */
 int ql_debug_inject(unsigned flags, unsigned long long wait_limit_ns);
 

@@ -80,6 +80,11 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
 // the n lowest bits (none for n <= 0, all for n >= 32)
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+// Barrier 1: the loader and the issuers (and warp 11) wait until every role is done, so that none sets the
+// abort flag any more; the softmax warps only arrive.
+__device__ __forceinline__ void roles_done() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(SM100_THREADS) : "memory"); }
+__device__ __forceinline__ void softmax_done() { asm volatile("barrier.cta.arrive 1, %0;" ::"n"(SM100_THREADS) : "memory"); }
+
 // 32 bytes in one store: a whole DRAM sector of a thread's own row
 __device__ __forceinline__ void st_global_32(void *dst, const uint32_t v[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
@@ -370,12 +375,16 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     __syncwarp();
                 }
             }
+            tmem_st_wait();  // (an aborted step's rescaling)
             tc_fence_before();
         }
+        softmax_done();
     } else if (warp == 8) {
         // ---------------------------------------------------------------- K / V loads
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (!(*reinterpret_cast<volatile unsigned *>(&g_debug_inject) & 2u)) {
+        const unsigned inject = *reinterpret_cast<volatile unsigned *>(&g_debug_inject);
+        if (!(inject & 2u)) {
+            const int loads = inject & 4u ? n : 2 * n;  // of K and V, one each a step (n: the test hook's half)
             const int ps = 1 << p.page_shift, box = min(ps, TKV), nb = TKV / box;
             // clears what no row sees in V of step j, once it has landed; only this warp refills
             // the stage, so its barrier still stands at that load
@@ -403,7 +412,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             int it = 0, page = 0, ahead[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) ahead[j] = page_index(j);
-            for (; it < 2 * n; ++it) {
+            for (; it < loads; ++it) {
                 if (it == min(STAGES, 2 * n - 1) && fix_first && n > 1) clear_v(0, &vfix[0]);
                 const int st = it % STAGES, pos = (t0 + (it >> 1)) * TKV + lane * box;
                 const bool in = lane < nb && pos < vhi && pos + box > vlo;
@@ -433,15 +442,20 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 if (n == 1 && (fix_first || fix_last)) clear_v(0, &vfix[0]);
                 if (fix_last && n > 1) clear_v(n - 1, &vfix[1]);
             }
-            if (*abort_flag) {  // let the copies in flight land before the CTA's memory is given up
+            // after an abort, whichever wait ran out, the copies land before their memory is given up
+            roles_done();
+            if (*abort_flag) {
                 const uint64_t from = globaltimer_ns();
                 for (int i = max(0, it - STAGES); i < it; ++i)
                     while (!mbar_try_wait(&full[i % STAGES], (i / STAGES) & 1) && globaltimer_ns() - from < 100000000ull) {
                     }
             }
+        } else {
+            roles_done();
         }
     } else if (warp == 11) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        roles_done();
     } else {
         // ---------------------------------------------------------------- MMAs of tile t
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -492,11 +506,13 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     if (ok) tc_commit(&sfull[t]);
                 }
             }
-            if (!ok) {  // aborted: the MMAs issued so far finish before TMEM is freed
-                tc_commit(&drain[t]);
-                const uint64_t from = globaltimer_ns();
-                while (!mbar_try_wait(&drain[t], 0) && globaltimer_ns() - from < 100000000ull) {
-                }
+        }
+        __syncwarp();
+        roles_done();
+        if (*abort_flag && lane == 0) {  // the same for the products, before TMEM is freed
+            tc_commit(&drain[t]);
+            const uint64_t from = globaltimer_ns();
+            while (!mbar_try_wait(&drain[t], 0) && globaltimer_ns() - from < 100000000ull) {
             }
         }
     }

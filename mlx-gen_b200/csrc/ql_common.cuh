@@ -226,7 +226,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 // The limit in force (kWaitLimitNs unless a test shortened it through ql_debug_inject), and
 // the test hook's injection flags (bit 0: the tcgen05 GEMM's TMA producer issues nothing, bit
-// 1: the tcgen05 attention's).
+// 1: the tcgen05 attention's, bit 2: that one stops half-way).
 __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
 __device__ unsigned g_debug_inject = 0;
 

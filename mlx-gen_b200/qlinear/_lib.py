@@ -146,13 +146,14 @@ def check(status: int) -> None:
 DEV_ERR_TIMEOUT_FULL, DEV_ERR_TIMEOUT_EMPTY, DEV_ERR_TIMEOUT_ACC, DEV_ERR_BAD_INDEX = 1, 2, 4, 8
 INJECT_GEMM_PRODUCER_SILENT = 1
 INJECT_ATTENTION_PRODUCER_SILENT = 2
+INJECT_ATTENTION_PRODUCER_STOPS = 4
 
 
 def debug_inject(flags: int = 0, wait_limit_ns: int = 0) -> None:
     """Test hook (ql_debug_inject): shortens every kernel's bounded wait to `wait_limit_ns`
     (0 = the 2 s default) and sets injection flags (INJECT_GEMM_PRODUCER_SILENT: the tcgen05
     GEMM's TMA producer issues nothing, INJECT_ATTENTION_PRODUCER_SILENT: the tcgen05 attention's,
-    so that their consumers' waits run out)."""
+    INJECT_ATTENTION_PRODUCER_STOPS: that one stops half-way, so that their consumers' waits run out)."""
     check(lib().ql_debug_inject(int(flags), int(wait_limit_ns)))
 
 

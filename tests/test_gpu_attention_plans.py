@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import qlinear
+from qlinear import _lib
 from test_gpu_decoder import BF, HF, U, attention_reference, gen, paged, rnd, within
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +123,25 @@ def test_chunk_of_more_than_a_million_rows(D):
     o, a = torch.einsum("ihj,ijd->ihd", p, v), torch.einsum("ihj,ijd->ihd", p, v.abs())
     within(got[at], o, U[BF] * (a + o.abs()) + 2 * 2.0 ** -24 * 64 * 2 ** 7 * a)
     assert qlinear.device_error() == 0
+
+
+# ------------------------------------------------------------------------ waits that run out under way
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("q_len,kv", [(4096, 4096), (200, 9000), (400, 700), (130, 130)])
+def test_loader_that_stops_half_way(D, q_len, kv):
+    """With half of each CTA's loads (a flag that only this sets) and the wait limit at 20 ms, a launch
+    that has products and copies behind it ends by itself and says so, and the next call is right."""
+    g = gen(D + kv)
+    q, kc, vc, table, starts, lens = paged(g, [q_len], [kv], 6, 2, D, 16, BF)
+    call = lambda: qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=q_len, max_kv=kv)  # noqa: E731
+    want = call()
+    assert qlinear.device_error() == 0
+    try:
+        _lib.debug_inject(_lib.INJECT_ATTENTION_PRODUCER_STOPS, 20_000_000)
+        call()
+        err = qlinear.device_error()
+    finally:
+        _lib.debug_inject(0, 0)
+    assert err & (_lib.DEV_ERR_TIMEOUT_FULL | _lib.DEV_ERR_TIMEOUT_EMPTY | _lib.DEV_ERR_TIMEOUT_ACC)
+    assert torch.equal(call(), want) and qlinear.device_error() == 0
