@@ -164,7 +164,7 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
                     (long long)table_stride, (long long)max_kv);
     if (!(scale > 0.f) || !isfinite(scale)) return fail(QL_EINVAL_ARG, "scale must be positive and finite");
     if (window < 0 || (window && !causal)) return fail(QL_EINVAL_ARG, "window must be >= 0, and needs causal");
-    if (T == 0 || B == 0 || max_q == 0) return QL_OK;
+    if (T == 0 || B == 0) return QL_OK;
     if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
         return fail(QL_EINVAL_ARG, "ql_paged_attention: NULL pointer");
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned32(out) || q_token_stride % 8 ||

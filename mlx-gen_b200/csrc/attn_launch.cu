@@ -97,9 +97,12 @@ static Kernels kernels_of(int Hq, int Hkv, int D, int64_t T, int64_t B, int64_t 
     return {T < B * max_q, true};  // all chunks of the longest length: none is short
 }
 
+// Row blocks of a sequence; one even where the bound is no rows, to report sequences that have some.
+static int64_t row_blocks(int64_t rows) { return rows > 0 ? (rows + ROWS_TILE - 1) / ROWS_TILE : 1; }
+
 static Plan make_plan(int Hq, int Hkv, int D, int64_t T, int64_t B, int64_t max_q, int64_t max_kv, int64_t window) {
     if (kernels_of(Hq, Hkv, D, T, B, max_q).tiles) return plan_tiles(T, Hq, Hkv, D, B, max_q, max_kv, window);
-    const int64_t rowblocks = (max_q * (Hq / Hkv) + ROWS_TILE - 1) / ROWS_TILE, windowed = window ? window + max_q : max_kv;
+    const int64_t rowblocks = row_blocks(max_q * (Hq / Hkv)), windowed = window ? window + max_q : max_kv;
     return plan_rows(B, B * Hkv * rowblocks, windowed < max_kv ? windowed : max_kv, window != 0, 4.0 * T * Hq * D);
 }
 
@@ -114,8 +117,8 @@ static int launch_t(Params &p, int64_t B, cudaStream_t st) {
             if (int rc = launch_sm100_t<T, D>(p, B, st)) return rc;
     }
     if (ks.rows) {
-        const int64_t most = (int64_t)p.max_q * p.G;
-        if (int rc = launch_rows_t<T, D>(p, B, ks.tiles ? ROWS_TILE : most, st)) return rc;
+        const int blocks = ks.tiles ? 1 : (int)row_blocks((int64_t)p.max_q * p.G);
+        if (int rc = launch_rows_t<T, D>(p, B, blocks, st)) return rc;
     }
     return p.nsplit > 1 && !p.cluster ? launch_join<T, D>(p, st) : QL_OK;
 }

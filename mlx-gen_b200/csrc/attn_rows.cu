@@ -404,8 +404,7 @@ static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t
 }
 
 template <typename T, int D>
-static int launch_rows_t(const Params &p, int64_t B, int64_t most_rows, cudaStream_t st) {
-    const int rowblocks = (int)((most_rows + ROWS_TILE - 1) / ROWS_TILE);
+static int launch_rows_t(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
     if (p.cluster) return launch_rows_c<T, D, true, false>(p, B, rowblocks, st);
     return p.adapt ? launch_rows_c<T, D, false, true>(p, B, rowblocks, st)
                    : launch_rows_c<T, D, false, false>(p, B, rowblocks, st);

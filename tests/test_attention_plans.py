@@ -38,3 +38,13 @@ def test_long_chunks_are_refused_only_where_a_grid_ends():
     assert call(T=n, mq=n, mk=n, Hq=4, Hkv=4, D=128) == _lib.QL_EUNSUPPORTED and call(T=n, mq=n, mk=n, Hq=4, Hkv=4, D=96) == _lib.QL_EINVAL_ARG
     n = (1 << 30) + 1
     assert call(T=n, mq=n, mk=100, Hq=4, Hkv=4, D=96) == _lib.QL_EUNSUPPORTED
+
+
+def test_any_sizes_have_an_answer():
+    """No new tokens, nothing cached, bounds at their ends: the query returns."""
+    ask = qlinear.paged_attention_workspace_size
+    for D in (64, 96, 128, 256):
+        for max_q in (0, 1, 41):
+            for max_kv in (0, 1, 300, 7000, 1 << 30):
+                for B in (0, 1, 2, 40):
+                    assert ask(41, 6, 2, D, B, max_q, max_kv) >= 0 and ask(41, 6, 2, D, B, max_q, max_kv, 64) >= 0

@@ -145,3 +145,16 @@ def test_loader_that_stops_half_way(D, q_len, kv):
         _lib.debug_inject(0, 0)
     assert err & (_lib.DEV_ERR_TIMEOUT_FULL | _lib.DEV_ERR_TIMEOUT_EMPTY | _lib.DEV_ERR_TIMEOUT_ACC)
     assert torch.equal(call(), want) and qlinear.device_error() == 0
+
+
+# ------------------------------------------------------------------------ bounds that are too low
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_a_bound_of_no_new_tokens_is_reported(D):
+    """max_q = 0 with tokens there: the error word is set, as for every bound that is too low."""
+    q, kc, vc, table, starts, lens = paged(gen(D), [1, 40], [10, 300], 6, 2, D, 16, BF)
+    assert qlinear.device_error() == 0
+    qlinear.paged_attention(q, kc, vc, table, starts, lens, max_q=0, max_kv=300)
+    assert qlinear.device_error() == _lib.DEV_ERR_BAD_INDEX
+    qlinear.paged_attention(q, kc, vc, table, torch.zeros_like(starts), lens, max_q=0, max_kv=300)  # no sequence has any
+    assert qlinear.device_error() == 0
