@@ -8,7 +8,7 @@ import torch
 
 import qlinear
 from qlinear import _lib
-from test_gpu_decoder import BF, HF, U, attention_reference, gen, paged, rnd, within
+from test_gpu_decoder import BF, HF, U, attention_reference, check_attention, gen, paged, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,49 @@ def test_a_bound_of_no_new_tokens_is_reported(D):
     assert qlinear.device_error() == _lib.DEV_ERR_BAD_INDEX
     qlinear.paged_attention(q, kc, vc, table, torch.zeros_like(starts), lens, max_q=0, max_kv=300)  # no sequence has any
     assert qlinear.device_error() == 0
+
+
+# ------------------------------------------------------------------------ every plan against 64 bits
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_pieces_of_many_sequences(D, dtype):
+    """More than 32 sequences over 2048 positions: fixed pieces, many of them empty."""
+    kv = [1, 5000, 2048, 2049, 17, 4096, 4097, 300] * 5
+    assert qlinear.paged_attention_workspace_size(40, 4, 2, D, 40, 1, 5000) > 0
+    check_attention(gen(D), [1] * 40, kv, 4, 2, D, 64, dtype)
+
+
+@pytest.mark.parametrize("D,causal,window", [(64, True, 0), (128, True, 0), (128, False, 0), (128, True, 3000), (256, True, 0)])
+def test_pieces_under_a_bound_far_above_the_lengths(D, causal, window):
+    """A bound of 140000 positions (what a captured graph is given): 64 longer pieces, nearly all empty."""
+    q_lens, kv, bound = [1] * 40, [1, 4000, 2600, 700] * 10, 140000
+    g = gen(D + window)
+    q, kc, vc, table, starts, lens = paged(g, q_lens, kv, 4, 2, D, 64, BF)
+    wide = torch.full((40, -(-bound // 64)), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    got = qlinear.paged_attention(q, kc, vc, wide, starts, lens, max_q=1, max_kv=bound, causal=causal, window=window)
+    o, a = attention_reference(q, kc, vc, table, q_lens, kv, D ** -0.5, causal, window)
+    within(got, o, U[BF] * (a + o.abs()) + 2 * 2.0 ** -24 * 64 * 2 ** 7 * a)
+    assert qlinear.device_error() == 0
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kv,window", [([20011], 0), ([7000, 1], 0), ([9000, 12001, 6400], 0), ([20011, 300, 7001], 6500)])
+def test_pieces_by_lengths(D, dtype, kv, window):
+    """A few sequences over 6000 positions: the kernel divides them by their lengths."""
+    assert qlinear.paged_attention_workspace_size(len(kv), 6, 2, D, len(kv), 1, max(kv), window) > 0
+    check_attention(gen(D + len(kv)), [1] * len(kv), kv, 6, 2, D, 32, dtype, True, window)
+
+
+@pytest.mark.parametrize("kv", [[700, 130, 2, 1], [5000], [9000, 6100], [12000] * 3])
+@pytest.mark.parametrize("D,causal,window", [(64, False, 0), (128, False, 0), (64, True, 1), (128, True, 100), (128, True, 2500)])
+def test_single_tokens_with_masks(kv, D, causal, window):
+    check_attention(gen(window + len(kv)), [1] * len(kv), kv, 4, 2, D, 16, BF, causal, window)
+
+
+@pytest.mark.parametrize("D", [64, 96, 256])
+@pytest.mark.parametrize("q_len", [2, 150])
+def test_long_contexts_of_other_head_sizes(D, q_len):
+    check_attention(gen(D + q_len), [q_len, q_len], [9001, 1000], 6, 2, D, 64)
