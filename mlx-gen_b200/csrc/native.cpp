@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/api/include/torch/version.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -357,4 +358,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__native() { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__native() {
+    PyObject *m = PyModule_Create(&g_module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
+}

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import re
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -29,6 +30,8 @@ class _Native:
         if not os.path.exists(path):
             raise ImportError(f"{path} not found; build it first (python -c 'import __graft_entry__ as g; g.build()')")
         from . import _native as m
+        if not re.match(re.escape(m.torch_version) + r"(?!\d)", torch.__version__):  # its tensors are that torch's
+            raise ImportError(f"{path} was built for torch {m.torch_version}, this is {torch.__version__}; build it again")
         L = lib()
         m.init(_lib.QlError, *(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
             "ql_last_error", "ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention",
