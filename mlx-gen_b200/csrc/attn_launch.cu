@@ -20,7 +20,8 @@ static Plan plan_rows(int64_t B, int64_t items, int64_t span, bool window, doubl
     if (pieces <= 1) return {1, 128, false, false};
     // Few items of moderate length: up to 8 splits in a cluster, one launch and no workspace.
     // One sequence of 8 kv heads: 777 positions 6.0 us (joined by a second launch 9.0), 4000
-    // positions 11.1 us (12.5 in 16 joined splits), 16000 positions 31.5 us (24.3).
+    // positions 11.1 us (12.5 in 16 joined splits), 16000 positions 31.5 us (24.3); one kv head, 6000
+    // positions 14.2 us, 6001 by lengths 17.8.
     if (2 * items <= kSMs && span <= 6000) {
         int64_t ns = (kSMs + items - 1) / items;
         ns = ns < MAX_CLUSTER ? ns : MAX_CLUSTER;
@@ -41,7 +42,8 @@ static Plan plan_rows(int64_t B, int64_t items, int64_t span, bool window, doubl
     }
     // Many items: pieces of 2048 even out different lengths by their number (8 kv heads: 64
     // sequences of 311 - 8003 positions whole 218 us, in pieces of 4096 / 2048 / 1024 positions 189
-    // / 180 / 189; 10 of 20000 159 / 141 / 152; 16 of 4000 62 / 52 / 54).
+    // / 180 / 189; 10 of 20000 159 / 141 / 152; 16 of 4000 62 / 52 / 54).  Up to 2048 positions there is
+    // one piece, however few items: 10 sequences of 2000 33 us, where 9 are split in clusters and take 17.
     if (span <= 2048) return {1, 2048, false, false};
     // Chunks of heads of 96 and 256 run here too, with row blocks that fill the SMs by themselves and
     // gigabytes of partial results in such pieces: those are held to 128 MiB, by fewer, longer pieces

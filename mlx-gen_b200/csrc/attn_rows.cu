@@ -10,8 +10,9 @@
 // Softmax: running maximum and sum per row in fp32, weights 2^(s - max) <= 1 (in f16 times 2^15:
 // kWeightShift) rounded to the cache's type for the second product, the sum taken before that rounding.
 //
-// Measured: 64 sequences of 311 - 8003 positions (24 / 8 heads of 128) 179 us = 6.08 TB/s, 2 x 131k
-// positions 180 us = 5.95 TB/s (a copy: 6.56 TB/s), one sequence of 777 positions 6.2 us.
+// Measured (24 / 8 heads of 128, a graph's replay): 64 sequences of 311 - 8003 positions 178 us = 6.14
+// TB/s (189 in calls back to back), 2 x 131k positions 181 us = 5.92 TB/s (a copy: 6.56 TB/s), one
+// sequence of 777 positions 6.9 us.
 //
 // Positions that no row of the CTA sees are zero-filled in shared memory, whatever the cache
 // holds there (a page's unused tail may hold anything); scores of positions that a row does

@@ -31,8 +31,10 @@
 // Bound: the chain scores -> softmax -> product of a tile, about 3700 cycles a step of 128 positions
 // for D = 128 (softmax 2050, of it 1024 at least in the special-function unit; products 1650), on
 // which two tiles alternate; the tensor pipe and the special-function unit are each 52 % active.
-// Measured: 512 tokens over 16021 positions (24 / 8 heads of 128) 101 us = 1010 TFLOP/s, 4096 tokens
-// causal 114 us = 904 TFLOP/s; cuBLAS reaches 1644 TFLOP/s in bf16.
+// TMEM has no room for a third tile's S and O; the 64 columns of S_t that P_t leaves free are unused.
+// Measured (24 / 8 heads of 128): 512 tokens over 16021 positions 101 us = 1013 TFLOP/s in a graph's
+// replay and 115 us = 887 in calls back to back, where the power cap lowers the clock; 4096 tokens causal
+// 114 us = 902 and 123 us = 836; cuBLAS reaches 1644 TFLOP/s in bf16.
 #include "attn_common.cuh"
 
 namespace ql {

@@ -10,8 +10,8 @@
 // Split: one CTA per row; a thread owns NCH chunks of VEC consecutive elements, so the row
 // is held in registers whatever D is (up to 32 elements for each of 1024 threads).  The two
 // sums of squares are block reductions; rows of up to 32 vectors run a warp each, eight to a CTA.
-// Measured: 4608 x 3840 bf16 with post norm, gate and modulation 31.8 us = 4.46 TB/s (issue slots
-// 78 % busy; without the reductions 27 us), 4 x 3072 2.1 us.  Rings of rows filled by bulk copies
+// Measured: 4608 x 3840 bf16 with post norm, gate and modulation 31.4 us = 4.51 TB/s (issue slots
+// 78 % busy; without the reductions 27 us), 4 x 3072 1.8 us (a graph's replay; back to back 32.0, 4.7).  Rings of rows filled by bulk copies
 // with the factors kept in registers took 31.5 us at best and were left out.
 #include <string.h>
 

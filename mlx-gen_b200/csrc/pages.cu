@@ -6,7 +6,7 @@
 // destination and no destination occurs twice (checked on the host), so the copies are
 // independent and their order does not matter.  Split: CTAs of 256 threads, each moving
 // 16 KB of one page (four 16-byte loads in flight per thread).  Measured: 213 pages of 32 KB in 56
-// planes 120.5 us = 6.49 TB/s, 3 pages 2.7 us.
+// planes 120 us = 6.52 TB/s, 3 pages 2.8 us.
 #include <stdlib.h>
 #include <string.h>
 

@@ -8,9 +8,10 @@
 // Bound: HBM (q, k, v read once, q and the cache lines written once).  Split: one CTA per
 // token; a thread owns one chunk of pairs and walks over the heads with it, so it reads its
 // cosines and sines once; its first chunks are loaded before the position is known.  Measured: 4096
-// tokens, 24 / 8 heads of 128, with the append 19.5 us = 4.42 TB/s (128 threads; 256 threads 24 us;
-// CTAs that walk over tokens with positions fetched ahead 25 - 27 us).  VEC = 8 moves 16 or 32 bytes per access; VEC = 1 takes any
-// alignment and any even rot.
+// tokens, 24 / 8 heads of 128, with the append 19.1 us = 4.51 TB/s (128 threads; 256 threads 24 us;
+// CTAs that walk over tokens with positions fetched ahead 25 - 27 us).  Bound then: latency, 7 CTAs of
+// 128 threads an SM (68 registers in bf16).  VEC = 8 moves 16 or 32 bytes per access; VEC = 1 takes
+// any alignment and any even rot.
 #include "pdl.cuh"
 
 namespace ql {
