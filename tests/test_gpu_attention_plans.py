@@ -204,3 +204,12 @@ def test_single_tokens_with_masks(kv, D, causal, window):
 @pytest.mark.parametrize("q_len", [2, 150])
 def test_long_contexts_of_other_head_sizes(D, q_len):
     check_attention(gen(D + q_len), [q_len, q_len], [9001, 1000], 6, 2, D, 64)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_clusters_of_eight(D, dtype):
+    """One sequence of up to 6000 positions: eight splits, with heads of 256 each CTA alone on its SM."""
+    assert qlinear.paged_attention_workspace_size(1, 6, 2, D, 1, 1, 6000) == 0
+    for kv, window in (([6000], 0), ([5999], 1500), ([1100], 0)):
+        check_attention(gen(D + kv[0]), [1], kv, 6, 2, D, 16, dtype, True, window)
