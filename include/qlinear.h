@@ -265,6 +265,53 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
 size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv,
                                          int64_t window);
 
+/* The same, always causal, with the first `sinks` positions visible beside the window: token p sees
+ * the positions j <= p with j > p - window or j < sinks.  sinks at most 1024, and 0 without a
+ * window.  Pages between the sinks and the windows of a sequence's new tokens are not used (their
+ * entries may be anything), so a sequence without end keeps a fixed number of pages.  The
+ * workspace is ql_paged_attention_workspace_size's for that window. */
+int ql_sink_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
+                      int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages, int64_t page_stride,
+                      int page_size, const int32_t *page_table, int64_t table_stride, const int32_t *q_starts,
+                      const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv, float scale, int64_t window,
+                      int64_t sinks, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The index tensors of a step in which sequence b gets new_tokens[b] tokens more than its
+ * lengths[b]: kv_lens[b] = their sum, q_starts [B + 1] = exclusive sums of new_tokens, and for each
+ * new token its position and its slot (page * page_size + offset, from page_table
+ * [B, table_width] with rows table_stride entries apart), in the order of the sequences.  Rows behind
+ * the last token, up to max_tokens, get position 0 and slot -1 (not cached).  With free_pages
+ * [num_free] the pages that the new tokens need beyond those of the old ones are taken from it,
+ * from entry taken[0] on in the order of the sequences, and entered in page_table; taken_out[0] =
+ * taken[0] + their number.  Without (NULL) the tables hold every page already, taken and taken_out
+ * are not used.  All or nothing: counts below 0, more tokens than max_tokens, pages past table_width or
+ * past num_free give a step without tokens (kv_lens = lengths, q_starts 0, nothing taken) and set
+ * the device error word; so does a negative table entry, whose tokens get slot -1.  kv_lens may be
+ * lengths and taken_out taken: a captured call then advances the sequences at every replay.
+ * page_size: a power of two. */
+int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                 const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, const int32_t *free_pages,
+                 int64_t num_free, const int32_t *taken, int64_t *positions, int64_t *slots, int32_t *q_starts,
+                 int32_t *kv_lens, int32_t *taken_out, void *stream);
+
+/* One token per row of logits [B, V] (row_stride elements between rows, 0: all the same) from random numbers u [B] in [0, 1):
+ *     w_i = exp((x_i - max x) / temperature); in the order of x (descending, equal ones by index) the
+ *     first top_k stay (0: all), of those the shortest prefix with a sum of at least top_p times
+ *     theirs (one token at least; 1: all), of those the ones with w_i >= min_p;
+ *     tokens[b] = the first that stays, by index, with (sum up to it) > u (sum of all that stay).
+ * temperature 0: the largest logit, the lowest index of equal ones.  Each setting is one number for each row
+ * (a pointer) or for all (NULL and the ..._all argument, kept in 64 bits).  Weights are computed in 64 bits and
+ * summed as whole numbers (of 2^-46, for more than 2^17 tokens 2^(ceil(log2 V) - 63)), so that a row's token does not
+ * depend on the rest of the batch; a logit of -inf is never drawn, those of +inf share everything.  u is taken as at
+ * least 0, and 1 or more gives the last token that stays.  A row with a NaN (logits, settings or u), a
+ * negative temperature or nothing above -inf: token -1, log-probability NaN.  logprobs [B] or
+ * NULL: the logarithm of the probability with which the token was drawn (0 for temperature 0).
+ * dtype f32, bf16 or f16, a row at most 1310208 bytes. */
+int ql_sample(const void *logits, int dtype, int64_t row_stride, int64_t B, int64_t V, const float *u,
+              const float *temperature, double temperature_all, const int32_t *top_k, int64_t top_k_all,
+              const float *top_p, double top_p_all, const float *min_p, double min_p_all, int64_t *tokens,
+              float *logprobs, void *stream);
+
 /* Copies pages inside a pool: page dst[i] := page src[i] in each of `planes` planes (the keys or
  * values of one layer), plane_stride bytes apart, pages page_stride bytes apart, page_bytes each
  * (all multiples of 16).  src and dst are HOST arrays of n indices, read before the call

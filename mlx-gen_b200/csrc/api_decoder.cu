@@ -1,5 +1,5 @@
 // api_decoder.cu -- the extern "C" entry points of the decoder operators (residual norm,
-// rotary positions, paged attention, page copies).  Everything the host can know is checked
+// rotary positions, paged attention, page copies, step planning, sampling).  Everything the host can know is checked
 // here before a launch; sizes and indices that live on the device are bounds-checked by the
 // kernels, which report them in the device error word.
 #include <math.h>
@@ -15,6 +15,9 @@ int launch_copy_pages(void *, int64_t, int64_t, int64_t, int64_t, const int32_t 
                       cudaStream_t);
 size_t paged_attention_workspace(int64_t, int, int, int, int64_t, int64_t, int64_t, int64_t);
 int launch_paged_attention(attn::Params &, int, int, int64_t, void *, cudaStream_t);
+int launch_plan_step(const plank::Params &, cudaStream_t);
+int launch_sample(const samplek::Params &, int, int64_t, cudaStream_t);
+int64_t sample_row_limit();
 
 static int elem_bytes(int dt) { return dt == QL_F32 ? 4 : 2; }
 static bool elem_aligned(const void *p, int dt) { return (reinterpret_cast<uintptr_t>(p) % elem_bytes(dt)) == 0; }
@@ -145,12 +148,12 @@ size_t ql_paged_attention_workspace_size(int64_t T, int Hq, int Hkv, int D, int6
     return paged_attention_workspace(T, Hq, Hkv, D, B, max_q, max_kv, effective_window(window, max_kv));
 }
 
-int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
-                       int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages,
-                       int64_t page_stride, int page_size, const int32_t *page_table, int64_t table_stride,
-                       const int32_t *q_starts, const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv,
-                       float scale, int causal, int64_t window, void *out, void *workspace, size_t workspace_bytes,
-                       void *stream) {
+static int attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
+                     int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages,
+                     int64_t page_stride, int page_size, const int32_t *page_table, int64_t table_stride,
+                     const int32_t *q_starts, const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv,
+                     float scale, int causal, int64_t window, int64_t sinks, void *out, void *workspace,
+                     size_t workspace_bytes, void *stream) {
     g_err[0] = 0;
     if (int rc = check_attention(T, Hq, Hkv, D, B, max_q, max_kv)) return rc;
     if (dtype != QL_BF16 && dtype != QL_F16) return fail(QL_EUNSUPPORTED, "ql_paged_attention: bf16 or f16");
@@ -164,6 +167,8 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
                     (long long)table_stride, (long long)max_kv);
     if (!(scale > 0.f) || !isfinite(scale)) return fail(QL_EINVAL_ARG, "scale must be positive and finite");
     if (window < 0 || (window && !causal)) return fail(QL_EINVAL_ARG, "window must be >= 0, and needs causal");
+    if (sinks < 0 || (sinks && !window)) return fail(QL_EINVAL_ARG, "sinks must be >= 0, and need a window");
+    if (sinks > attn::MAX_SINKS) return fail(QL_EUNSUPPORTED, "at most %d sinks (got %lld)", attn::MAX_SINKS, (long long)sinks);
     if (T == 0 || B == 0) return QL_OK;
     if (!q || !k_cache || !v_cache || !page_table || !q_starts || !kv_lens || !out)
         return fail(QL_EINVAL_ARG, "ql_paged_attention: NULL pointer");
@@ -184,8 +189,83 @@ int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t
     p.max_q = (int)max_q, p.max_kv = (int)max_kv;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.causal = causal != 0, p.window = (int)window;
+    p.sinks = window ? (int)sinks : 0;  // (a window that holds everything is none)
     p.out = out;
     return launch_paged_attention(p, dtype, D, B, workspace, (cudaStream_t)stream);
+}
+
+int ql_paged_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
+                       int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages,
+                       int64_t page_stride, int page_size, const int32_t *page_table, int64_t table_stride,
+                       const int32_t *q_starts, const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv,
+                       float scale, int causal, int64_t window, void *out, void *workspace, size_t workspace_bytes,
+                       void *stream) {
+    return attention(q, dtype, q_token_stride, q_head_stride, T, Hq, Hkv, D, k_cache, v_cache, num_pages, page_stride, page_size,
+                     page_table, table_stride, q_starts, kv_lens, B, max_q, max_kv, scale, causal, window, 0, out, workspace,
+                     workspace_bytes, stream);
+}
+
+int ql_sink_attention(const void *q, int dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t T, int Hq,
+                      int Hkv, int D, const void *k_cache, const void *v_cache, int64_t num_pages, int64_t page_stride,
+                      int page_size, const int32_t *page_table, int64_t table_stride, const int32_t *q_starts,
+                      const int32_t *kv_lens, int64_t B, int64_t max_q, int64_t max_kv, float scale, int64_t window,
+                      int64_t sinks, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+    return attention(q, dtype, q_token_stride, q_head_stride, T, Hq, Hkv, D, k_cache, v_cache, num_pages, page_stride, page_size,
+                     page_table, table_stride, q_starts, kv_lens, B, max_q, max_kv, scale, 1, window, sinks, out, workspace,
+                     workspace_bytes, stream);
+}
+
+int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                 const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, const int32_t *free_pages,
+                 int64_t num_free, const int32_t *taken, int64_t *positions, int64_t *slots, int32_t *q_starts,
+                 int32_t *kv_lens, int32_t *taken_out, void *stream) {
+    g_err[0] = 0;
+    if (B < 0 || B > INT32_MAX - 1 || max_tokens < 0 || max_tokens > INT32_MAX || num_free < 0 || num_free > INT32_MAX)
+        return fail(QL_EINVAL_SHAPE, "ql_plan_step: bad sizes (B=%lld, max_tokens=%lld, num_free=%lld)", (long long)B,
+                    (long long)max_tokens, (long long)num_free);
+    if (!pow2(page_size)) return fail(QL_EUNSUPPORTED, "page size must be a power of two (got %d)", page_size);
+    if (table_width < 0 || (B > 1 && table_stride < table_width))
+        return fail(QL_EINVAL_SHAPE, "ql_plan_step: the page table's rows overlap (%lld entries, stride %lld)", (long long)table_width,
+                    (long long)table_stride);
+    if (B && (!lengths || !new_tokens || !kv_lens || (table_width && !page_table))) return fail(QL_EINVAL_ARG, "ql_plan_step: NULL pointer");
+    if (!q_starts || (max_tokens && (!positions || !slots))) return fail(QL_EINVAL_ARG, "ql_plan_step: NULL pointer");
+    if (free_pages && (!taken || !taken_out)) return fail(QL_EINVAL_ARG, "ql_plan_step: a free list needs taken and taken_out");
+    const void *words[] = {page_table, lengths, new_tokens, free_pages, taken, q_starts, kv_lens, taken_out};
+    for (const void *w : words)
+        if (reinterpret_cast<uintptr_t>(w) % 4) return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
+    if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(slots) % 8)
+        return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
+    const ql::plank::Params p{page_table, table_stride, table_width, lengths, new_tokens, B, max_tokens, log2i(page_size),
+                              free_pages, num_free, taken, positions, slots, q_starts, kv_lens, taken_out};
+    return launch_plan_step(p, (cudaStream_t)stream);
+}
+
+int ql_sample(const void *logits, int dtype, int64_t row_stride, int64_t B, int64_t V, const float *u,
+              const float *temperature, double temperature_all, const int32_t *top_k, int64_t top_k_all,
+              const float *top_p, double top_p_all, const float *min_p, double min_p_all, int64_t *tokens,
+              float *logprobs, void *stream) {
+    g_err[0] = 0;
+    if (!valid_dtype(dtype)) return fail(QL_EUNSUPPORTED, "unknown dtype");
+    if (B < 0 || V < 1 || row_stride < 0)
+        return fail(QL_EINVAL_SHAPE, "ql_sample: bad sizes (B=%lld, V=%lld, row stride %lld)", (long long)B, (long long)V,
+                    (long long)row_stride);
+    if (V * elem_bytes(dtype) > sample_row_limit())
+        return fail(QL_EUNSUPPORTED, "ql_sample: a row of %lld logits is too long (at most %lld bytes)", (long long)V,
+                    (long long)sample_row_limit());
+    if ((!temperature && !(temperature_all >= 0.0)) || (!top_p && !(top_p_all >= 0.0)) || (!min_p && !(min_p_all >= 0.0 && min_p_all <= 1.0)) ||
+        (!top_k && top_k_all < 0))
+        return fail(QL_EINVAL_ARG, "ql_sample: temperature, top_k and top_p must not be negative, min_p in [0, 1]");
+    if (B == 0) return QL_OK;
+    if (!logits || !u || !tokens) return fail(QL_EINVAL_ARG, "ql_sample: NULL pointer");
+    if (!elem_aligned(logits, dtype) || reinterpret_cast<uintptr_t>(tokens) % 8) return fail(QL_EINVAL_ARG, "ql_sample: pointer not aligned to its dtype");
+    const void *words[] = {u, temperature, top_k, top_p, min_p, logprobs};
+    for (const void *w : words)
+        if (reinterpret_cast<uintptr_t>(w) % 4) return fail(QL_EINVAL_ARG, "ql_sample: pointer not aligned to its dtype");
+    // weights are whole numbers up to 2^scale, sums of V of them fit 63 bits
+    const int scale = 63 - log2i(V) < 46 ? 63 - log2i(V) : 46;
+    const ql::samplek::Params p{logits, row_stride, (int)V, 0, scale, u, temperature, top_p, min_p, top_k,
+                                temperature_all, top_p_all, min_p_all, top_k_all, tokens, logprobs};
+    return launch_sample(p, dtype, B, (cudaStream_t)stream);
 }
 
 int ql_copy_pages(void *pool, int64_t planes, int64_t plane_stride, int64_t num_pages, int64_t page_stride,

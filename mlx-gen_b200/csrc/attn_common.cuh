@@ -5,7 +5,8 @@
 //
 // Token i of a sequence with q_len new tokens and kv_len cached positions (the new ones
 // included) stands at position p = kv_len - q_len + i; it sees j < kv_len, with `causal` only
-// j <= p, with a window only j > p - window.  A token that sees nothing gets zeros.
+// j <= p, with a window only j > p - window and, with sinks, j < sinks.  A token that sees nothing
+// gets zeros.
 //
 // The q heads of one kv head are packed: row r of a (sequence, kv head) is token r / G, head
 // r % G of the group (G = Hq / Hkv), so a group's heads read each key and value together.
@@ -19,6 +20,7 @@ namespace attn {
 constexpr int kSMs = 148;         // B200; used for planning only
 constexpr int ROWS_TILE = 16;     // rows of the small-row kernel (one m16 tile)
 constexpr int MAX_CLUSTER = 8;    // splits of the small-row kernel that can join inside a cluster
+constexpr int MAX_SINKS = 1024;   // first positions that stay visible (more would be work that the splits do not share)
 constexpr float NEG_INF = -INFINITY;
 
 struct Params {
@@ -41,6 +43,7 @@ struct Params {
     bool adapt;                   // small-row kernel: the chunk follows from the sequences' lengths (adapted_chunk)
     bool cluster;                 // small-row kernel: the splits join inside a cluster, part_* unused
     int rows_kernel_most;         // sequences with up to so many rows go to the small-row kernel
+    int sinks;                    // first positions that stay visible beside the window (0: none)
 };
 
 struct Seq {
@@ -60,25 +63,30 @@ __device__ __forceinline__ Seq load_seq(const Params &p, int b) {
     return s;
 }
 
-// [lo, hi): the positions that token `tok` sees
+// [lo, hi): the positions that token `tok` sees, without the sinks below lo
 __device__ __forceinline__ void visible(const Params &p, const Seq &s, int tok, int &lo, int &hi) {
     hi = p.causal ? min(s.kv_len, max(0, s.ctx + tok + 1)) : s.kv_len;
     lo = p.window ? max(0, s.ctx + tok + 1 - p.window) : 0;
 }
 
-// [lo, hi): the positions that some of the packed rows [r0, r1) sees
+// [lo, hi): the positions that some of the packed rows [r0, r1) sees (without the sinks below lo)
 __device__ __forceinline__ void visible_rows(const Params &p, const Seq &s, int r0, int r1, int &lo, int &hi) {
     int unused;
     visible(p, s, r0 / p.G, lo, unused);
     visible(p, s, (r1 - 1) / p.G, unused, hi);
 }
 
-// The splits divide what the CTA's rows see, [lo, hi), from lo's 128-boundary on.
+// The splits divide what the CTA's rows see, [lo, hi), from lo's 128-boundary on; the sinks below that
+// go to the first, in steps before the window's (`lead` of them).
 __device__ __forceinline__ void take_split(const Params &p, int split, int chunk, int &lo, int &hi) {
     if (p.nsplit == 1) return;
     const int64_t from = (lo & ~127) + (int64_t)split * chunk;
     lo = (int)max((int64_t)lo, min(from, (int64_t)hi));
     hi = (int)min((int64_t)hi, from + chunk);
+}
+
+__device__ __forceinline__ int lead_steps(const Params &p, int split, int lo, int hi, int step) {
+    return split == 0 && lo < hi ? min((p.sinks + step - 1) / step, lo / step) : 0;
 }
 
 // The page that holds position pos; an index outside the cache is reported and reads page 0.

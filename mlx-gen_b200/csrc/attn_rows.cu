@@ -16,7 +16,8 @@
 //
 // Positions that no row of the CTA sees are zero-filled in shared memory, whatever the cache
 // holds there (a page's unused tail may hold anything); scores of positions that a row does
-// not see are replaced by -inf.
+// not see are replaced by -inf.  With SINKS the first `lead` blocks are the first tokens', which every
+// row sees, and the window's follow.
 #include "attn_common.cuh"
 
 namespace ql {
@@ -86,9 +87,9 @@ __device__ __forceinline__ void mma16816<__half>(float c[4], const uint32_t a[4]
 
 // One stretch of positions [lo, hi) for one row block of a (sequence, kv head).  Its result is
 // partial result number `slot` of `slots`, or the output itself where slots is 1 (and not CLUSTER).
-template <typename T, int D, bool CLUSTER, bool ALONE>
-__device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int b, int kvh, int rb, int lo, int hi, int slot,
-                                             int slots, uint8_t *smem) {
+template <typename T, int D, bool CLUSTER, bool ALONE, bool SINKS>
+__device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int b, int kvh, int rb, int lo, int hi, int lead,
+                                             int slot, int slots, uint8_t *smem) {
     using C = RowsCfg<D, ALONE>;
     constexpr int RW = C::RW;
     constexpr float SHIFT = kWeightShift<T, 0>;
@@ -124,27 +125,32 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
-    const int blk0 = lo / RKV, nblk = hi > lo ? (hi + RKV - 1) / RKV - blk0 : 0;
-    const int mine = nblk > warp ? (nblk - warp + RW - 1) / RW : 0;  // blocks blk0 + warp + i * RW
+    const int blk0 = lo / RKV, nblk = (hi > lo ? (hi + RKV - 1) / RKV - blk0 : 0) + (SINKS ? lead : 0);
+    const int mine = nblk > warp ? (nblk - warp + RW - 1) / RW : 0;  // blocks warp + i * RW
+    auto block_at = [&](int i) {  // first position of this warp's block i
+        const int k = warp + i * RW;
+        return (SINKS ? (k < lead ? k : blk0 + k - lead) : blk0 + k) * RKV;
+    };
     const uint32_t ring = smem_u32(smem) + warp * C::WARP_BYTES;
     const int64_t head_at = (int64_t)kvh * ((int64_t)D << p.page_shift);
     const int in_page = (1 << p.page_shift) - 1;
 
     auto issue = [&](int i, int page) {  // block i of this warp into its stage
-        const int pos = (blk0 + warp + i * RW) * RKV;
+        const int pos = block_at(i);
         const uint32_t ks = ring + (i % C::STAGES) * 2 * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
-        const int64_t at = page * p.page_stride + head_at + (int64_t)(pos & in_page) * D;
-        const uint16_t *kp = reinterpret_cast<const uint16_t *>(p.k_cache) + at;
-        const uint16_t *vp = reinterpret_cast<const uint16_t *>(p.v_cache) + at;
+        const int64_t from = page * p.page_stride + head_at + (int64_t)(pos & in_page) * D;
+        const uint16_t *kp = reinterpret_cast<const uint16_t *>(p.k_cache) + from;
+        const uint16_t *vp = reinterpret_cast<const uint16_t *>(p.v_cache) + from;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
             const int idx = j * 32 + lane, row = idx / (D / 8), col = idx % (D / 8);
-            const bool in = pos + row >= lo && pos + row < hi;
+            const int at = pos + row;
+            const bool in = SINKS ? (at >= lo && at < hi) || (at < p.sinks && (at < hi || warp + i * RW < lead)) : at >= lo && at < hi;
             cp_async16(ks + row * C::ROW_BYTES + col * 16, kp + row * D + col * 8, in);
             cp_async16(vs + row * C::ROW_BYTES + col * 16, vp + row * D + col * 8, in);
         }
     };
-    auto page_at = [&](int i) { return i < mine ? page_of(p, b, (blk0 + warp + i * RW) * RKV) : 0; };
+    auto page_at = [&](int i) { return i < mine ? page_of(p, b, block_at(i)) : 0; };
 
     int pages[C::STAGES];
 #pragma unroll
@@ -173,14 +179,15 @@ __device__ __forceinline__ void rows_stretch(const Params &p, const Seq &s, int 
             mma16816<T>(sc[0], qf[k], kb[0], kb[1]);
             mma16816<T>(sc[1], qf[k], kb[2], kb[3]);
         }
-        const int pos = (blk0 + warp + i * RW) * RKV + t4 * 2;
+        const int pos = block_at(i) + t4 * 2;
+        const int end = SINKS && warp + i * RW < lead ? INT32_MAX : hi;
         float mx[2] = {NEG_INF, NEG_INF};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int at = pos + n * 8 + (e & 1), r = e >> 1;
-                const bool in = at >= max(rlo[r], lo) && at < min(rhi[r], hi);
+                const bool in = (at >= max(rlo[r], lo) || (SINKS && at < p.sinks)) && at < min(rhi[r], end);
                 sc[n][e] = in ? sc[n][e] * p.scale_log2 : NEG_INF;
                 mx[r] = fmaxf(mx[r], sc[n][e]);
             }
@@ -363,7 +370,7 @@ __device__ __forceinline__ int adapted_chunk(const Params &p, int B) {
 // grid: kv head * rowblocks + row block, sequence and split; the split runs fastest (x) with
 // CLUSTER and slowest (z) without, so that pieces which hold something come before empty ones and
 // the first of them go one to an SM.
-template <typename T, int D, bool CLUSTER, bool ALONE>
+template <typename T, int D, bool CLUSTER, bool ALONE, bool SINKS>
 __global__ void __launch_bounds__(RowsCfg<D, ALONE>::RW * 32) rows_kernel(const Params p, int rowblocks) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_trigger();
@@ -379,20 +386,21 @@ __global__ void __launch_bounds__(RowsCfg<D, ALONE>::RW * 32) rows_kernel(const 
     if (r0 >= rows || rows > p.rows_kernel_most) return;
     int lo, hi;
     visible_rows(p, s, r0, min(rows, r0 + ROWS_TILE), lo, hi);
+    const int lead = SINKS ? lead_steps(p, split, lo, hi, RKV) : 0;
     take_split(p, split, ALONE ? adapted_chunk(p, gridDim.y) : p.chunk, lo, hi);
-    if (!CLUSTER && p.nsplit > 1 && lo >= hi) {  // nothing in this split
+    if (!CLUSTER && p.nsplit > 1 && lo >= hi && lead == 0) {  // nothing in this split
         const int r = threadIdx.x;
         if (r < min(ROWS_TILE, rows - r0))
             p.part_lse[((s.q0 + (int64_t)((r0 + r) / p.G)) * p.Hq + kvh * p.G + (r0 + r) % p.G) * p.nsplit + split] = NEG_INF;
         return;
     }
-    rows_stretch<T, D, CLUSTER, ALONE>(p, s, b, kvh, rb, lo, hi, split, p.nsplit, smem);
+    rows_stretch<T, D, CLUSTER, ALONE, SINKS>(p, s, b, kvh, rb, lo, hi, lead, split, p.nsplit, smem);
 }
 
-template <typename T, int D, bool CLUSTER, bool ALONE>
-static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
+template <typename T, int D, bool CLUSTER, bool ALONE, bool SINKS>
+static int launch_rows_s(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
     using C = RowsCfg<D, ALONE>;
-    auto kernel = rows_kernel<T, D, CLUSTER, ALONE>;
+    auto kernel = rows_kernel<T, D, CLUSTER, ALONE, SINKS>;
     static PerDeviceFlag configured;
     const int dev = current_device();
     if (!configured.test(dev)) {
@@ -402,6 +410,12 @@ static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t
     const dim3 grid = CLUSTER ? dim3(p.nsplit, p.Hkv * rowblocks, (unsigned)B) : dim3(p.Hkv * rowblocks, (unsigned)B, p.nsplit);
     QL_CUDA_TRY(launch_pdl(kernel, grid, dim3(C::RW * 32), C::SMEM, st, CLUSTER ? p.nsplit : 1, p, rowblocks));
     return QL_OK;
+}
+
+template <typename T, int D, bool CLUSTER, bool ALONE>
+static int launch_rows_c(const Params &p, int64_t B, int rowblocks, cudaStream_t st) {
+    return p.sinks ? launch_rows_s<T, D, CLUSTER, ALONE, true>(p, B, rowblocks, st)
+                   : launch_rows_s<T, D, CLUSTER, ALONE, false>(p, B, rowblocks, st);
 }
 
 template <typename T, int D>

@@ -56,7 +56,7 @@ struct Sm100Cfg {
     static constexpr int COL_O = 256, COL_P = P_APART ? 256 + 2 * D : 0, P_STEP = P_APART ? TKV / 2 : TKV;
     static constexpr int SMEM_Q = 0, SMEM_KV = 2 * TILE_BYTES;
     static constexpr int SMEM_BAR = SMEM_KV + STAGES * TILE_BYTES;
-    static constexpr int NBAR = 2 * STAGES + 2 * 8 + 2;
+    static constexpr int NBAR = 2 * STAGES + 2 * 8 + 3;
     static constexpr int SMEM = SMEM_BAR + NBAR * 8 + 16 + 1024;
 };
 
@@ -108,7 +108,7 @@ __host__ __device__ constexpr uint32_t attn_idesc(int N, bool b_mn_major) {
            (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(TQ >> 4) << 24);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SINKS>
 __global__ void __launch_bounds__(SM100_THREADS, 1)
     sm100_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
     using C = Sm100Cfg<D>;
@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint64_t *drain = ofull + 2;       // [2] an aborted tile's MMAs are done
     uint64_t *turn = drain + 2;        // [2] the other tile's exponentials of the step are done
     uint64_t *sread = turn + 2;        // [2] S_t of the step is in registers (P_APART)
-    uint64_t *vfix = sread + 2;        // [2] V of the first / last step cleared outside [vlo, vhi)
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 2);
+    uint64_t *vfix = sread + 2;        // [3] V of the window's first / the last / the sinks' last step cleared where no row sees it
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 3);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     pdl_wait();
@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     int vlo, vhi, unused;
     visible(p, s, row0 / p.G, vlo, unused);
     visible(p, s, (row0 + nrows - 1) / p.G, unused, vhi);
+    const int lead = SINKS ? lead_steps(p, split, vlo, vhi, TKV) : 0;
     take_split(p, split, p.chunk, vlo, vhi);
     if (vhi <= vlo) {  // nothing to see: no partial result, or zeros
         for (int idx = threadIdx.x; idx < nrows; idx += SM100_THREADS) {
@@ -161,8 +162,11 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
         }
         return;
     }
-    const int t0 = vlo / TKV, n = (vhi + TKV - 1) / TKV - t0;
-    const bool fix_first = vlo > t0 * TKV, fix_last = vhi < (t0 + n) * TKV;
+    // steps: `lead` of the sinks below the window, then the window's from tile t0 on
+    const int t0 = vlo / TKV, n = lead + (vhi + TKV - 1) / TKV - t0;
+    auto step_at = [&](int j) { return (SINKS ? (j < lead ? j : t0 + j - lead) : t0 + j) * TKV; };  // first position
+    const bool fix_first = vlo > (SINKS ? max(t0 * TKV, p.sinks) : t0 * TKV), fix_last = vhi < (t0 + n - lead) * TKV;
+    const bool fix_lead = SINKS && p.sinks < lead * TKV;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -180,6 +184,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             mbar_init(&sread[t], 4);
             mbar_init(&vfix[t], 1);
         }
+        if constexpr (SINKS) mbar_init(&vfix[2], 1);
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_tmap(&tm_k);
@@ -256,12 +261,13 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sread[t]);
                 }
-                const int kv0 = (t0 + j) * TKV;
+                const int kv0 = step_at(j);
                 // a step that some row of the tile does not see whole (the same for all its threads)
                 if (kv0 < max_lo || kv0 + TKV > min_hi) {
 #pragma unroll
                     for (int w = 0; w < TKV / 32; ++w) {  // one bit per position: two instructions a score
-                        const uint32_t see = bits_below(rhi - kv0 - w * 32) & ~bits_below(rlo - kv0 - w * 32);
+                        uint32_t see = bits_below(rhi - kv0 - w * 32) & ~bits_below(rlo - kv0 - w * 32);
+                        if constexpr (SINKS) see |= bits_below(min(rhi, p.sinks) - kv0 - w * 32);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) sc[w * 32 + i] = (see & (1u << i)) ? sc[w * 32 + i] : NEG_INF;
                     }
@@ -391,12 +397,12 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             // clears what no row sees in V of step j, once it has landed; only this warp refills
             // the stage, so its barrier still stands at that load
             auto clear_v = [&](int j, uint64_t *done) {
-                const int it = 2 * j + 1, st = it % STAGES, kv0 = (t0 + j) * TKV;
+                const int it = 2 * j + 1, st = it % STAGES, kv0 = step_at(j);
                 if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, DEV_ERR_TIMEOUT_FULL))) return;
                 uint8_t *vs = smem + C::SMEM_KV + st * C::TILE_BYTES;
                 for (int idx = lane; idx < TKV * 8; idx += 32) {
                     const int row = idx >> 3;
-                    if (kv0 + row >= vlo && kv0 + row < vhi) continue;
+                    if ((kv0 + row >= vlo || (SINKS && kv0 + row < p.sinks)) && kv0 + row < vhi) continue;
 #pragma unroll
                     for (int h = 0; h < C::HALVES; ++h)
                         *reinterpret_cast<uint4 *>(vs + h * C::HALF_BYTES + row * 128 + (idx & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -407,17 +413,20 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             };
             // this lane's page of step j, where there is something to see; indices are fetched four
             // steps ahead
+            auto wanted = [&](int pos) { return lane < nb && pos < vhi && (pos + box > vlo || (SINKS && pos < p.sinks)); };
             auto page_index = [&](int j) {
-                const int pos = (t0 + j) * TKV + lane * box;
-                return j < n && lane < nb && pos < vhi && pos + box > vlo ? p.table[b * p.table_stride + (pos >> p.page_shift)] : 0;
+                const int pos = step_at(j) + lane * box;
+                return j < n && wanted(pos) ? p.table[b * p.table_stride + (pos >> p.page_shift)] : 0;
             };
             int it = 0, page = 0, ahead[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) ahead[j] = page_index(j);
             for (; it < loads; ++it) {
-                if (it == min(STAGES, 2 * n - 1) && fix_first && n > 1) clear_v(0, &vfix[0]);
-                const int st = it % STAGES, pos = (t0 + (it >> 1)) * TKV + lane * box;
-                const bool in = lane < nb && pos < vhi && pos + box > vlo;
+                // V of step j is cleared before the load that waits for its products
+                if (SINKS && fix_lead && it == min(2 * (lead - 1) + STAGES, 2 * n - 1)) clear_v(lead - 1, &vfix[2]);
+                if (it == min(2 * lead + STAGES, 2 * n - 1) && fix_first && lead < n - 1) clear_v(lead, &vfix[0]);
+                const int st = it % STAGES, pos = step_at(it >> 1) + lane * box;
+                const bool in = wanted(pos);
                 if (!(it & 1)) {
                     page = ahead[0], ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
                     ahead[3] = page_index((it >> 1) + 4);
@@ -441,8 +450,8 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
             }
             if (it == 2 * n) {
-                if (n == 1 && (fix_first || fix_last)) clear_v(0, &vfix[0]);
-                if (fix_last && n > 1) clear_v(n - 1, &vfix[1]);
+                if (lead == n - 1 && (fix_first || fix_last)) clear_v(lead, &vfix[0]);
+                if (fix_last && lead < n - 1) clear_v(n - 1, &vfix[1]);
             }
             // after an abort, whichever wait ran out, the copies land before their memory is given up
             roles_done();
@@ -488,8 +497,9 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
                 const int it = 2 * j + 1, st = it % STAGES;
                 ok = mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, DEV_ERR_TIMEOUT_FULL);
-                if (ok && j == 0 && (fix_first || (n == 1 && fix_last))) ok = mbar_wait(&vfix[0], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
-                if (ok && j > 0 && j == n - 1 && fix_last) ok = mbar_wait(&vfix[1], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (SINKS && ok && fix_lead && j == lead - 1) ok = mbar_wait(&vfix[2], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (ok && j == lead && (fix_first || (lead == n - 1 && fix_last))) ok = mbar_wait(&vfix[0], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (ok && j > lead && j == n - 1 && fix_last) ok = mbar_wait(&vfix[1], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
                 const uint32_t vs = ring + st * C::TILE_BYTES;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -540,22 +550,27 @@ static int cache_map(CUtensorMap *map, const void *base, const Params &p, int D)
     return r == CUDA_SUCCESS ? QL_OK : fail(QL_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
-template <typename T, int D>
-static int launch_sm100_t(const Params &p, int64_t B, cudaStream_t st) {
+template <typename T, int D, bool SINKS>
+static int launch_sm100_s(const Params &p, int64_t B, cudaStream_t st) {
     using C = Sm100Cfg<D>;
     static PerDeviceFlag configured;
     const int dev = current_device();
     if (!configured.test(dev)) {
-        QL_CUDA_TRY(cudaFuncSetAttribute(sm100_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        QL_CUDA_TRY(cudaFuncSetAttribute(sm100_kernel<T, D, SINKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         configured.set(dev);
     }
     CUtensorMap mk, mv;
     if (int rc = cache_map<T>(&mk, p.k_cache, p, D)) return rc;
     if (int rc = cache_map<T>(&mv, p.v_cache, p, D)) return rc;
     const int tiles = (int)(((int64_t)p.max_q * p.G + SM100_ROWS - 1) / SM100_ROWS);
-    QL_CUDA_TRY(launch_pdl(sm100_kernel<T, D>, dim3(p.Hkv * p.nsplit, tiles, (unsigned)B), dim3(SM100_THREADS), C::SMEM, st, 1,
+    QL_CUDA_TRY(launch_pdl(sm100_kernel<T, D, SINKS>, dim3(p.Hkv * p.nsplit, tiles, (unsigned)B), dim3(SM100_THREADS), C::SMEM, st, 1,
                            mk, mv, p));
     return QL_OK;
+}
+
+template <typename T, int D>
+static int launch_sm100_t(const Params &p, int64_t B, cudaStream_t st) {
+    return p.sinks ? launch_sm100_s<T, D, true>(p, B, st) : launch_sm100_s<T, D, false>(p, B, st);
 }
 
 }  // namespace attn

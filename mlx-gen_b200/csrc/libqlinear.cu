@@ -15,6 +15,8 @@
 #include "norm_residual.cu"
 #include "rope.cu"
 #include "pages.cu"
+#include "plan.cu"
+#include "sample.cu"
 #include "attn_rows.cu"
 #include "attn_sm100.cu"
 #include "attn_launch.cu"

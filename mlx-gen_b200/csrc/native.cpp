@@ -18,6 +18,8 @@
 
 #include <cmath>
 #include <sstream>
+#include <string>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/qlinear.h"
@@ -31,6 +33,9 @@ decltype(&ql_rope_append) p_rope_append;
 decltype(&ql_paged_attention) p_paged_attention;
 decltype(&ql_paged_attention_workspace_size) p_paged_attention_workspace_size;
 decltype(&ql_copy_pages) p_copy_pages;
+decltype(&ql_sink_attention) p_sink_attention;
+decltype(&ql_plan_step) p_plan_step;
+decltype(&ql_sample) p_sample;
 PyObject *g_error;  // QlError(status, message)
 
 struct PythonError {};  // a Python exception is set
@@ -232,12 +237,12 @@ const int32_t *index_tensor(const at::Tensor &t, const char *name, c10::Device d
     return t.const_data_ptr<int32_t>();
 }
 
-// (q, k_cache, v_cache, page_table, q_starts, kv_lens, max_q, max_kv, scale, causal, window, out, workspace) -> out
+// (q, k_cache, v_cache, page_table, q_starts, kv_lens, max_q, max_kv, scale, causal, window, sinks, out, workspace) -> out
 PyObject *paged_attention(PyObject *const *a) {
     at::Tensor q = tensor(a[0], "q");
     const at::Tensor &kc = tensor(a[1], "k_cache"), &vc = tensor(a[2], "v_cache"), &table = tensor(a[3], "page_table");
     const at::Tensor &starts = tensor(a[4], "q_starts"), &lens = tensor(a[5], "kv_lens");
-    const int64_t max_q = integer(a[6]), max_kv = integer(a[7]), window = integer(a[10]);
+    const int64_t max_q = integer(a[6]), max_kv = integer(a[7]), window = integer(a[10]), sinks = integer(a[11]);
     const c10::Device dev = on_cuda(q);
     VALUE(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", q.sizes());
     const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2);
@@ -256,9 +261,9 @@ PyObject *paged_attention(PyObject *const *a) {
     if (q.stride(2) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16)
         q = q.clone(at::MemoryFormat::Contiguous);
     at::Tensor out;
-    if (a[11] == Py_None) out = fresh(q.sizes(), q.scalar_type(), dev);
+    if (a[12] == Py_None) out = fresh(q.sizes(), q.scalar_type(), dev);
     else {
-        out = tensor(a[11], "out");
+        out = tensor(a[12], "out");
         VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == dev && out.is_contiguous(),
               "out must be contiguous, of q's shape, dtype and device");
     }
@@ -266,19 +271,137 @@ PyObject *paged_attention(PyObject *const *a) {
     const size_t need = p_paged_attention_workspace_size(T, hq, hkv, d, B, max_q, max_kv, window);
     at::Tensor ws;
     if (need) {
-        if (a[12] != Py_None) {
-            ws = tensor(a[12], "workspace");
+        if (a[13] != Py_None) {
+            ws = tensor(a[13], "workspace");
             VALUE(ws.device() == dev && ws.is_contiguous(), "workspace must be contiguous on ", dev);
         }
         if (!ws.defined() || ws.nbytes() < need) ws = fresh({(int64_t)need}, at::kByte, dev);
     }
     const float scale = a[8] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)real(a[8]);
-    check(p_paged_attention(q.const_data_ptr(), dtype_code(q), q.stride(0), q.stride(1), T, hq, hkv, d, kc.const_data_ptr(),
-                            vc.const_data_ptr(), c.pages, c.stride, (int)c.page_size, tp,
-                            B > 1 ? table.stride(0) : table.size(1), sp, lp, B, max_q, max_kv, scale, truth(a[9]),
-                            window, out.mutable_data_ptr(), need ? ws.mutable_data_ptr() : nullptr, need,
-                            stream_of(dev)));
+    const int64_t ts = B > 1 ? table.stride(0) : table.size(1);
+    const bool causal = truth(a[9]);
+    void *wp = need ? ws.mutable_data_ptr() : nullptr;
+    if (sinks) {
+        VALUE(causal, "sinks need causal");
+        check(p_sink_attention(q.const_data_ptr(), dtype_code(q), q.stride(0), q.stride(1), T, hq, hkv, d, kc.const_data_ptr(),
+                               vc.const_data_ptr(), c.pages, c.stride, (int)c.page_size, tp, ts, sp, lp, B, max_q, max_kv, scale,
+                               window, sinks, out.mutable_data_ptr(), wp, need, stream_of(dev)));
+    } else {
+        check(p_paged_attention(q.const_data_ptr(), dtype_code(q), q.stride(0), q.stride(1), T, hq, hkv, d, kc.const_data_ptr(),
+                                vc.const_data_ptr(), c.pages, c.stride, (int)c.page_size, tp, ts, sp, lp, B, max_q, max_kv, scale,
+                                causal, window, out.mutable_data_ptr(), wp, need, stream_of(dev)));
+    }
     return THPVariable_Wrap(std::move(out));
+}
+
+// A contiguous int32 vector of n entries (any number for n < 0) on dev.
+const int32_t *counts(const at::Tensor &t, const char *name, int64_t n, c10::Device dev) {
+    VALUE(t.dim() == 1 && (n < 0 || t.size(0) == n) && t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == dev, name,
+          " must be a contiguous int32 vector", n < 0 ? "" : " of " + std::to_string(n), " on ", dev, ", got ", t.sizes(), " ",
+          t.scalar_type(), " on ", t.device());
+    return t.const_data_ptr<int32_t>();
+}
+// An output of plan_step: entry i of `out`, or a new tensor.
+at::Tensor result(PyObject *out, int i, const char *name, int64_t n, at::ScalarType type, c10::Device dev) {
+    if (out == Py_None) return fresh({n}, type, dev);
+    const at::Tensor &t = tensor(PyTuple_GET_ITEM(out, i), name);
+    VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous() && t.device() == dev, "out's ", name,
+          " must be a contiguous ", type, " vector of ", n, " on ", dev, ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
+    return t;
+}
+
+// (page_table, lengths, new_tokens, page_size, max_tokens, free_pages, taken, out) -> (positions, slots, q_starts, kv_lens, taken)
+PyObject *plan_step(PyObject *const *a) {
+    const at::Tensor &table = tensor(a[0], "page_table"), &lengths = tensor(a[1], "lengths"), &fresh_tokens = tensor(a[2], "new_tokens");
+    const c10::Device dev = on_cuda(table);
+    VALUE(lengths.dim() == 1 && table.dim() == 2 && table.size(0) == lengths.size(0), "expected lengths [B] and page_table [B, pages], got ",
+          lengths.sizes(), " and ", table.sizes());
+    const int64_t B = lengths.size(0), max_tokens = integer(a[4]);
+    VALUE(max_tokens >= 0 && max_tokens <= INT32_MAX, "max_tokens is out of range: ", max_tokens);
+    VALUE(B <= 1 || table.size(1) == 0 || table.stride(0) >= table.size(1), "page_table's rows overlap");
+    const int32_t *lp = counts(lengths, "lengths", B, dev), *np = counts(fresh_tokens, "new_tokens", B, dev);
+    index_tensor(table, "page_table", dev);
+    const int32_t *fp = nullptr, *tp = nullptr;
+    int64_t num_free = 0;
+    const bool grows = a[5] != Py_None;
+    VALUE(grows == (a[6] != Py_None), "free_pages and taken go together");
+    if (grows) {
+        const at::Tensor &pages = tensor(a[5], "free_pages");
+        fp = counts(pages, "free_pages", -1, dev);
+        tp = counts(tensor(a[6], "taken"), "taken", 1, dev);
+        num_free = pages.size(0);
+    }
+    TYPE(a[7] == Py_None || (PyTuple_Check(a[7]) && PyTuple_GET_SIZE(a[7]) == 5), "out must be what a call returned: (positions, slots, q_starts, kv_lens, taken)");
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor positions = result(a[7], 0, "positions", max_tokens, at::kLong, dev), slots = result(a[7], 1, "slots", max_tokens, at::kLong, dev);
+    at::Tensor starts = result(a[7], 2, "q_starts", B + 1, at::kInt, dev), lens = result(a[7], 3, "kv_lens", B, at::kInt, dev);
+    at::Tensor taken;
+    if (grows) taken = result(a[7], 4, "taken", 1, at::kInt, dev);
+    // (an empty free list has no address of its own)
+    if (grows && !fp) fp = tp;
+    check(p_plan_step(const_cast<int32_t *>(table.const_data_ptr<int32_t>()), B > 1 ? table.stride(0) : table.size(1), table.size(1), lp, np,
+                      B, int32(a[3], "page_size"), max_tokens, fp, num_free, tp, positions.mutable_data_ptr<int64_t>(),
+                      slots.mutable_data_ptr<int64_t>(), starts.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(),
+                      grows ? taken.mutable_data_ptr<int32_t>() : nullptr, stream_of(dev)));
+    PyObject *last = Py_None;
+    if (grows) last = THPVariable_Wrap(std::move(taken));
+    else Py_INCREF(last);
+    return Py_BuildValue("NNNNN", THPVariable_Wrap(std::move(positions)), THPVariable_Wrap(std::move(slots)),
+                         THPVariable_Wrap(std::move(starts)), THPVariable_Wrap(std::move(lens)), last);
+}
+
+// A setting of sample: a tensor with one number for each row, or a number for all.
+template <typename N>
+struct Setting {
+    const N *each = nullptr;
+    PyObject *all = nullptr;
+};
+template <typename N>
+Setting<N> setting(PyObject *o, const char *name, int64_t B, c10::Device dev) {
+    Setting<N> s;
+    if (!THPVariable_Check(o)) {
+        s.all = o;
+        return s;
+    }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    constexpr at::ScalarType type = std::is_same_v<N, float> ? at::kFloat : at::kInt;
+    VALUE(t.dim() == 1 && t.size(0) == B && t.is_contiguous() && t.device() == dev, name, " must be a number or a contiguous vector of ", B,
+          " on ", dev, ", got ", t.sizes(), " on ", t.device());
+    TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    s.each = t.const_data_ptr<N>();
+    return s;
+}
+
+// (logits, u, temperature, top_k, top_p, min_p, logprobs) -> tokens, or (tokens, logprobs)
+PyObject *sample(PyObject *const *a) {
+    at::Tensor x = tensor(a[0], "logits");
+    const at::Tensor &u = tensor(a[1], "u");
+    const c10::Device dev = on_cuda(x);
+    VALUE(x.dim() == 2 && x.size(1) > 0, "logits must be [rows, vocabulary], got ", x.sizes());
+    const int64_t B = x.size(0), V = x.size(1);
+    const int dt = dtype_code(x);
+    TYPE(u.scalar_type() == at::kFloat, "u must be float32, got ", u.scalar_type());
+    VALUE(u.dim() == 1 && u.size(0) == B && u.is_contiguous() && u.device() == dev, "u must be a contiguous vector of ", B, " on ", dev,
+          ", got ", u.sizes(), " on ", u.device());
+    const Setting<float> t = setting<float>(a[2], "temperature", B, dev), p = setting<float>(a[4], "top_p", B, dev),
+                         m = setting<float>(a[5], "min_p", B, dev);
+    const Setting<int32_t> k = setting<int32_t>(a[3], "top_k", B, dev);
+    const double t_all = t.all ? real(t.all) : 0.0, p_all = p.all ? real(p.all) : 0.0, m_all = m.all ? real(m.all) : 0.0;
+    const int64_t k_all = k.all ? integer(k.all) : 0;
+    VALUE(t_all >= 0.0, "temperature must not be negative, got ", t_all);
+    VALUE(k_all >= 0, "top_k must not be negative, got ", k_all);
+    VALUE(p_all >= 0.0, "top_p must not be negative, got ", p_all);
+    VALUE(m_all >= 0.0 && m_all <= 1.0, "min_p must be in [0, 1], got ", m_all);
+    const bool wants = truth(a[6]);
+    const c10::cuda::CUDAGuard guard(dev);
+    if (V > 1 && x.stride(1) != 1) x = x.contiguous();
+    at::Tensor tokens = fresh({B}, at::kLong, dev), logprobs;
+    if (wants) logprobs = fresh({B}, at::kFloat, dev);
+    check(p_sample(x.const_data_ptr(), dt, B > 1 ? x.stride(0) : V, B, V, u.const_data_ptr<float>(), t.each, t_all, k.each, k_all,
+                   p.each, p_all, m.each, m_all, tokens.mutable_data_ptr<int64_t>(), wants ? logprobs.mutable_data_ptr<float>() : nullptr,
+                   stream_of(dev)));
+    if (!wants) return THPVariable_Wrap(std::move(tokens));
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(tokens)), THPVariable_Wrap(std::move(logprobs)));
 }
 
 std::vector<int32_t> indices(PyObject *o, const char *name) {
@@ -330,9 +453,9 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // (error class, addresses in the order below)
 PyObject *init(PyObject *, PyObject *args) {
-    unsigned long long f[7];
+    unsigned long long f[10];
     PyObject *err;
-    if (!PyArg_ParseTuple(args, "OKKKKKKK", &err, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6])) return nullptr;
+    if (!PyArg_ParseTuple(args, "OKKKKKKKKKK", &err, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8], &f[9])) return nullptr;
     Py_INCREF(err);
     g_error = err;
     p_norm_residual = reinterpret_cast<decltype(p_norm_residual)>(f[1]);
@@ -341,6 +464,9 @@ PyObject *init(PyObject *, PyObject *args) {
     p_paged_attention = reinterpret_cast<decltype(p_paged_attention)>(f[4]);
     p_paged_attention_workspace_size = reinterpret_cast<decltype(p_paged_attention_workspace_size)>(f[5]);
     p_copy_pages = reinterpret_cast<decltype(p_copy_pages)>(f[6]);
+    p_sink_attention = reinterpret_cast<decltype(p_sink_attention)>(f[7]);
+    p_plan_step = reinterpret_cast<decltype(p_plan_step)>(f[8]);
+    p_sample = reinterpret_cast<decltype(p_sample)>(f[9]);
     p_last_error = reinterpret_cast<decltype(p_last_error)>(f[0]);
     Py_RETURN_NONE;
 }
@@ -351,8 +477,9 @@ PyMethodDef method(const char *name) {
 }
 PyMethodDef g_methods[] = {
     {"init", init, METH_VARARGS, nullptr},  method<norm_residual, 11>("norm_residual"), method<rope, 5>("rope"),
-    method<rope_append, 9>("rope_append"),  method<paged_attention, 13>("paged_attention"),
-    method<copy_pages, 3>("copy_pages"),    {nullptr, nullptr, 0, nullptr},
+    method<rope_append, 9>("rope_append"),  method<paged_attention, 14>("paged_attention"),
+    method<copy_pages, 3>("copy_pages"),    method<plan_step, 8>("plan_step"), method<sample, 7>("sample"),
+    {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -68,6 +68,7 @@ enum : unsigned {
     DEV_ERR_TIMEOUT_EMPTY = 1u << 1,
     DEV_ERR_TIMEOUT_ACC = 1u << 2,
     DEV_ERR_BAD_INDEX = 1u << 3,
+    DEV_ERR_NO_ROOM = 1u << 4,  // a planned step needs more pages, columns or rows than there are
 };
 // Defined here: libqlinear is built as a single translation unit (libqlinear.cu).
 __device__ unsigned g_dev_error = 0;

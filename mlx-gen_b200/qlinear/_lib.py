@@ -50,6 +50,9 @@ EXPORTS = (
     "ql_paged_attention",
     "ql_paged_attention_workspace_size",
     "ql_copy_pages",
+    "ql_sink_attention",
+    "ql_plan_step",
+    "ql_sample",
 )
 
 
@@ -128,7 +131,13 @@ def lib():
         L.ql_paged_attention_workspace_size.argtypes = [i64, i32, i32, i32, i64, i64, i64, i64]
         L.ql_paged_attention_workspace_size.restype = sz
         L.ql_copy_pages.argtypes = [vp, i64, i64, i64, i64, i64, vp, vp, i64, vp]
-        for f in ("ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention", "ql_copy_pages"):
+        L.ql_sink_attention.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i64, i64, i32, vp, i64, vp, vp,
+                                        i64, i64, i64, f32, i64, i64, vp, vp, sz, vp]
+        L.ql_plan_step.argtypes = [vp, i64, i64, vp, vp, i64, i32, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
+        L.ql_sample.argtypes = [vp, i32, i64, i64, i64, vp, vp, C.c_double, vp, i64, vp, C.c_double, vp, C.c_double, vp,
+                                vp, vp]
+        for f in ("ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention", "ql_copy_pages",
+                  "ql_sink_attention", "ql_plan_step", "ql_sample"):
             getattr(L, f).restype = i32
         for f in ("ql_quantize", "ql_dequantize", "ql_dequantize_rows", "ql_layernorm_modulate", "ql_quantized_matmul",
                   "ql_quantized_matmul_noalloc"):
@@ -144,6 +153,7 @@ def check(status: int) -> None:
 
 
 DEV_ERR_TIMEOUT_FULL, DEV_ERR_TIMEOUT_EMPTY, DEV_ERR_TIMEOUT_ACC, DEV_ERR_BAD_INDEX = 1, 2, 4, 8
+DEV_ERR_NO_ROOM = 16
 INJECT_GEMM_PRODUCER_SILENT = 1
 INJECT_ATTENTION_PRODUCER_SILENT = 2
 INJECT_ATTENTION_PRODUCER_STOPS = 4
@@ -158,5 +168,5 @@ def debug_inject(flags: int = 0, wait_limit_ns: int = 0) -> None:
 
 
 def device_error(clear: bool = True) -> int:
-    """Device-side error word (bounded-wait timeouts, bad gather ids); 0 = none."""
+    """Device-side error word (bounded-wait timeouts, bad gather ids, steps without room); 0 = none."""
     return lib().ql_device_error(1 if clear else 0)

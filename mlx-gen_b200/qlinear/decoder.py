@@ -1,6 +1,7 @@
 """Decoder operators: what stands between the quantized linears of a decoder layer or a DiT
 block -- the residual norm, rotary positions with the append to a paged cache, attention over
-that cache, and copies of its pages.
+that cache (with a window and sinks), copies of its pages -- and between one decode step and the next:
+sampling and the next step's index tensors.
 
 torch holds the device memory and names the stream; the arithmetic runs in libqlinear's
 kernels (include/qlinear.h describes each call).  Wrong shapes, types and devices raise
@@ -35,8 +36,8 @@ class _Native:
         L = lib()
         m.init(_lib.QlError, *(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
             "ql_last_error", "ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention",
-            "ql_paged_attention_workspace_size", "ql_copy_pages")))
-        for f in ("norm_residual", "rope", "rope_append", "paged_attention", "copy_pages"):
+            "ql_paged_attention_workspace_size", "ql_copy_pages", "ql_sink_attention", "ql_plan_step", "ql_sample")))
+        for f in ("norm_residual", "rope", "rope_append", "paged_attention", "copy_pages", "plan_step", "sample"):
             setattr(self, f, getattr(m, f))
         return self.__dict__[name]
 
@@ -181,7 +182,7 @@ def paged_attention_workspace_size(T: int, Hq: int, Hkv: int, D: int, B: int, ma
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     q_starts: torch.Tensor, kv_lens: torch.Tensor, *, max_q: int, max_kv: int,
-                    scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                    scale: Optional[float] = None, causal: bool = True, window: int = 0, sinks: int = 0,
                     out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of each sequence's new tokens over its pages (their own keys and values already
     appended).  q ``[T, Hq, D]``: all sequences' new tokens, sequence b's from ``q_starts[b]`` to
@@ -190,9 +191,46 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the longest sequence (upper bounds are fine: a captured graph replays with the bounds it was
     captured with).  scale: ``1 / sqrt(D)`` by default.  Token i of q_len stands at ``p = kv_len -
     q_len + i`` and sees the positions up to p (all, without ``causal``), with a window only the
-    last ``window`` of them.  Returns ``[T, Hq, D]``; a token that sees nothing gets zeros."""
+    last ``window`` of them and, with sinks (at most 1024), the sequence's first ``sinks`` positions, which
+    stay visible; pages between the two are not used and may be given back.  Returns ``[T, Hq, D]``; a token that sees nothing gets zeros."""
     return _native.paged_attention(q, k_cache, v_cache, page_table, q_starts, kv_lens, max_q, max_kv, scale, causal, window,
-                                   out, workspace)
+                                   sinks, out, workspace)
+
+
+# ------------------------------------------------------------------------ from step to step
+
+def plan_step(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor, *, page_size: int, max_tokens: int,
+              free_pages: Optional[torch.Tensor] = None, taken: Optional[torch.Tensor] = None,
+              out: Optional[tuple] = None) -> tuple:
+    """The index tensors of a step in which sequence b, ``lengths[b]`` tokens long, gets ``new_tokens[b]``
+    more (int32 ``[B]`` both): returns ``(positions, slots, q_starts, kv_lens, taken)`` for ``rope_append`` and
+    ``paged_attention`` -- int64 ``[max_tokens]`` twice, int32 ``[B + 1]`` and ``[B]``; rows behind the last new token
+    get position 0 and slot -1 (not cached).
+
+    ``page_table [B, pages]`` (int32).  With a free list -- ``free_pages`` (int32) and ``taken [1]``, the number of its
+    entries in use -- pages that the new tokens need are taken from it in the order of the sequences
+    and entered in the page table; the returned ``taken`` counts them.  Without, the table holds every page
+    already and ``taken`` is None.  A step that finds too few pages, columns or rows (or counts below 0) has no
+    tokens and changes nothing; ``device_error()`` tells.  ``out``: what an earlier call returned, to be
+    written again; its kv_lens may be ``lengths`` and its taken ``taken``, so that each replay of a captured call
+    goes one step on."""
+    return _native.plan_step(page_table, lengths, new_tokens, page_size, max_tokens, free_pages, taken, out)
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: bool = False):
+    """One token per row of ``logits [B, V]`` from the random numbers ``u [B]`` (float32 in [0, 1)): int64 ``[B]``,
+    with ``logprobs`` also the logarithms of the probabilities with which they were drawn (float32 ``[B]``)::
+
+        w_i = exp((x_i - max x) / temperature)
+        in the order of x (descending, equal ones by index) stay: the first top_k; of those the shortest
+        prefix with a sum of at least top_p times theirs; of those the ones with w_i >= min_p
+        token = the first that stays, by index, with (sum up to it) > u * (sum of all that stay)
+
+    Each setting is a number or a tensor ``[B]`` (float32, top_k int32) with each row's own; top_k 0, top_p 1 and
+    min_p 0 filter nothing.  temperature 0 takes the largest logit, the lowest index of equal ones.
+    Sums are exact, so a row's token does not depend on the rest of the batch.  A row with a NaN
+    (among the logits or its settings), a negative temperature or no logit above -inf gives token -1 and log-probability NaN."""
+    return _native.sample(logits, u, temperature, top_k, top_p, min_p, logprobs)
 
 
 # ------------------------------------------------------------------------ pages

@@ -156,6 +156,20 @@ extern "C" {
                               workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn ql_paged_attention_workspace_size(t: i64, hq: c_int, hkv: c_int, d: c_int, b: i64, max_q: i64,
                                              max_kv: i64, window: i64) -> usize;
+    pub fn ql_sink_attention(q: *const c_void, dtype: c_int, q_token_stride: i64, q_head_stride: i64, t: i64,
+                             hq: c_int, hkv: c_int, d: c_int, k_cache: *const c_void, v_cache: *const c_void,
+                             num_pages: i64, page_stride: i64, page_size: c_int, page_table: *const i32,
+                             table_stride: i64, q_starts: *const i32, kv_lens: *const i32, b: i64, max_q: i64,
+                             max_kv: i64, scale: f32, window: i64, sinks: i64, out: *mut c_void,
+                             workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ql_plan_step(page_table: *mut i32, table_stride: i64, table_width: i64, lengths: *const i32,
+                        new_tokens: *const i32, b: i64, page_size: c_int, max_tokens: i64, free_pages: *const i32,
+                        num_free: i64, taken: *const i32, positions: *mut i64, slots: *mut i64, q_starts: *mut i32,
+                        kv_lens: *mut i32, taken_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ql_sample(logits: *const c_void, dtype: c_int, row_stride: i64, b: i64, v: i64, u: *const f32,
+                     temperature: *const f32, temperature_all: f64, top_k: *const i32, top_k_all: i64,
+                     top_p: *const f32, top_p_all: f64, min_p: *const f32, min_p_all: f64, tokens: *mut i64,
+                     logprobs: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ql_copy_pages(pool: *mut c_void, planes: i64, plane_stride: i64, num_pages: i64, page_stride: i64,
                          page_bytes: i64, src: *const i32, dst: *const i32, n: i64, stream: *mut c_void) -> c_int;
 }

@@ -307,6 +307,60 @@ pub fn paged_attention(q: Heads, dtype: Dtype, t: i64, q_heads: i32, kv: &PagedK
     })
 }
 
+/// [`paged_attention`], causal, with the first `sinks` positions visible beside the window; the same workspace.
+#[allow(clippy::too_many_arguments)]
+pub fn sink_attention(q: Heads, dtype: Dtype, t: i64, q_heads: i32, kv: &PagedKv, s: &Sequences, scale: f32, window: i64,
+                      sinks: i64, out: DevicePtr, workspace: DevicePtr, workspace_bytes: usize, stream: Stream) -> Result<()> {
+    check(unsafe {
+        sys::ql_sink_attention(q.ptr.0, dtype.raw(), q.token_stride, q.head_stride, t, q_heads, kv.kv_heads, kv.head_dim,
+                               kv.k.0, kv.v.0, kv.num_pages, kv.page_stride, kv.page_size, s.page_table.0 as *const i32,
+                               s.table_stride, s.q_starts.0 as *const i32, s.kv_lens.0 as *const i32, s.b, s.max_q,
+                               s.max_kv, scale, window, sinks, out.0, workspace.0, workspace_bytes, stream.0)
+    })
+}
+
+/// A list of free pages on the device (i32) and how many of its entries are taken (`[1]`, read and written).
+#[derive(Debug, Clone, Copy)]
+pub struct FreePages {
+    pub pages: DevicePtr,
+    pub count: i64,
+    pub taken: DevicePtr,
+}
+
+/// Positions, slots and offsets of the step in which sequence i of `s.b` gets `new_tokens[i]` tokens; advances
+/// `s.kv_lens` in place and writes `s.q_starts`.  `positions` and `slots`: i64 `[max_tokens]`.
+#[allow(clippy::too_many_arguments)]
+pub fn plan_step(s: &Sequences, table_width: i64, new_tokens: DevicePtr, page_size: i32, max_tokens: i64, free: Option<FreePages>,
+                 positions: DevicePtr, slots: DevicePtr, stream: Stream) -> Result<()> {
+    let null = std::ptr::null_mut();
+    let (pages, count, taken) = free.map_or((null, 0, null), |f| (f.pages.0, f.count, f.taken.0));
+    check(unsafe {
+        sys::ql_plan_step(s.page_table.0 as *mut i32, s.table_stride, table_width, s.kv_lens.0 as *const i32,
+                          new_tokens.0 as *const i32, s.b, page_size, max_tokens, pages as *const i32, count,
+                          taken as *const i32, positions.0 as *mut i64, slots.0 as *mut i64, s.q_starts.0 as *mut i32,
+                          s.kv_lens.0 as *mut i32, taken as *mut i32, stream.0)
+    })
+}
+
+/// Settings of [`sample`], the same for all rows (top_k 0, top_p 1 and min_p 0: no filter; temperature 0: the largest).
+#[derive(Debug, Clone, Copy)]
+pub struct Sampling {
+    pub temperature: f64,
+    pub top_k: i64,
+    pub top_p: f64,
+    pub min_p: f64,
+}
+
+/// One token per row of `logits` `[b, v]` from random numbers `u` `[b]` (f32 in [0, 1)): `tokens` i64 `[b]`.
+#[allow(clippy::too_many_arguments)]
+pub fn sample(logits: DevicePtr, dtype: Dtype, b: i64, v: i64, u: DevicePtr, s: &Sampling, tokens: DevicePtr, stream: Stream) -> Result<()> {
+    let null = std::ptr::null();
+    check(unsafe {
+        sys::ql_sample(logits.0, dtype.raw(), v, b, v, u.0 as *const f32, null, s.temperature, std::ptr::null(), s.top_k, null,
+                       s.top_p, null, s.min_p, tokens.0 as *mut i64, std::ptr::null_mut(), stream.0)
+    })
+}
+
 /// Copies pages `src[i]` to `dst[i]` in each of `planes` planes of a pool.
 pub fn copy_pages(pool: DevicePtr, planes: i64, plane_stride: i64, num_pages: i64, page_bytes: i64, src: &[i32],
                   dst: &[i32], stream: Stream) -> Result<()> {
