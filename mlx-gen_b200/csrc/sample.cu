@@ -27,11 +27,14 @@ namespace samplek {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int BINS = 2048, GROUPS = 32, GROUP = BINS / GROUPS;  // of a histogram
-constexpr int LIST = 512;         // elements that are compared one by one (one a thread)
-constexpr int MAX_CTAS = 8;       // of a cluster
+constexpr int LIST = 512;         // elements that are put in order one by one (one a thread)
+constexpr int WINDOW = 128;       // .. that top-p's border is looked for among
+constexpr int FEW = 128;          // .. up to which each is compared with every other
+constexpr int NEAR = 128;         // bins around a group that are looked at together
+constexpr int MAX_CTAS = 16;      // of a cluster
 constexpr int MAX_SLICE = 160 << 10;  // bytes of a row in one CTA's shared memory
 constexpr uint32_t NO_INDEX = 0xffffffffu;
-static_assert(LIST <= THREADS && GROUPS == 32 && GROUP == 64 && BINS == 4 * THREADS, "the divisions among threads and lanes below");
+static_assert(LIST <= THREADS && THREADS == 512 && MAX_CTAS <= WARPS && NEAR == 4 * 32 && GROUPS == 32 && GROUP == 64 && BINS == 4 * THREADS, "the divisions among threads and lanes below");
 
 struct Params {
     const void *logits;
@@ -63,19 +66,25 @@ struct Shared {
         struct {
             uint32_t lo[BINS / 2], hi[BINS / 2];    // sums of weights as lo + 2^32 hi
         };
-        struct {                                    // the cluster's list
-            ulonglong2 all[LIST];                   // place in the order (place_of), weight
-        };
+        uint64_t near_group[MAX_CTAS][GROUPS];      // what the warps read of the CTAs' histograms
+        uint32_t near_bins[MAX_CTAS / 2][2 * NEAR];
     };
+    uint32_t offset[BINS];                          // sums of the elements' places in their bins, in 256ths
     uint64_t group[2][GROUPS];                      // sums of a histogram's groups of bins
-    uint32_t group_count[2][GROUPS];
-    uint32_t list_key[LIST], list_index[LIST];      // this CTA's part of it
+    uint32_t group_count[2][GROUPS], elements[GROUPS];
+    uint64_t list[LIST];                            // this CTA's part of it: places
+    uint64_t other[THREADS];                        // a value of each thread
+    ulonglong2 all[FEW];                            // of few elements: places and weights
     double table[16];
-    uint64_t warp_sum[WARPS];
-    uint64_t cta_sum[2];
-    uint32_t warp_max[WARPS], warp_min[WARPS], cta_max, cta_min, cta_first;
-    uint32_t list_count[2], tie_index[2];
-    // what warp 0 found in a histogram
+    uint64_t warp_sum[WARPS], scratch[3][WARPS];
+    uint32_t warp_max[WARPS], warp_min[WARPS], first, tie;
+    uint32_t list_count[2];
+    // written by each CTA of the cluster, for itself and the others, before a barrier
+    uint64_t sum_of[2][MAX_CTAS];
+    uint32_t max_of[MAX_CTAS], min_of[MAX_CTAS], first_of[MAX_CTAS], tie_of[2][MAX_CTAS], listed_of[2][MAX_CTAS];
+    // what warp 0 found
+    uint64_t sum, before;
+    uint32_t listed;
     uint64_t found_before, found_estimate;
     uint32_t found_bin, found_count, found_first, found_last;
     int hit;
@@ -164,30 +173,43 @@ __device__ __forceinline__ uint64_t ld_cluster_u64(const void *p, uint32_t rank)
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
     return v;
 }
-// f(CTA) of each of the cluster's, its loads in flight together; 0 past the last
-template <typename V, typename F>
-__device__ __forceinline__ void of_all(V (&v)[MAX_CTAS], uint32_t ctas, F f) {
-#pragma unroll
-    for (uint32_t c = 0; c < MAX_CTAS; ++c) v[c] = c < ctas ? f(c) : V(0);
+__device__ __forceinline__ void st_cluster_u32(void *p, uint32_t rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), rank)), "r"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t sum_u32(const void *p, uint32_t ctas) {
-    uint32_t v[MAX_CTAS], s = 0;
-    of_all(v, ctas, [&](uint32_t c) { return ld_cluster_u32(p, c); });
+__device__ __forceinline__ void st_cluster_u64(void *p, uint32_t rank, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), rank)), "l"(v) : "memory");
+}
+// *p += n where `in`, without a branch: a warp's elements stay one block of instructions
+__device__ __forceinline__ void add_if(uint32_t *p, uint32_t n, bool in) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p red.shared::cta.add.u32 [%0], %1;\n\t}" ::"r"(smem_u32(p)), "r"(n), "r"((uint32_t)in)
+                 : "memory");
+}
+// Sum of a word of all CTAs.  Eight loads are in flight together, without a branch between them: they take as long as
+// one (5000 cycles for three such sums of 16 CTAs one after the other).  ctas: a power of two.
+template <typename V, typename L>
+__device__ __forceinline__ V sum_of_ctas(uint32_t ctas, L load) {
+    V s = 0;
+    for (uint32_t c0 = 0; c0 < ctas; c0 += 8) {
+        V v[8];
 #pragma unroll
-    for (int c = 0; c < MAX_CTAS; ++c) s += v[c];
+        for (uint32_t c = 0; c < 8; ++c) v[c] = load((c0 + c) & (ctas - 1));
+#pragma unroll
+        for (uint32_t c = 0; c < 8; ++c) s += c0 + c < ctas ? v[c] : V(0);
+    }
     return s;
 }
-__device__ __forceinline__ uint64_t sum_u64(const void *p, uint32_t ctas) {
-    uint64_t v[MAX_CTAS], s = 0;
-    of_all(v, ctas, [&](uint32_t c) { return ld_cluster_u64(p, c); });
-#pragma unroll
-    for (int c = 0; c < MAX_CTAS; ++c) s += v[c];
-    return s;
+__device__ __noinline__ uint32_t sum_u32(const uint32_t *p, uint32_t ctas) {
+    return sum_of_ctas<uint32_t>(ctas, [&](uint32_t c) { return ld_cluster_u32(p, c); });
 }
+__device__ __noinline__ uint64_t sum_u64(const uint64_t *p, uint32_t ctas) {
+    return sum_of_ctas<uint64_t>(ctas, [&](uint32_t c) { return ld_cluster_u64(p, c); });
+}
+// (modulo 2^64, in three parts whose sums fit 32 bits: a third of the time of five rounds of shuffles)
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3fffffu);
+    const uint32_t b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 22) & 0x1fffffu);
+    const uint32_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 43));
+    return a + ((uint64_t)b << 22) + ((uint64_t)c << 43);
 }
 __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
     const int lane = threadIdx.x & 31;
@@ -197,6 +219,61 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
         if (lane >= o) v += up;
     }
     return v;
+}
+
+// The block's values in falling order, thread t the t-th; only the first 2^log threads hold any (else 0).  A bitonic
+// network: distances within a warp by shuffles, the others through `buf`.
+__device__ __noinline__ uint64_t sort_down(uint64_t v, int log, uint64_t *buf) {
+    const int tid = threadIdx.x;
+    for (int k = 1; k <= log; ++k)
+        for (int j = k - 1; j >= 0; --j) {
+            uint64_t o;
+            if (j >= 5) {
+                __syncthreads();
+                buf[tid] = v;
+                __syncthreads();
+                o = buf[tid ^ (1 << j)];
+            } else o = __shfl_xor_sync(0xffffffffu, v, 1 << j);
+            const bool larger = ((tid >> j) & 1) == ((tid >> k) & 1);
+            v = (v > o) == larger ? v : o;
+        }
+    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ int log_of(uint32_t n) { return n > 1 ? 32 - __clz((int)(n - 1)) : 0; }  // 2^log >= n
+// Inclusive sum over the block's threads up to this one; `total` of all.  scratch: WARPS words, free after the next barrier.
+__device__ __noinline__ uint64_t block_scan(uint64_t v, uint64_t *scratch, uint64_t &total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    v = warp_scan(v);
+    if (lane == 31) scratch[warp] = v;
+    __syncthreads();
+    uint64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        const uint64_t x = scratch[w];
+        before += w < warp ? x : 0ull;
+        all += x;
+    }
+    total = all;
+    return v + before;
+}
+
+// Of `count` <= FEW elements, thread t's the t-th: how many have a larger place, and the sum of their weights.
+__device__ __noinline__ ulonglong2 sum_over_few(Shared *sh, uint32_t count, uint64_t place, uint64_t weight) {
+    const uint32_t tid = threadIdx.x;
+    __syncthreads();
+    if (tid < FEW) sh->all[tid] = make_ulonglong2(place, weight);
+    __syncthreads();
+    uint64_t s = 0;
+    uint32_t n = 0;
+    if (tid < count)
+#pragma unroll 8
+        for (uint32_t k = 0; k < count; ++k) {
+            const ulonglong2 a = sh->all[k];
+            s += a.x > place ? a.y : 0ull;
+            n += a.x > place ? 1u : 0u;
+        }
+    return make_ulonglong2(n, s);
 }
 
 // fp32 to fp64 in integer instructions (the conversion has a quarter of the fp64 rate).  Values below 2^-126 keep their
@@ -215,8 +292,8 @@ struct Weigher {
     int scale;         // S
     const double *table;
 
-    __device__ __forceinline__ Weigher(float largest, double temperature, int scale_, const double *table_)
-        : max(widen(largest)), scale(scale_), table(table_) {
+    // all but the row's largest logit, which comes later
+    __device__ __forceinline__ Weigher(double temperature, int scale_, const double *table_) : max(0.0), scale(scale_), table(table_) {
         // The temperature is held between 2e-29 and 4e28: beyond, only logits below 1e-26 or above 1e26 could
         // tell the difference.
         const double limit = 16.0 * (scale + 2);
@@ -244,7 +321,7 @@ struct Weigher {
     }
     __device__ __forceinline__ uint64_t operator()(float x, bool keep = true) const { return biased(x, keep) - BIAS; }
     // ln(w / sum): w from its distance, the sum without its factor 2^S
-    __device__ __forceinline__ float logprob(float x, uint64_t sum) const {
+    __device__ __noinline__ float logprob(float x, uint64_t sum) const {
         return (float)((widen(x) - max) * (rate * C) - log((double)sum * exp2(-(double)scale)));
     }
     // the same, 0 where w 2^S is below `least`
@@ -254,6 +331,9 @@ struct Weigher {
         return t * e >= least ? (uint64_t)__double_as_longlong(fma(t, e, 4503599627370496.0)) - BIAS : 0ull;
     }
 };
+
+// One weight, where no loop needs it inlined (most of the kernel's time with few rows is instruction fetches).
+__device__ __noinline__ uint64_t weight_of(const Weigher w, float x, double least) { return w.at_least(x, true, least); }
 
 template <bool CLUSTER>
 __device__ __forceinline__ void sync_all() {
@@ -269,11 +349,12 @@ struct Row {
     static constexpr int N = Ty::N, UNIT = Ty::UNIT;
     uint4 *data;
     Shared *sh;
-    int first, last;         // this warp's words
+    int first, last;         // this warp's words, `per` of them
+    int per, tokens;         // .. and the slice's tokens
     int skew;                // places before the slice in the first word
     uint32_t base;           // index of the slice's first token
     uint32_t ctas, rank;
-    uint64_t *slot;          // of the next sum
+    int sums;                // so far
     int turn;                // of the next histogram
 
     __device__ __forceinline__ uint32_t index(int word, int e) const { return base + (uint32_t)(word * N + e - skew); }
@@ -309,6 +390,21 @@ struct Row {
         return x > cut.value || (x == cut.value && index(w, e) <= cut.index);
     }
 
+    // A value of this CTA to all CTAs (lanes of one warp); read after a barrier.
+    __device__ __forceinline__ void tell(uint32_t *of, uint32_t v) const {
+        const uint32_t lane = threadIdx.x & 31;
+        if (CLUSTER ? lane < ctas : lane == 0) {
+            if (CLUSTER) st_cluster_u32(&of[rank], lane, v);
+            else of[0] = v;
+        }
+    }
+    // Sum over the block (every thread has it); scratch[i] is free again after the next barrier.
+    __device__ __forceinline__ uint64_t block_sum(uint64_t v, int i) const {
+        v = warp_sum(v);
+        if ((threadIdx.x & 31) == 0) sh->scratch[i][threadIdx.x >> 5] = v;
+        __syncthreads();
+        return warp_sum((threadIdx.x & 31) < WARPS ? sh->scratch[i][threadIdx.x & 31] : 0ull);
+    }
     // Sum over the cluster of a value of each thread; `before` is that of the CTAs before this one, and
     // warp_sum[] holds the warps'.
     __device__ __forceinline__ uint64_t total(uint64_t v, uint64_t &before) {
@@ -317,17 +413,25 @@ struct Row {
         __syncthreads();
         if (lane == 0) sh->warp_sum[warp] = v;
         __syncthreads();
-        const uint64_t cta = warp_sum(lane < WARPS ? sh->warp_sum[lane] : 0ull);
         if (!CLUSTER) {
             before = 0;
-            return cta;
+            return warp_sum(lane < WARPS ? sh->warp_sum[lane] : 0ull);
         }
-        if (threadIdx.x == 0) *slot = cta;
+        uint64_t *of = sh->sum_of[sums++ & 1];
+        if (warp == 0) {
+            const uint64_t cta = warp_sum(lane < WARPS ? sh->warp_sum[lane] : 0ull);
+            if (lane < ctas) st_cluster_u64(&of[rank], lane, cta);
+        }
         cluster_sync_all();
-        const uint64_t mine = lane < ctas ? ld_cluster_u64(slot, lane) : 0ull;
-        slot = slot == &sh->cta_sum[0] ? &sh->cta_sum[1] : &sh->cta_sum[0];
-        before = warp_sum(lane < rank ? mine : 0ull);
-        return warp_sum(mine);
+        // (one warp for all: what every warp does for itself takes sixteen times the issue slots)
+        if (warp == 0) {
+            const uint64_t x = lane < ctas ? of[lane] : 0ull;
+            const uint64_t sum = warp_sum(x), first = warp_sum(lane < rank ? x : 0ull);
+            if (lane == 0) sh->sum = sum, sh->before = first;
+        }
+        __syncthreads();
+        before = sh->before;
+        return sh->sum;
     }
 
     // This CTA's elements for which f(x, w, e) holds, as its part of the list; the number of the cluster's.
@@ -339,56 +443,48 @@ struct Row {
         each_from(low, [&](float x, int w, int e) {
             if (f(x, w, e)) append(which, x, w, e);
         });
-        sync_all<CLUSTER>();
-        return sum_u32(&sh->list_count[which], ctas);
+        return share_list(which);
     }
     __device__ __forceinline__ void append(int which, float x, int w, int e) const {
         const uint32_t at = atomicAdd(&sh->list_count[which], 1u);
-        if (at < LIST) {
-            sh->list_key[at] = key_of<UNIT>(x);
-            sh->list_index[at] = index(w, e);
-        }
+        if (at < LIST) sh->list[at] = place_of(key_of<UNIT>(x), index(w, e));
     }
-    // Brings the cluster's list (at most LIST) together in all[]; true where this thread has an element of it.
-    // No CTA may refill its part before the others have read it: a barrier of the cluster stands
-    // before every collect.
-    template <typename M>
-    __device__ __forceinline__ bool gather(int which, uint64_t &place, uint64_t &own, M measure) const {
-        uint32_t n[MAX_CTAS], at = threadIdx.x, from = MAX_CTAS;
-        of_all(n, ctas, [&](uint32_t c) { return ld_cluster_u32(&sh->list_count[which], c); });
-#pragma unroll
-        for (uint32_t c = 0; c < MAX_CTAS; ++c) {  // this thread's element: the at-th of CTA `from`
-            if (from == MAX_CTAS && at < n[c]) from = c;
-            if (from == MAX_CTAS) at -= n[c];
-        }
-        const bool has = from < MAX_CTAS;
-        place = own = 0;
-        if (has) {
-            const uint32_t key = ld_cluster_u32(&sh->list_key[at], from);
-            place = place_of(key, ld_cluster_u32(&sh->list_index[at], from));
-            own = measure(value_of<UNIT>(key));
-            sh->all[threadIdx.x] = make_ulonglong2(place, own);
+    __device__ __forceinline__ uint32_t share_list(int which) const {
+        __syncthreads();
+        if (threadIdx.x < 32) tell(sh->listed_of[which], sh->list_count[which]);
+        sync_all<CLUSTER>();
+        if (threadIdx.x < 32) {
+            const uint32_t n = __reduce_add_sync(0xffffffffu, threadIdx.x < ctas ? sh->listed_of[which][threadIdx.x] : 0u);
+            if (threadIdx.x == 0) sh->listed = n;
         }
         __syncthreads();
-        return has;
+        return sh->listed;
+    }
+    // The cluster's list (`count`, at most LIST), an element a thread: its place, 0 past the last.  More than FEW come in
+    // their order.  No CTA may refill its part before the others have read it: a barrier of the cluster
+    // stands before every collect.
+    __device__ __forceinline__ uint64_t listed(int which, uint32_t count) const {
+        uint64_t place = 0;
+        if (threadIdx.x < count) {
+            uint32_t at = threadIdx.x, from = 0;  // the at-th of CTA `from`
+            for (uint32_t n; from < ctas && at >= (n = sh->listed_of[which][from]); ++from) at -= n;
+            if (from < ctas) place = CLUSTER ? ld_cluster_u64(&sh->list[at], from) : sh->list[at];
+        }
+        return count > FEW ? sort_down(place, log_of(count), sh->other) : place;
     }
     // Of the list's `count` elements in their order, the one at which the sum of the measure reaches
-    // `need`: sh->cut, and true; false if it does not.
+    // `need`: sh->cut, and true; false if it does not.  place, own: this thread's element.
     template <typename M>
-    __device__ __forceinline__ bool resolve(int which, uint32_t count, uint64_t need, M measure) const {
-        uint64_t place, own;
+    __device__ __forceinline__ bool resolve(int which, uint32_t count, uint64_t need, M measure, uint64_t &place, uint64_t &own) const {
         if (threadIdx.x == 0) sh->hit = 0;
-        if (gather(which, place, own, measure)) {
-            uint64_t before = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < count; ++i) {
-                const ulonglong2 a = sh->all[i];
-                before += a.x > place ? a.y : 0ull;
-            }
-            if (before + own >= need && before < need) {
-                sh->cut = {value_of<UNIT>((uint32_t)(place >> 32)), ~(uint32_t)place};
-                sh->hit = 1;
-            }
+        place = listed(which, count);
+        own = place ? measure(value_of<UNIT>((uint32_t)(place >> 32))) : 0ull;
+        uint64_t before;
+        if (count > FEW) before = block_scan(own, sh->scratch[2], before) - own;
+        else before = sum_over_few(sh, count, place, own).y;
+        if (before + own >= need && before < need) {
+            sh->cut = {value_of<UNIT>((uint32_t)(place >> 32)), ~(uint32_t)place};
+            sh->hit = 1;
         }
         __syncthreads();
         const bool hit = sh->hit != 0;
@@ -405,52 +501,49 @@ __device__ __forceinline__ void finish(const Row<T, CLUSTER> &row, const Weigher
                                        uint64_t need, double least, double u, int64_t *token, float *logprob) {
     constexpr int UNIT = Type<T>::UNIT;
     Shared *sh = row.sh;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    auto block_sum = [&](uint64_t v) {
-        v = warp_sum(v);
-        __syncthreads();
-        if (lane == 0) sh->warp_sum[warp] = v;
-        __syncthreads();
-        return warp_sum(lane < WARPS ? sh->warp_sum[lane] : 0ull);
-    };
-    uint64_t place, own;
-    bool stays = row.gather(which, place, own, [&](float x) { return weigh(x); });
+    const uint32_t tid = threadIdx.x;
+    const uint64_t place = row.listed(which, count);
     const float x = value_of<UNIT>((uint32_t)(place >> 32));
-    uint64_t before = 0;
-    uint32_t rank = 0;
-    if (stays)
-#pragma unroll 4
-        for (uint32_t i = 0; i < count; ++i) {
-            const ulonglong2 a = sh->all[i];
-            before += a.x > place ? a.y : 0ull;
-            rank += a.x > place ? 1u : 0u;
-        }
-    if (k) {
-        stays = stays && rank < k;
-        if (p < 1.0) {
-            const uint64_t sum = block_sum(stays ? own : 0ull);
-            const double target = ceil((double)sum * p);
-            need = target >= 1.0 ? min(sum, (uint64_t)target) : 1ull;
-        }
+    uint64_t own = place ? weight_of(weigh, x, 0.0) : 0ull, before, sum;
+    uint32_t rank = tid;
+    if (count > FEW) {
+        if (k && tid >= k) own = 0;
+        before = block_scan(own, sh->scratch[0], sum) - own;
+    } else {
+        const ulonglong2 r = sum_over_few(sh, count, place, own);
+        rank = (uint32_t)r.x, before = r.y;
+        if (k && rank >= k) own = 0;
+        if (k && p < 1.0) sum = row.block_sum(own, 0);
     }
-    if (need) stays = stays && before < need;
-    if (stays && least > 0.0) own = weigh.at_least(x, true, least);
-    if (!stays) own = 0;
-    const uint64_t sum = block_sum(own);  // (all[] has been read)
-    sh->all[tid] = make_ulonglong2(~(uint32_t)place, own);
-    __syncthreads();
-    if (!own) return;
+    if (k && p < 1.0) {
+        const double target = ceil((double)sum * p);
+        need = target >= 1.0 ? min(sum, (uint64_t)target) : 1ull;
+    }
+    if (need && before >= need) own = 0;
+    if (own && least > 0.0) own = weight_of(weigh, x, least);
+    // those that stay, by their indices (the lower half of a place falls as the index rises)
+    const uint32_t low = own ? (uint32_t)place : 0u;
+    uint64_t drawn = own;
+    uint32_t holder = tid;
+    if (count > FEW) {
+        // (sorted, so the first threads': a weight is never above the one before it)
+        const int stay = __syncthreads_count(own != 0);
+        const uint64_t by_index = sort_down(own ? (uint64_t)low << 32 | tid : 0ull, log_of(stay), sh->other);
+        sh->other[tid] = own;
+        __syncthreads();
+        holder = (uint32_t)by_index;
+        drawn = by_index ? sh->other[holder] : 0ull;
+        before = block_scan(drawn, sh->scratch[1], sum) - drawn;
+    } else {
+        sum = row.block_sum(own, 1);
+        before = sum_over_few(sh, count, low, own).y;
+    }
     const double at = fmax(u, 0.0) * (double)sum;
     const uint64_t target = at < (double)sum ? min((uint64_t)at, sum - 1) : sum - 1;
-    const uint32_t index = ~(uint32_t)place;
-    uint64_t upto = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < count; ++i) {
-        const ulonglong2 a = sh->all[i];
-        upto += (uint32_t)a.x < index ? a.y : 0ull;
-    }
-    if (upto <= target && target < upto + own) {
-        *token = index;
+    if (before <= target && target < before + drawn) sh->found_bin = holder;  // the thread that has its logit
+    __syncthreads();
+    if (tid == sh->found_bin) {
+        *token = ~(uint32_t)place;
         if (logprob) *logprob = weigh.logprob(x, sum);
     }
 }
@@ -472,8 +565,7 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER> &row, float to
     });
     __syncthreads();
     for (int g = warp; g < GROUPS; g += WARPS) {
-        const uint2 n = *reinterpret_cast<const uint2 *>(count + g * GROUP + 2 * lane);
-        const uint32_t s = __reduce_add_sync(0xffffffffu, n.x + n.y);
+        const uint32_t s = __reduce_add_sync(0xffffffffu, count[g * GROUP + lane] + count[g * GROUP + 32 + lane]);
         if (lane == 0) group[g] = s;
     }
     sync_all<CLUSTER>();
@@ -483,10 +575,10 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER> &row, float to
         const unsigned past = __ballot_sync(0xffffffffu, upto >= k);
         const int g = past ? __ffs(past) - 1 : 0;
         const uint64_t before = __shfl_sync(0xffffffffu, upto - s, g);
-        const uint64_t a = sum_u32(&count[g * GROUP + 2 * lane], row.ctas), b = sum_u32(&count[g * GROUP + 2 * lane + 1], row.ctas);
-        upto = before + warp_scan(a + b);
+        // (to two bins: the bound may be lower than it could be, not higher)
+        upto = before + warp_scan((uint64_t)(sum_u32(&count[g * GROUP + 2 * lane], row.ctas) + sum_u32(&count[g * GROUP + 2 * lane + 1], row.ctas)));
         const unsigned here = __ballot_sync(0xffffffffu, upto >= k);
-        if (here && lane == __ffs(here) - 1) sh->found_bin = g * GROUP + 2 * lane + (upto - b >= k ? 0 : 1);
+        if (here && lane == 0) sh->found_bin = g * GROUP + 2 * __ffs(here) - 1;
         if (!past && lane == 0) sh->found_bin = NO_INDEX;
     }
     __syncthreads();
@@ -504,7 +596,9 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER> &row, float to
 // holds the border, until it holds at most LIST elements or one value.
 template <bool WEIGHT, typename T, bool CLUSTER>
 __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, Cut cut, uint32_t high, uint32_t low, uint64_t need) {
-    constexpr int UNIT = Type<T>::UNIT, LOG = WEIGHT ? 10 : 11, PER = (1 << LOG) / GROUPS / 32;  // bins of a group's lane
+    constexpr int UNIT = Type<T>::UNIT, LOG = 10;
+    constexpr int BINS = 1 << LOG, GROUP = BINS / GROUPS;  // (half of the others': two more words a bin)
+    static_assert(GROUP == 32, "one bin a lane");
     Shared *sh = row.sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t cut_key = key_of<UNIT>(cut.value);
@@ -512,7 +606,7 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
     auto inside = [&](uint32_t key, int w, int e) {
         return key >= low && key <= high && (key != cut_key || row.index(w, e) <= cut.index);
     };
-    auto measure = [&](float x) { return WEIGHT ? weigh(x) : 1ull; };
+    auto measure = [&](float x) { return WEIGHT ? weight_of(weigh, x, 0.0) : 1ull; };
     for (;;) {
         const float from = value_of<UNIT>(low);
         const uint32_t range = high - low;
@@ -527,21 +621,10 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
         row.each_from(from, [&](float x, int w, int e) {
             const uint32_t key = key_of<UNIT>(x);
             const bool in = inside(key, w, e);
-            const unsigned active = __ballot_sync(0xffffffffu, in);
-            if (!active) return;
-            uint64_t weight = WEIGHT ? weigh(x, in) : 0ull;
-            // equal elements of a warp (a row of few values) count as one
-            uint32_t n = 1;
-            const uint32_t one = __shfl_sync(0xffffffffu, key, __ffs(active) - 1);
-            if (__all_sync(0xffffffffu, !in || key == one)) {
-                if (lane != __ffs(active) - 1) return;
-                n = __popc(active);
-                weight *= n;
-            }
-            if (!in) return;
-            const uint32_t b = (high - key) >> shift;
-            atomicAdd(&count[b], n);
-            if (WEIGHT) {
+            const uint32_t b = in ? (high - key) >> shift : 0u;
+            add_if(&count[b], 1u, in);
+            if (WEIGHT && in) {
+                const uint64_t weight = weigh(x);
                 const uint32_t lo = (uint32_t)weight, old = atomicAdd(&sh->lo[b], lo);
                 const uint32_t hi = (uint32_t)(weight >> 32) + (old + lo < old ? 1u : 0u);
                 if (hi) atomicAdd(&sh->hi[b], hi);
@@ -549,12 +632,8 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
         });
         __syncthreads();
         for (int g = warp; g < GROUPS; g += WARPS) {
-            uint64_t s = 0;
-            for (int k = 0; k < PER; ++k) {
-                const int i = (g * PER + k) * 32 + lane;
-                s += WEIGHT ? ((uint64_t)sh->hi[i] << 32) + sh->lo[i] : (uint64_t)count[i];
-            }
-            s = warp_sum(s);
+            const int i = g * GROUP + lane;
+            const uint64_t s = warp_sum(WEIGHT ? ((uint64_t)sh->hi[i] << 32) + sh->lo[i] : (uint64_t)count[i]);
             if (lane == 0) group[g] = s;
         }
         sync_all<CLUSTER>();
@@ -565,26 +644,21 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
             uint64_t upto = warp_scan(s);
             const unsigned past = __ballot_sync(0xffffffffu, upto >= need);
             const int g = past ? __ffs(past) - 1 : 0;
-            uint64_t before = __shfl_sync(0xffffffffu, upto - s, g);
-            bool found = false;
-            for (int k = 0; k < PER && !found; ++k) {
-                const int i = (g * PER + k) * 32 + lane;
-                const uint32_t n = sum_u32(&count[i], row.ctas);
-                s = n;
-                if (WEIGHT) {
-                    s = 0;
-                    for (uint32_t c = 0; c < row.ctas; ++c)
-                        s += (uint64_t)ld_cluster_u32(&sh->lo[i], c) + ((uint64_t)ld_cluster_u32(&sh->hi[i], c) << 32);
-                }
-                upto = before + warp_scan(s);
-                const unsigned here = __ballot_sync(0xffffffffu, upto >= need);
-                found = here != 0;
-                if (found && lane == __ffs(here) - 1) {
-                    sh->found_bin = i;
-                    sh->found_count = n;
-                    sh->found_before = upto - s;
-                }
-                before = __shfl_sync(0xffffffffu, upto, 31);
+            const uint64_t before = __shfl_sync(0xffffffffu, upto - s, g);
+            const int i = g * GROUP + lane;
+            const uint32_t n = sum_u32(&count[i], row.ctas);
+            s = n;
+            if (WEIGHT) {
+                s = 0;
+                for (uint32_t c = 0; c < row.ctas; ++c)
+                    s += (uint64_t)ld_cluster_u32(&sh->lo[i], c) + ((uint64_t)ld_cluster_u32(&sh->hi[i], c) << 32);
+            }
+            upto = before + warp_scan(s);
+            const unsigned here = __ballot_sync(0xffffffffu, upto >= need);
+            if (here && lane == __ffs(here) - 1) {
+                sh->found_bin = i;
+                sh->found_count = n;
+                sh->found_before = upto - s;
             }
             if (!past && lane == 0) sh->found_bin = NO_INDEX;
         }
@@ -597,7 +671,8 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
         __syncthreads();
         if (n <= LIST) {
             row.collect(WEIGHT, value_of<UNIT>(low), [&](float x, int w, int e) { return inside(key_of<UNIT>(x), w, e); });
-            return row.resolve(WEIGHT, n, need, measure) ? sh->cut : cut;
+            uint64_t place, own;
+            return row.resolve(WEIGHT, n, need, measure, place, own) ? sh->cut : cut;
         }
         if (shift == 0) {
             // more equal elements than that: the last of them that is needed, by index
@@ -608,7 +683,7 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
             row.each_from(value, [&](float x, int w, int e) { mine += inside(key_of<UNIT>(x), w, e) ? 1u : 0u; });
             row.total(mine, before);
             // the warp whose elements hold it looks for it; its CTA tells the others
-            if (tid == 0) sh->tie_index[WEIGHT] = NO_INDEX;
+            if (tid == 0) sh->tie = NO_INDEX;
             __syncthreads();
             uint64_t at = before;
             for (int i = 0; i < warp; ++i) at += sh->warp_sum[i];
@@ -624,117 +699,289 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, C
                         uint64_t left = ties - (upto - m);
 #pragma unroll
                         for (int e = 0; e < Type<T>::N; ++e)
-                            if (inside(key_of<UNIT>(x[e]), w, e) && --left == 0) sh->tie_index[WEIGHT] = row.index(w, e);
+                            if (inside(key_of<UNIT>(x[e]), w, e) && --left == 0) sh->tie = row.index(w, e);
                     }
                     at = __shfl_sync(0xffffffffu, upto, 31);
                 });
             }
+            __syncthreads();
+            if (warp == 0) row.tell(sh->tie_of[WEIGHT], sh->tie);
             sync_all<CLUSTER>();
             uint32_t ix = NO_INDEX;
-            for (uint32_t c = 0; c < row.ctas; ++c) ix = min(ix, ld_cluster_u32(&sh->tie_index[WEIGHT], c));
+            for (uint32_t c = 0; c < row.ctas; ++c) ix = min(ix, sh->tie_of[WEIGHT][c]);
             return {value, ix};
         }
     }
 }
 
+// Weights below (1 - p) / (2 V) of the largest (1, so of the sum) sum up to less than (1 - p), so none of them is in
+// top-p's prefix: how far below the largest logit the others may be (with a margin for roundings).
+__device__ __forceinline__ double reach_of(const Weigher &weigh, double p, int V) {
+    const double smallest = fmax(0.5, 0.5 * (1.0 - p) / V * exp2((double)weigh.scale));
+    return (weigh.scale - log2(smallest)) * 16.0 / weigh.rate * 1.000001;
+}
+
+// Where in the bins of width 1 / c below the largest logit an element is, and its bin, the nearest whole number, as 1.5 * 2^23
+// more (without a conversion, which has a quarter of the rate); x falling, neither falls.  Every step is rounded by
+// itself: passes that count and passes that list must agree on an element's bin, and a product and a sum that are
+// fused in one of them only would part them.
+constexpr float BIN0 = 12582912.f;
+__device__ __forceinline__ float bins_below(float top, float x, float c) { return __fmul_rn(__fsub_rn(top, x), c); }
+__device__ __forceinline__ float bin_at(float at) { return fminf(__fadd_rn(at, BIN0), BIN0 + (BINS - 1)); }
+
+// The passes over the logits, each a function of its own: inlined into one kernel they share its registers, and spilled
+// values in their loops tripled their time.
+// Sum of the weights within the cut; elements of at least `low` counted in bins of the width 1 / c below `top`.
+template <bool WHOLE, typename T, bool CLUSTER>
+__device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+                                               uint32_t *count) {
+    constexpr int N = Type<T>::N;
+    uint32_t *offset = row.sh->offset;
+    uint64_t mine = 0;
+    row.words_from(cut.value, [&](const uint4 &v, int w) {
+        float x[N];
+        Type<T>::load(v, x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) mine += weigh.biased(x[e], WHOLE || row.kept(cut, x[e], w, e));
+        mine -= N * Weigher::BIAS;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const bool in = x[e] >= low && (WHOLE || row.kept(cut, x[e], w, e));
+            const float at = in ? bins_below(top, x[e], c) : 0.f, bin = bin_at(at);
+            const uint32_t b = __float_as_uint(bin) - __float_as_uint(BIN0);
+            add_if(&count[b], 1u, in);
+            // (where in it, from its lower edge on: 0 to 256)
+            add_if(&offset[b], __float_as_uint(fmaf(at - (bin - BIN0), 256.f, BIN0 + 128.f)) - __float_as_uint(BIN0), in);
+        }
+    });
+    return mine;
+}
+// Sum of the weights within the cut, of at least `low` and before bin `first`; those in bins from that to `last` to the list.
+template <bool WHOLE, typename T, bool CLUSTER>
+__device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+                                              float first, float last) {
+    constexpr int N = Type<T>::N;
+    uint64_t mine = 0;
+    row.words_from(low, [&](const uint4 &v, int w) {
+        float x[N];
+        Type<T>::load(v, x);
+        uint32_t listed = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float bin = bin_at(bins_below(top, x[e], c));
+            const bool in = x[e] >= low && (WHOLE || row.kept(cut, x[e], w, e));
+            mine += weigh.biased(x[e], in && bin < first);
+            listed |= in && bin >= first && bin <= last ? 1u << e : 0u;
+        }
+        mine -= N * Weigher::BIAS;
+        if (listed) {
+            const T *p = reinterpret_cast<const T *>(row.data + w);
+#pragma unroll 1
+            for (int e = 0; e < N; ++e)
+                if (listed & (1u << e)) row.append(1, (float)p[e], w, e);
+        }
+    });
+    return mine;
+}
+// Sum of the weights within the cut, of at least `least`.
+template <bool PLAIN, typename T, bool CLUSTER>
+__device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, double least) {
+    constexpr int N = Type<T>::N;
+    uint64_t mine = 0;
+    row.words_from(cut.value, [&](const uint4 &v, int w) {
+        float x[N];
+        Type<T>::load(v, x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) mine += PLAIN ? weigh.biased(x[e], true) : weigh.at_least(x[e], row.kept(cut, x[e], w, e), least);
+        if (PLAIN) mine -= N * Weigher::BIAS;
+    });
+    return mine;
+}
+// One warp's elements within the cut and of at least `least`, `at` the sum of those before: the one at which it passes
+// `target` is the token.
+template <typename T, bool CLUSTER>
+__device__ __noinline__ void draw(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, double least, uint64_t at, uint64_t target,
+                                  uint64_t sum, int64_t *token, float *logprob) {
+    constexpr int N = Type<T>::N;
+    row.words_from(cut.value, [&](const uint4 &v, int w) {
+        if (at > target) return;
+        float x[N];
+        Type<T>::load(v, x);
+        uint64_t own[N], mine = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) mine += own[e] = weigh.at_least(x[e], row.kept(cut, x[e], w, e), least);
+        const uint64_t upto = at + warp_scan(mine);
+        if (upto > target && upto - mine <= target) {
+            uint64_t run = upto - mine;
+            float found = 0.f;
+            uint32_t index = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (run <= target && target < run + own[e]) index = row.index(w, e), found = x[e];
+                run += own[e];
+            }
+            *token = index;
+            if (logprob) *logprob = weigh.logprob(found, sum);
+        }
+        at = __shfl_sync(0xffffffffu, upto, 31);
+    });
+}
+
+enum Outcome { LISTED, CUT, CUT_AND_SUM };
 // Top-p among the elements within `cut`: their weights' sum `total`, of which the prefix has to reach `need` = p times that.  One
-// pass sums the weights and counts the elements in bins of equal width; each counted as an element at its bin's
-// middle, they say about where the border is.  (Sums of weights in each bin would cost three atomic additions
+// pass sums the weights and counts the elements in bins of equal width; each counted as an element in the
+// middle of those of its bin, they say about where the border is.  (Sums of weights in each bin would cost three atomic additions
 // for every element.)  Where all elements down to the border fit the list, the list is all that is needed: true, its
 // length in `listed`.  Else a pass over the elements above a few bins around the border sums them exactly and lists
 // those in the bins; where the border is not among these after all, the sum tells by how much the
 // estimate is off.  `cut` is then the one after the prefix.
 template <typename T, bool CLUSTER>
-__device__ __forceinline__ bool nucleus(Row<T, CLUSTER> &row, const Weigher &weigh, Cut &cut, float top, double p, int V, uint64_t &need,
-                                        uint32_t &listed) {
+__device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER> &row, const Weigher &weigh, Cut &cut, float top, double p, double reach, uint64_t &need,
+                                           uint32_t &listed, uint64_t &sum, uint64_t &before) {
     constexpr int UNIT = Type<T>::UNIT, N = Type<T>::N;
     Shared *sh = row.sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // Weights below (1 - p) / (2 V) of the largest (1, so of the sum) sum up to less than (1 - p), so none of them is in
-    // the prefix, and only logits above that (with a margin for roundings) are counted.
-    const double smallest = fmax(0.5, 0.5 * (1.0 - p) / V * exp2((double)weigh.scale));
-    const double reach = (weigh.scale - log2(smallest)) * 16.0 / weigh.rate * 1.000001;
     const float low = fmaxf(fminf(top, fmaxf((float)((double)top - reach - 1e-6 * fabs((double)top)), -3.4028234e38f)), cut.value);
     const float c = top > low ? (BINS - 1) / (top - low) : 0.f, width = top > low ? (top - low) / (BINS - 1) : 0.f;
-    // (not decreasing as x falls: every step is a rounded operation of that kind)
-    auto bin_of = [&](float x) { return min((int)((top - x) * c), BINS - 1); };
-    auto middle = [&](int b) { return weigh(fmaf(-(float)b - 0.5f, width, top)); };
+    // four bins' elements, each counted as one in the middle of its bin's
+    auto estimate = [&](const uint32_t (&n)[4], const uint32_t (&offset)[4], int b, uint64_t (&w)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float middle = (float)offset[q] / (256.f * (float)n[q]) - 0.5f;
+            w[q] = n[q] * weigh(fmaf(-((float)(b + q) + middle), width, top), n[q] != 0);
+        }
+    };
     uint32_t *count = sh->count[row.turn & 1], *group_count = sh->group_count[row.turn & 1];
     uint64_t *group = sh->group[row.turn & 1];
     ++row.turn;
     *reinterpret_cast<uint4 *>(count + 4 * tid) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4 *>(sh->offset + 4 * tid) = make_uint4(0, 0, 0, 0);
+    if (tid < GROUPS) sh->elements[tid] = 0;
     __syncthreads();
-    uint64_t mine = 0, before;
     const bool whole = cut.value == -INFINITY;
-    row.words_from(cut.value, [&](const uint4 &v, int w) {
-        float x[N];
-        Type<T>::load(v, x);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const bool in = whole || row.kept(cut, x[e], w, e);
-            mine += weigh.biased(x[e], in);
-            if (in && x[e] >= low) atomicAdd(&count[bin_of(x[e])], 1u);
-        }
-        mine -= N * Weigher::BIAS;
-    });
+    uint64_t mine = whole ? sum_and_count<true>(row, weigh, cut, top, low, c, count) : sum_and_count<false>(row, weigh, cut, top, low, c, count);
     __syncthreads();
     {
-        const uint4 n = *reinterpret_cast<const uint4 *>(count + 4 * tid);
-        uint64_t s = 0;
-        if (n.x | n.y | n.z | n.w)
-            s = n.x * middle(4 * tid) + n.y * middle(4 * tid + 1) + n.z * middle(4 * tid + 2) + n.w * middle(4 * tid + 3);
-        uint32_t k = n.x + n.y + n.z + n.w;
+        const uint4 n4 = *reinterpret_cast<const uint4 *>(count + 4 * tid), o4 = *reinterpret_cast<const uint4 *>(sh->offset + 4 * tid);
+        const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w}, o[4] = {o4.x, o4.y, o4.z, o4.w};
+        uint64_t w[4];
+        estimate(n, o, 4 * tid, w);
+        uint64_t s = w[0] + w[1] + w[2] + w[3];
+        uint32_t k = n[0] + n[1] + n[2] + n[3];
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), k += __shfl_xor_sync(0xffffffffu, k, o);
         if ((tid & 15) == 0) group[tid >> 4] = s, group_count[tid >> 4] = k;
     }
-    const uint64_t sum = row.total(mine, before);
+    sum = row.total(mine, before);
     const double target = ceil((double)sum * p);
     need = target >= 1.0 ? min(sum, (uint64_t)target) : 1ull;
     // the border is in bin `first` or after it, and before bin `end`
     int first = 0, end = BINS;
     uint64_t seek = need;  // in sums of the estimate
+    const double sure = exp2(-1.01 * width * weigh.rate / 16.0) * (1.0 - 1e-6);
     for (;;) {
+        // a warp for each CTA reads its groups, then its bins around the group of the border
+        const uint32_t of = (uint32_t)warp < row.ctas ? warp : 0;
+        sh->near_group[warp][lane] = ld_cluster_u64(&group[lane], of);
+        const uint32_t counted = ld_cluster_u32(&group_count[lane], of);
+        if ((uint32_t)warp < row.ctas) atomicAdd(&sh->elements[lane], counted);
+        __syncthreads();
         if (warp == 0) {
-            const uint64_t s = sum_u64(&group[lane], row.ctas);
-            const uint32_t k = sum_u32(&group_count[lane], row.ctas);
-            uint64_t upto = warp_scan(s);
-            const uint32_t elements = (uint32_t)warp_scan((uint64_t)k);
-            // up to which group the weights reach `need` for certain: none is less than the middle's by more than half a bin
-            const double sure = exp2(-0.51 * width * weigh.rate / 16.0) * (1.0 - 1e-6);
+            uint64_t s = 0;
+            for (uint32_t k = 0; k < row.ctas; ++k) s += sh->near_group[k][lane];
+            const uint64_t upto = warp_scan(s);
+            const unsigned past = __ballot_sync(0xffffffffu, upto >= seek);
+            const int g = past ? __ffs(past) - 1 : GROUPS - 1;
+            // up to which group the weights reach `need` for certain: a bin's elements are no wider apart than it
             const unsigned reached = __ballot_sync(0xffffffffu, (double)upto * sure >= (double)need);
             const int last = reached ? __ffs(reached) - 1 : 0;
-            const uint32_t all = __shfl_sync(0xffffffffu, elements, last);
-            if (first == 0 && end == BINS && reached && all <= LIST) {
+            const uint32_t all = __reduce_add_sync(0xffffffffu, lane <= last ? sh->elements[lane] : 0u);
+            if (lane == g) sh->found_before = upto - s, sh->found_first = g;
+            if (lane == 0) sh->found_count = first == 0 && end == BINS && reached && all <= LIST ? all : NO_INDEX, sh->found_last = last;
+        }
+        __syncthreads();
+        const uint64_t start = sh->found_before;  // before the border's group
+        const int g = sh->found_first, last = sh->found_last, near0 = min(max(g * GROUP - NEAR / 4, 0), BINS - NEAR);
+        const bool listable = sh->found_count != NO_INDEX;
+        const uint32_t all = sh->found_count;
+        __syncthreads();
+        if (warp == 0) sh->elements[lane] = 0;  // (for another round)
+        if (!listable) {
+            // (16 CTAs: two to a row)
+            uint32_t v[2 * NEAR / 32];
+#pragma unroll
+            for (int q = 0; q < NEAR / 32; ++q) {
+                v[q] = ld_cluster_u32(count + near0 + q * 32 + lane, of);
+                v[NEAR / 32 + q] = ld_cluster_u32(sh->offset + near0 + q * 32 + lane, of);
+            }
+            uint32_t *row_of = sh->near_bins[warp & 7];
+            if (warp < 8)
+#pragma unroll
+                for (int q = 0; q < 2 * NEAR / 32; ++q) row_of[q * 32 + lane] = v[q];
+            __syncthreads();
+            if (warp >= 8 && (uint32_t)warp < row.ctas)
+#pragma unroll
+                for (int q = 0; q < 2 * NEAR / 32; ++q) row_of[q * 32 + lane] += v[q];
+        }
+        __syncthreads();
+        if (warp == 0) {
+            if (listable) {
                 if (lane == 0) sh->found_bin = last * GROUP + GROUP - 1, sh->found_count = all;
             } else {
-                const unsigned past = __ballot_sync(0xffffffffu, upto >= seek);
-                const int g = past ? __ffs(past) - 1 : GROUPS - 1;
-                const uint64_t start = __shfl_sync(0xffffffffu, upto - s, g);  // before the group
-                const int i = g * GROUP + 2 * lane;
-                const uint32_t a = sum_u32(&count[i], row.ctas), b = sum_u32(&count[i + 1], row.ctas);
-                const uint64_t wa = a ? a * middle(i) : 0ull, wb = b ? b * middle(i + 1) : 0ull;
-                upto = start + warp_scan(wa + wb);
-                const unsigned here = __ballot_sync(0xffffffffu, upto >= seek);
-                int bin = BINS - 1;
-                if (here) {
-                    const int l = __ffs(here) - 1;
-                    bin = g * GROUP + 2 * l + (__shfl_sync(0xffffffffu, upto - wb >= seek ? 1 : 0, l) ? 0 : 1);
+                // four bins a lane
+                uint32_t n[4], o[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) n[q] = o[q] = 0;
+                for (uint32_t k = 0; k < min(row.ctas, 8u); ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) n[q] += sh->near_bins[k][4 * lane + q], o[q] += sh->near_bins[k][NEAR + 4 * lane + q];
+                uint64_t w[4];
+                estimate(n, o, near0 + 4 * lane, w);
+                const uint64_t mine4 = w[0] + w[1] + w[2] + w[3];
+                // sums from near0 on; what lies before the group's start among them
+                const uint64_t scan = warp_scan(mine4);
+                const int lane_of_group = (g * GROUP - near0) / 4;
+                const uint64_t head = lane_of_group ? __shfl_sync(0xffffffffu, scan, lane_of_group - 1) : 0ull;
+                const uint64_t base = start - head;  // the estimate before near0
+                uint64_t run = base + scan - mine4;
+                int my_bin = BINS;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    run += w[q];
+                    if (run >= seek && my_bin == BINS) my_bin = near0 + 4 * lane + q;
                 }
-                if (bin < first || bin >= end) bin = (first + end) / 2;  // (the estimate has not come closer)
-                // the bins around it that fit the list: 2^n to either side
-                const int at = bin - 16 + lane;
-                const uint32_t n = at >= first && at < end ? sum_u32(&count[at], row.ctas) : 0u;
-                uint32_t m = __reduce_add_sync(0xffffffffu, n);
-                int side = 16;
-                while (m > LIST && side > 0) {
-                    side >>= 1;
-                    m = __reduce_add_sync(0xffffffffu, lane >= 16 - side && lane <= 16 + side ? n : 0u);
+                int bin = (int)__reduce_min_sync(0xffffffffu, (unsigned)my_bin);
+                if (bin == BINS) bin = BINS - 1;
+                const bool lost = bin < first || bin >= end || bin < near0 || bin >= near0 + NEAR;  // (the estimate has not come closer)
+                if (bin < first || bin >= end) bin = (first + end) / 2;
+                // the lanes (of four bins) around it that fit the window, else its bin alone
+                int b0 = bin, b1 = bin;
+                uint32_t m = 0;
+                uint64_t est = 0;
+                if (lost) m = sum_u32(&count[bin], row.ctas);
+                else {
+                    const int l = (bin - near0) / 4;
+                    const uint32_t four = n[0] + n[1] + n[2] + n[3];
+                    int side = 16;
+                    for (;;) {
+                        m = __reduce_add_sync(0xffffffffu, lane >= l - side && lane <= l + side ? four : 0u);
+                        if (m <= WINDOW || side == 0) break;
+                        side >>= 1;
+                    }
+                    if (m <= WINDOW) {
+                        b0 = max(near0 + 4 * max(l - side, 0), first);
+                        b1 = min(near0 + 4 * min(l + side, 31) + 3, end - 1);
+                    }
+                    m = 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int at = near0 + 4 * lane + q;
+                        m += at >= b0 && at <= b1 ? n[q] : 0u;
+                        est += at < b0 ? w[q] : 0ull;
+                    }
+                    m = __reduce_add_sync(0xffffffffu, m);
+                    est = base + warp_sum(est);
                 }
-                const int b0 = max(bin - side, first), b1 = min(bin + min(side, 15), end - 1);
-                // the estimate of what is before the first of them, from the start of the group
-                uint64_t est = start + warp_sum((i < b0 ? wa : 0ull) + (i + 1 < b0 ? wb : 0ull));
-                if (b0 < g * GROUP) est = start - warp_sum(at >= b0 && at < g * GROUP && n ? n * middle(at) : 0ull);
                 if (lane == 0) {
                     sh->found_bin = NO_INDEX;
                     sh->found_count = m;
@@ -750,31 +997,36 @@ __device__ __forceinline__ bool nucleus(Row<T, CLUSTER> &row, const Weigher &wei
         const uint64_t est = sh->found_estimate;
         __syncthreads();
         if (through != NO_INDEX) {
-            listed = row.collect(1, low, [&](float x, int w, int e) { return x >= low && bin_of(x) <= (int)through && row.kept(cut, x, w, e); });
-            return true;
+            listed = row.collect(1, low, [&](float x, int w, int e) { return x >= low && bin_at(bins_below(top, x, c)) <= BIN0 + (float)through && row.kept(cut, x, w, e); });
+            return LISTED;
         }
         if (n > LIST) {  // a bin of many elements, likely equal ones
             Row<T, CLUSTER> other = row;
             cut = select<true>(other, weigh, cut, key_of<UNIT>(top), key_of<UNIT>(low), need);
-            row.turn = other.turn;
-            return false;
+            row.turn = other.turn, row.sums = other.sums;
+            return CUT;
         }
-        mine = 0;
         if (tid == 0) sh->list_count[1] = 0;
         __syncthreads();
-        row.each_from(low, [&](float x, int w, int e) {
-            const int b = bin_of(x);
-            const bool in = x >= low && b <= b1 && (whole || row.kept(cut, x, w, e));
-            mine += weigh(x, in && b < b0);
-            if (in && b >= b0) row.append(1, x, w, e);
-        });
+        mine = whole ? sum_and_list<true>(row, weigh, cut, top, low, c, BIN0 + b0, BIN0 + b1) : sum_and_list<false>(row, weigh, cut, top, low, c, BIN0 + b0, BIN0 + b1);
+        __syncthreads();
+        if (warp == 0) row.tell(sh->listed_of[1], sh->list_count[1]);
         const uint64_t above = row.total(mine, before);
+        uint64_t place, own;
         if (above >= need) end = b0;
-        else if (row.resolve(1, n, need - above, [&](float x) { return weigh(x); })) {
+        else if (row.resolve(1, n, need - above, [&](float x) { return weight_of(weigh, x, 0.0); }, place, own)) {
             cut = sh->cut;
-            return false;
+            // what the list adds to the sums before this CTA, of its warps, of all
+            const uint32_t ix = ~(uint32_t)place;
+            if (place < place_of(key_of<UNIT>(cut.value), cut.index)) own = 0;
+            sum = above + row.block_sum(own, 0);
+            before += row.block_sum(ix < row.base ? own : 0ull, 1);
+            if (own && ix >= row.base && ix - row.base < (uint32_t)row.tokens)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&sh->warp_sum[(ix - row.base + row.skew) / N / row.per]), own);
+            __syncthreads();
+            return CUT_AND_SUM;
         } else first = b1 + 1;
-        if (first >= end) return false;  // all of them together do not reach it
+        if (first >= end) return CUT;  // all of them together do not reach it
         seek = need + est - above;
         sync_all<CLUSTER>();  // the lists are filled again
     }
@@ -787,13 +1039,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared *sh = reinterpret_cast<Shared *>(smem);
     pdl_trigger();
+    if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_wait();
     Row<T, CLUSTER> row;
     row.sh = sh;
     row.data = reinterpret_cast<uint4 *>(smem + (sizeof(Shared) + 15) / 16 * 16);
     row.ctas = CLUSTER ? gridDim.x : 1;
     row.rank = CLUSTER ? blockIdx.x : 0;
-    row.slot = &sh->cta_sum[0];
+    row.sums = 0;
     row.turn = 0;
     const int64_t b = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -810,7 +1063,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(row.data + w)), "l"(src + at) : "memory");
         } else {
             T *dst = reinterpret_cast<T *>(row.data + w);
-#pragma unroll
+#pragma unroll 1
             for (int e = 0; e < N; ++e) {
                 if (at + e >= 0 && at + e < n) dst[e] = src[at + e];
                 else dst[e] = T(-INFINITY);
@@ -822,12 +1075,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const double min_p = p.min_p ? (double)p.min_p[b] : p.min_p_all;
     const int64_t top_k = p.top_k ? (int64_t)p.top_k[b] : p.top_k_all;
     const float u = p.u[b];
+    // (what takes divisions and functions of fp64, under the copies)
+    Weigher weigh(temperature, p.scale, sh->table);
+    const double least = fmin(fmax(min_p, 0.0), 1.0) * exp2((double)p.scale);
+    const double reach = top_p < 1.0 ? reach_of(weigh, top_p, p.V) : 0.0;
     if (tid < 16) sh->table[tid] = exp2(-tid / 16.0);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    const int per = (words + THREADS - 1) / THREADS * 32;
-    row.first = min(words, warp * per);
-    row.last = min(words, row.first + per);
+    row.tokens = n;
+    row.per = (words + THREADS - 1) / THREADS * 32;
+    row.first = min(words, warp * row.per);
+    row.last = min(words, row.first + row.per);
 
     // ---- the largest logit
     float largest = -INFINITY, smallest = INFINITY;  // of the words' largest; of those above -inf
@@ -842,10 +1100,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     top = __reduce_max_sync(0xffffffffu, lane < WARPS ? sh->warp_max[lane] : 0u);
     bottom = __reduce_min_sync(0xffffffffu, lane < WARPS ? sh->warp_min[lane] : NO_INDEX);
     if (CLUSTER) {
-        if (tid == 0) sh->cta_max = top, sh->cta_min = bottom;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
+        if (warp == 0) row.tell(sh->max_of, top), row.tell(sh->min_of, bottom);
         cluster_sync_all();
-        top = __reduce_max_sync(0xffffffffu, lane < row.ctas ? ld_cluster_u32(&sh->cta_max, lane) : 0u);
-        bottom = __reduce_min_sync(0xffffffffu, lane < row.ctas ? ld_cluster_u32(&sh->cta_min, lane) : NO_INDEX);
+        top = __reduce_max_sync(0xffffffffu, lane < row.ctas ? sh->max_of[lane] : 0u);
+        bottom = __reduce_min_sync(0xffffffffu, lane < row.ctas ? sh->min_of[lane] : NO_INDEX);
     }
     const uint32_t none = key_of<UNIT>(-INFINITY);
     int64_t token = -1;
@@ -862,11 +1121,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             if (x == value) at = min(at, row.index(w, e));
         });
         at = __reduce_min_sync(0xffffffffu, at);
-        if (tid == 0) sh->cta_first = NO_INDEX;
+        if (tid == 0) sh->first = NO_INDEX;
         __syncthreads();
-        if (lane == 0) atomicMin(&sh->cta_first, at);
+        if (lane == 0) atomicMin(&sh->first, at);
+        __syncthreads();
+        if (warp == 0) row.tell(sh->first_of, sh->first);
         sync_all<CLUSTER>();
-        at = __reduce_min_sync(0xffffffffu, lane < row.ctas ? ld_cluster_u32(&sh->cta_first, lane) : NO_INDEX);
+        at = __reduce_min_sync(0xffffffffu, lane < row.ctas ? sh->first_of[lane] : NO_INDEX);
         token = at;
         logprob = 0.f;
     } else {
@@ -874,20 +1135,20 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             // infinite logits share everything: they are 0 in the slice from here on, the others -inf
             for (int w = row.first + lane; w < row.last; w += 32) {
                 T *x = reinterpret_cast<T *>(row.data + w);
-#pragma unroll
+#pragma unroll 1
                 for (int e = 0; e < N; ++e) x[e] = (float)x[e] == INFINITY ? T(0.f) : T(-INFINITY);
             }
             __syncwarp();
             top = bottom = key_of<UNIT>(0.f);
         }
         const float peak = value_of<UNIT>(top);
-        const Weigher weigh(peak, temperature, p.scale, sh->table);
-        const double least = fmin(fmax(min_p, 0.0), 1.0) * exp2((double)p.scale);
+        weigh.max = widen(peak);
         Cut cut{-INFINITY, NO_INDEX};
         // whether all that may be drawn is in the list, its length, which counter, and what is left to do with it
         bool in_list = false;
         uint32_t listed = 0;
-        uint64_t k = 0, need = 0, before;
+        uint64_t k = 0, need = 0, before = 0, sum = 0;
+        bool summed = false;  // whether sum, before and warp_sum[] are those of the kept
         if (top_k > 0 && top_k < p.V) {
             const float low = top_k <= p.V / N ? bound_of_largest(row, peak, value_of<UNIT>(bottom), (uint64_t)top_k) : -INFINITY;
             if (top_k <= LIST && low > -INFINITY) {
@@ -898,60 +1159,31 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             if (!in_list) {
                 Row<T, CLUSTER> other = row;
                 cut = select<false>(other, weigh, cut, top, low > -INFINITY ? max(none + 1, key_of<UNIT>(low)) : none + 1, (uint64_t)top_k);
-                row.turn = other.turn;
+                row.turn = other.turn, row.sums = other.sums;
                 k = 0;
             }
         }
-        if (!in_list && top_p < 1.0) in_list = nucleus(row, weigh, cut, peak, top_p, p.V, need, listed);
+        if (!in_list && top_p < 1.0) {
+            const Outcome o = nucleus(row, weigh, cut, peak, top_p, reach, need, listed, sum, before);
+            in_list = o == LISTED;
+            summed = o == CUT_AND_SUM && least == 0.0;
+        }
         writer = false;
         if (in_list) {
             if (row.rank == 0)
                 finish(row, weigh, k ? 0 : 1, listed, k, top_p, need, least, (double)u, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
         } else {
             // ---- the kept ones' sum, and the place of u in it
-            auto weight_kept = [&](float x, int w, int e) { return weigh.at_least(x, row.kept(cut, x, w, e), least); };
-            uint64_t mine = 0;
-            const bool plain = cut.value == -INFINITY && least == 0.0;
-            row.words_from(cut.value, [&](const uint4 &v, int w) {
-                float x[N];
-                Ty::load(v, x);
-                if (plain) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) mine += weigh.biased(x[e], true);
-                    mine -= N * Weigher::BIAS;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) mine += weight_kept(x[e], w, e);
-                }
-            });
-            const uint64_t sum = row.total(mine, before);
+            if (!summed) {
+                const uint64_t mine = cut.value == -INFINITY && least == 0.0 ? sum_kept<true>(row, weigh, cut, 0.0) : sum_kept<false>(row, weigh, cut, least);
+                sum = row.total(mine, before);
+            }
             const double place = fmax((double)u, 0.0) * (double)sum;
             const uint64_t target = place < (double)sum ? min((uint64_t)place, sum - 1) : sum - 1;
             uint64_t at = before;
             for (int i = 0; i < warp; ++i) at += sh->warp_sum[i];
-            if (at <= target && target < at + sh->warp_sum[warp]) {
-                row.words_from(cut.value, [&](const uint4 &v, int w) {
-                    float x[N];
-                    Ty::load(v, x);
-                    uint64_t own[N], mine = 0;
-#pragma unroll
-                    for (int e = 0; e < N; ++e) mine += own[e] = weight_kept(x[e], w, e);
-                    const uint64_t upto = at + warp_scan(mine);
-                    if (upto > target && upto - mine <= target) {
-                        uint64_t run = upto - mine;
-#pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            if (run <= target && target < run + own[e]) {
-                                token = row.index(w, e);
-                                logprob = weigh.logprob(x[e], sum);
-                                writer = true;
-                            }
-                            run += own[e];
-                        }
-                    }
-                    at = __shfl_sync(0xffffffffu, upto, 31);
-                });
-            }
+            if (at <= target && target < at + sh->warp_sum[warp])
+                draw(row, weigh, cut, least, at, target, sum, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
         }
     }
     if (writer) {
@@ -967,8 +1199,10 @@ static int launch(const Params &q, int64_t B, cudaStream_t st) {
     Params p = q;
     const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T);
     int ctas = MAX_CTAS;
-    while (ctas > 1 && B * ctas >= 8 * 148 && bytes * 2 / ctas <= (64 << 10)) ctas /= 2;
-    while (ctas > 1 && bytes / ctas < 2048) ctas /= 2;
+    // CTAs of a row: 16 where that leaves SMs idle.  More rows than that: fewer and longer slices, up to 80 KB (two CTAs of
+    // 64 KB an SM; 256 rows of 256 KB without filter in 4 CTAs 90 us, in 8 130, in 2 128; 96 rows of 607 KB in 8 67, in 16
+    // 92).  Short rows: 4 KB at least.
+    while (ctas > 1 && (B * ctas > 148 || bytes / ctas < 4096) && bytes * 2 / ctas <= (80 << 10)) ctas /= 2;
     p.slice = ((p.V + ctas - 1) / ctas + 15) / 16 * 16;
     const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)p.slice * sizeof(T) + 32;
     auto kernel = ctas > 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
@@ -978,6 +1212,7 @@ static int launch(const Params &q, int64_t B, cudaStream_t st) {
         const int most = (int)((sizeof(Shared) + 15) / 16 * 16 + MAX_SLICE + 32);
         QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured.set(dev);
     }
     const unsigned gy = (unsigned)(B < 32768 ? B : 32768);
@@ -1000,7 +1235,7 @@ static int launch(const Params &q, int64_t B, cudaStream_t st) {
 }  // namespace samplek
 
 // bytes of one row's logits that a call can take
-int64_t sample_row_limit() { return (int64_t)samplek::MAX_CTAS * samplek::MAX_SLICE - 16 * 4 * samplek::MAX_CTAS; }
+int64_t sample_row_limit() { return (int64_t)8 * samplek::MAX_SLICE - 16 * 4 * 8; }
 
 int launch_sample(const samplek::Params &p, int dtype, int64_t B, cudaStream_t st) {
     using namespace samplek;

@@ -114,6 +114,14 @@ def test_batches_with_settings_of_their_own(rows, V):
     assert torch.equal(qlinear.sample(x[one:one + 1], u[one:one + 1], **{k: v[one:one + 1] for k, v in own.items()}), whole[one:one + 1])
 
 
+@pytest.mark.parametrize("settings", [dict(top_p=0.9, temperature=1.3), dict(top_p=0.98), dict(top_k=3000, top_p=0.8), dict(top_k=400)], ids=str)
+def test_many_rows_of_distinct_logits(settings):
+    """Every logit its own value: some lie on the borders of whatever the rows are divided by on the way."""
+    g = gen(60)
+    x = torch.randn(300, 60001, generator=g, device="cuda") * 2
+    check(x, torch.rand(300, generator=g, device="cuda"), **settings)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("V", [64, 1000, 16384, 100000])
 def test_equal_logits(dtype, V):
