@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     uint64_t *drain = ofull + 2;       // [2] an aborted tile's MMAs are done
     uint64_t *turn = drain + 2;        // [2] the other tile's exponentials of the step are done
     uint64_t *sread = turn + 2;        // [2] S_t of the step is in registers (P_APART)
-    uint64_t *vfix = sread + 2;        // [3] V of the window's first / the last / the sinks' last step cleared where no row sees it
+    uint64_t *vfix = sread + 2;        // [3] V of the last step of the gap before the window / of the last / of the gap's other step cleared where no row sees it
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfix + 3);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -150,7 +150,6 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
     int vlo, vhi, unused;
     visible(p, s, row0 / p.G, vlo, unused);
     visible(p, s, (row0 + nrows - 1) / p.G, unused, vhi);
-    const int lead = SINKS ? lead_steps(p, split, vlo, vhi, TKV) : 0;
     take_split(p, split, p.chunk, vlo, vhi);
     if (vhi <= vlo) {  // nothing to see: no partial result, or zeros
         for (int idx = threadIdx.x; idx < nrows; idx += SM100_THREADS) {
@@ -162,11 +161,27 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
         }
         return;
     }
-    // steps: `lead` of the sinks below the window, then the window's from tile t0 on
-    const int t0 = vlo / TKV, n = lead + (vhi + TKV - 1) / TKV - t0;
-    auto step_at = [&](int j) { return (SINKS ? (j < lead ? j : t0 + j - lead) : t0 + j) * TKV; };  // first position
-    const bool fix_first = vlo > (SINKS ? max(t0 * TKV, p.sinks) : t0 * TKV), fix_last = vhi < (t0 + n - lead) * TKV;
-    const bool fix_lead = SINKS && p.sinks < lead * TKV;
+    // The steps go over places.  Without sinks a place is its position; with SINKS, first come the sinks in whole
+    // blocks of 16 (`lead` of them; by the first split, and only if the window begins behind them), then
+    // the window's positions from its block of 16 on, each `shift` lower than its place.
+    [[maybe_unused]] int lead = 0, shift = 0, sunk = 0, gap0 = 0, gap = 0;  // (places below `sunk` are sinks)
+    [[maybe_unused]] bool fix_lead = false;
+    if constexpr (SINKS) {
+        int origin = vlo & ~15;
+        if (split == 0) {
+            if (p.sinks < origin) lead = (p.sinks + 15) & ~15;
+            else origin = 0;
+        }
+        shift = lead - origin;
+        sunk = lead ? p.sinks : p.sinks - origin;
+        vlo += shift, vhi += shift;
+        // the places up to the window that no row sees lie in one step or in two
+        gap0 = max(sunk, 0) / TKV, gap = (vlo - 1) / TKV;
+        fix_lead = sunk < vlo && gap0 < gap;
+    }
+    const int t0 = SINKS ? 0 : vlo / TKV, n = (vhi + TKV - 1) / TKV - t0;
+    const bool fix_first = vlo > (SINKS ? max(sunk, 0) : t0 * TKV), fix_last = vhi < (t0 + n) * TKV;
+    const int jf = SINKS && fix_first ? gap : 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -232,6 +247,7 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             // a step inside [max_lo, min_hi) is seen whole by every row of the tile
             visible(p, s, (row0 + t * TQ) / p.G, unused, min_hi);
             visible(p, s, min(rows - 1, row0 + t * TQ + TQ - 1) / p.G, max_lo, unused);
+            if constexpr (SINKS) min_hi += shift, max_lo += shift, rlo += shift, rhi += shift;
             min_hi = min(min_hi, vhi);
             max_lo = max(max_lo, vlo);
             rlo = max(rlo, vlo);
@@ -261,13 +277,13 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sread[t]);
                 }
-                const int kv0 = step_at(j);
+                const int kv0 = (t0 + j) * TKV;
                 // a step that some row of the tile does not see whole (the same for all its threads)
                 if (kv0 < max_lo || kv0 + TKV > min_hi) {
 #pragma unroll
                     for (int w = 0; w < TKV / 32; ++w) {  // one bit per position: two instructions a score
                         uint32_t see = bits_below(rhi - kv0 - w * 32) & ~bits_below(rlo - kv0 - w * 32);
-                        if constexpr (SINKS) see |= bits_below(min(rhi, p.sinks) - kv0 - w * 32);
+                        if constexpr (SINKS) see |= bits_below(min(rhi, sunk) - kv0 - w * 32);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) sc[w * 32 + i] = (see & (1u << i)) ? sc[w * 32 + i] : NEG_INF;
                     }
@@ -393,16 +409,16 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
         const unsigned inject = *reinterpret_cast<volatile unsigned *>(&g_debug_inject);
         if (!(inject & 2u)) {
             const int loads = inject & 4u ? n : 2 * n;  // of K and V, one each a step (n: the test hook's half)
-            const int ps = 1 << p.page_shift, box = min(ps, TKV), nb = TKV / box;
+            const int ps = 1 << p.page_shift, box = SINKS ? 16 : min(ps, TKV), nb = TKV / box;
             // clears what no row sees in V of step j, once it has landed; only this warp refills
             // the stage, so its barrier still stands at that load
             auto clear_v = [&](int j, uint64_t *done) {
-                const int it = 2 * j + 1, st = it % STAGES, kv0 = step_at(j);
+                const int it = 2 * j + 1, st = it % STAGES, kv0 = (t0 + j) * TKV;
                 if (!__all_sync(0xffffffffu, mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, DEV_ERR_TIMEOUT_FULL))) return;
                 uint8_t *vs = smem + C::SMEM_KV + st * C::TILE_BYTES;
                 for (int idx = lane; idx < TKV * 8; idx += 32) {
                     const int row = idx >> 3;
-                    if ((kv0 + row >= vlo || (SINKS && kv0 + row < p.sinks)) && kv0 + row < vhi) continue;
+                    if ((kv0 + row >= vlo || (SINKS && kv0 + row < sunk)) && kv0 + row < vhi) continue;
 #pragma unroll
                     for (int h = 0; h < C::HALVES; ++h)
                         *reinterpret_cast<uint4 *>(vs + h * C::HALF_BYTES + row * 128 + (idx & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -413,20 +429,22 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
             };
             // this lane's page of step j, where there is something to see; indices are fetched four
             // steps ahead
-            auto wanted = [&](int pos) { return lane < nb && pos < vhi && (pos + box > vlo || (SINKS && pos < p.sinks)); };
+            // places and their positions
+            auto wanted = [&](int v) { return lane < nb && v < vhi && (v + box > vlo || (SINKS && v < sunk)); };
+            auto position = [&](int v) { return SINKS && v >= lead ? v - shift : v; };
             auto page_index = [&](int j) {
-                const int pos = step_at(j) + lane * box;
-                return j < n && wanted(pos) ? p.table[b * p.table_stride + (pos >> p.page_shift)] : 0;
+                const int v = (t0 + j) * TKV + lane * box;
+                return j < n && wanted(v) ? p.table[b * p.table_stride + (position(v) >> p.page_shift)] : 0;
             };
             int it = 0, page = 0, ahead[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) ahead[j] = page_index(j);
             for (; it < loads; ++it) {
                 // V of step j is cleared before the load that waits for its products
-                if (SINKS && fix_lead && it == min(2 * (lead - 1) + STAGES, 2 * n - 1)) clear_v(lead - 1, &vfix[2]);
-                if (it == min(2 * lead + STAGES, 2 * n - 1) && fix_first && lead < n - 1) clear_v(lead, &vfix[0]);
-                const int st = it % STAGES, pos = step_at(it >> 1) + lane * box;
-                const bool in = wanted(pos);
+                if (SINKS && fix_lead && it == min(2 * gap0 + STAGES, 2 * n - 1)) clear_v(gap0, &vfix[2]);
+                if (it == min(2 * jf + STAGES, 2 * n - 1) && fix_first && jf < n - 1) clear_v(jf, &vfix[0]);
+                const int st = it % STAGES, place = (t0 + (it >> 1)) * TKV + lane * box, pos = position(place);
+                const bool in = wanted(place);
                 if (!(it & 1)) {
                     page = ahead[0], ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
                     ahead[3] = page_index((it >> 1) + 4);
@@ -450,8 +468,8 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
             }
             if (it == 2 * n) {
-                if (lead == n - 1 && (fix_first || fix_last)) clear_v(lead, &vfix[0]);
-                if (fix_last && lead < n - 1) clear_v(n - 1, &vfix[1]);
+                if (jf == n - 1 && (fix_first || fix_last)) clear_v(jf, &vfix[0]);
+                if (fix_last && jf < n - 1) clear_v(n - 1, &vfix[1]);
             }
             // after an abort, whichever wait ran out, the copies land before their memory is given up
             roles_done();
@@ -497,9 +515,9 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
                 }
                 const int it = 2 * j + 1, st = it % STAGES;
                 ok = mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, DEV_ERR_TIMEOUT_FULL);
-                if (SINKS && ok && fix_lead && j == lead - 1) ok = mbar_wait(&vfix[2], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
-                if (ok && j == lead && (fix_first || (lead == n - 1 && fix_last))) ok = mbar_wait(&vfix[0], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
-                if (ok && j > lead && j == n - 1 && fix_last) ok = mbar_wait(&vfix[1], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (SINKS && ok && fix_lead && j == gap0) ok = mbar_wait(&vfix[2], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (ok && j == jf && (fix_first || (jf == n - 1 && fix_last))) ok = mbar_wait(&vfix[0], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
+                if (ok && j > jf && j == n - 1 && fix_last) ok = mbar_wait(&vfix[1], 0, abort_flag, DEV_ERR_TIMEOUT_FULL);
                 const uint32_t vs = ring + st * C::TILE_BYTES;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -534,15 +552,15 @@ __global__ void __launch_bounds__(SM100_THREADS, 1)
 }
 
 // keys or values of one layer as [pages][heads][page][D]; a box is the rows of one page that
-// fall in a step, 64 elements wide
+// fall in a step (up to `rows`), 64 elements wide
 template <typename T>
-static int cache_map(CUtensorMap *map, const void *base, const Params &p, int D) {
+static int cache_map(CUtensorMap *map, const void *base, const Params &p, int D, int rows) {
     gemm::PFN_encodeTiled enc = gemm::get_encode();
     if (!enc) return fail(QL_ECUDA, "cuTensorMapEncodeTiled unavailable");
     const uint64_t ps = 1ull << p.page_shift;
     cuuint64_t dims[4] = {(cuuint64_t)D, ps, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
     cuuint64_t strides[3] = {(cuuint64_t)D * 2, ps * D * 2, (cuuint64_t)p.page_stride * 2};
-    cuuint32_t box[4] = {64, (cuuint32_t)(ps < TKV ? ps : TKV), 1, 1}, es[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)(ps < rows ? ps : rows), 1, 1}, es[4] = {1, 1, 1, 1};
     const CUresult r =
         enc(map, __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
             const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -560,8 +578,9 @@ static int launch_sm100_s(const Params &p, int64_t B, cudaStream_t st) {
         configured.set(dev);
     }
     CUtensorMap mk, mv;
-    if (int rc = cache_map<T>(&mk, p.k_cache, p, D)) return rc;
-    if (int rc = cache_map<T>(&mv, p.v_cache, p, D)) return rc;
+    const int rows = SINKS ? 16 : TKV;  // the sinks and the window begin at any block of 16
+    if (int rc = cache_map<T>(&mk, p.k_cache, p, D, rows)) return rc;
+    if (int rc = cache_map<T>(&mv, p.v_cache, p, D, rows)) return rc;
     const int tiles = (int)(((int64_t)p.max_q * p.G + SM100_ROWS - 1) / SM100_ROWS);
     QL_CUDA_TRY(launch_pdl(sm100_kernel<T, D, SINKS>, dim3(p.Hkv * p.nsplit, tiles, (unsigned)B), dim3(SM100_THREADS), C::SMEM, st, 1,
                            mk, mv, p));

@@ -301,9 +301,16 @@ const int32_t *counts(const at::Tensor &t, const char *name, int64_t n, c10::Dev
           t.scalar_type(), " on ", t.device());
     return t.const_data_ptr<int32_t>();
 }
-// An output of plan_step: entry i of `out`, or a new tensor.
-at::Tensor result(PyObject *out, int i, const char *name, int64_t n, at::ScalarType type, c10::Device dev) {
-    if (out == Py_None) return fresh({n}, type, dev);
+// A vector of n entries in `whole`'s memory from byte `at` on (a multiple of the entry's size).
+at::Tensor part(const at::Tensor &whole, int64_t at, int64_t n, at::ScalarType type) {
+    const auto meta = c10::scalarTypeToTypeMeta(type);
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), meta);
+    t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)meta.itemsize());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+}
+// An output of plan_step: entry i of `out`, which was given.
+at::Tensor given(PyObject *out, int i, const char *name, int64_t n, at::ScalarType type, c10::Device dev) {
     const at::Tensor &t = tensor(PyTuple_GET_ITEM(out, i), name);
     VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous() && t.device() == dev, "out's ", name,
           " must be a contiguous ", type, " vector of ", n, " on ", dev, ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
@@ -333,10 +340,17 @@ PyObject *plan_step(PyObject *const *a) {
     }
     TYPE(a[7] == Py_None || (PyTuple_Check(a[7]) && PyTuple_GET_SIZE(a[7]) == 5), "out must be what a call returned: (positions, slots, q_starts, kv_lens, taken)");
     const c10::cuda::CUDAGuard guard(dev);
-    at::Tensor positions = result(a[7], 0, "positions", max_tokens, at::kLong, dev), slots = result(a[7], 1, "slots", max_tokens, at::kLong, dev);
-    at::Tensor starts = result(a[7], 2, "q_starts", B + 1, at::kInt, dev), lens = result(a[7], 3, "kv_lens", B, at::kInt, dev);
-    at::Tensor taken;
-    if (grows) taken = result(a[7], 4, "taken", 1, at::kInt, dev);
+    at::Tensor positions, slots, starts, lens, taken;
+    if (a[7] == Py_None) {  // five vectors in one allocation
+        const at::Tensor whole = fresh({16 * max_tokens + 4 * (2 * B + 2)}, at::kByte, dev);
+        positions = part(whole, 0, max_tokens, at::kLong), slots = part(whole, 8 * max_tokens, max_tokens, at::kLong);
+        starts = part(whole, 16 * max_tokens, B + 1, at::kInt), lens = part(whole, 16 * max_tokens + 4 * (B + 1), B, at::kInt);
+        if (grows) taken = part(whole, 16 * max_tokens + 4 * (2 * B + 1), 1, at::kInt);
+    } else {
+        positions = given(a[7], 0, "positions", max_tokens, at::kLong, dev), slots = given(a[7], 1, "slots", max_tokens, at::kLong, dev);
+        starts = given(a[7], 2, "q_starts", B + 1, at::kInt, dev), lens = given(a[7], 3, "kv_lens", B, at::kInt, dev);
+        if (grows) taken = given(a[7], 4, "taken", 1, at::kInt, dev);
+    }
     // (an empty free list has no address of its own)
     if (grows && !fp) fp = tp;
     check(p_plan_step(const_cast<int32_t *>(table.const_data_ptr<int32_t>()), B > 1 ? table.stride(0) : table.size(1), table.size(1), lp, np,

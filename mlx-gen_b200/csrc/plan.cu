@@ -10,8 +10,8 @@
 // CTA sums the counts of all sequences by itself (a thread has B / threads neighbours), then takes
 // tiles of one token a thread: each sequence marks its first token in the tile, and a token's
 // sequence is the last mark at or before it.  A page is entered in its table by the token
-// at its first position, which is always a new one.  Many tokens: a cluster of CTAs shares the
-// tiles; lengths and counts may be updated in place because all CTAs have read them (cluster
+// at its first position, which is always a new one.  Many tokens: a CTA for each tile.  Where lengths or the count
+// of taken pages are updated in place, a cluster of 8 shares the tiles instead, so that all CTAs have read them (cluster
 // barrier) before one writes them.
 #include "pdl.cuh"
 
@@ -42,12 +42,12 @@ struct Shared {
 };
 
 template <bool CLUSTER>
-__global__ void __launch_bounds__(MAX_THREADS) plan_kernel(const Params p) {
+__global__ void __launch_bounds__(MAX_THREADS) plan_kernel(const __grid_constant__ Params p) {
     __shared__ Shared sh;
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31, nw = nt >> 5;
-    const int rank = CLUSTER ? blockIdx.x : 0, ctas = CLUSTER ? gridDim.x : 1;
+    const int rank = blockIdx.x, ctas = gridDim.x;
     const int ps = 1 << p.page_shift;
     const int64_t per = (p.B + nt - 1) / nt, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     if (tid == 0) sh.bad = 0;
@@ -157,10 +157,13 @@ int launch_plan_step(const plank::Params &p, cudaStream_t st) {
     const int64_t most = p.B > p.max_tokens ? p.B : p.max_tokens;
     const int threads = most >= MAX_THREADS ? MAX_THREADS : most < 32 ? 32 : (int)((most + 31) / 32 * 32);
     int64_t ctas = (p.max_tokens + threads - 1) / threads;
-    ctas = ctas < 1 ? 1 : ctas < MAX_CTAS ? ctas : MAX_CTAS;
-    if (ctas > 1)
+    auto overlap = [](const int32_t *a, const int32_t *b, int64_t n) { return a < b + n && b < a + n; };
+    const bool in_place = overlap(p.kv_lens, p.lengths, p.B) || (p.free_pages && p.taken == p.taken_out);
+    const int64_t most_ctas = in_place ? MAX_CTAS : 8 * 148;  // (more tiles than that: several each)
+    ctas = ctas < 1 ? 1 : ctas < most_ctas ? ctas : most_ctas;
+    if (ctas > 1 && in_place)
         QL_CUDA_TRY(launch_pdl(plan_kernel<true>, dim3((unsigned)ctas), dim3(threads), 0, st, (unsigned)ctas, p));
-    else QL_CUDA_TRY(launch_pdl(plan_kernel<false>, dim3(1), dim3(threads), 0, st, 1, p));
+    else QL_CUDA_TRY(launch_pdl(plan_kernel<false>, dim3((unsigned)ctas), dim3(threads), 0, st, 1, p));
     return QL_OK;
 }
 
