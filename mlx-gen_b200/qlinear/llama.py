@@ -1,8 +1,8 @@
 """A Llama-shaped decoder on the quantized linears and the decoder operators: the prompt-refine
 path (Llama-3.2-3B: hidden 3072, 28 layers, 24 query and 8 key / value heads of 128, SwiGLU 8192) with
-chunked prompts, batched decoding, and continuations that share their prompt's pages.
+chunked prompts, batched decoding, sampling, and continuations that share their prompt's pages.
 
-    python -m qlinear.llama --layers 28 --prompt 700 --new 64 --forks 4
+    python -m qlinear.llama --layers 28 --prompt 700 --new 64 --forks 4 --temperature 0.7 --top-p 0.9 --graph
 
 runs it on random weights (no checkpoint is read here; ``qlinear.io`` loads packed ones) and prints
 the prompt's and the decode step's times.
@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import argparse
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
 import torch
 
@@ -38,6 +38,21 @@ class Config:
     eps: float = 1e-5
     bits: int = 4
     group_size: int = 64
+    window: int = 0  # positions that a token sees (0: all before it), and the first ones beside them
+    sinks: int = 0
+
+
+@dataclass
+class Sampling:
+    """How tokens are drawn (see ``decoder.sample``): numbers, or tensors with each sequence's own."""
+
+    temperature: Union[float, torch.Tensor] = 1.0
+    top_k: Union[int, torch.Tensor] = 0
+    top_p: Union[float, torch.Tensor] = 1.0
+    min_p: Union[float, torch.Tensor] = 0.0
+
+    def draw(self, logits: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+        return decoder.sample(logits, u, temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p)
 
 
 @dataclass
@@ -95,7 +110,8 @@ class Decoder:
             q, k, v = qkv.split([c.heads, c.kv_heads, c.kv_heads], 1)
             kc, vc = cache.layer(i)
             q = decoder.rope_append(q, k, v, self.table, step.positions, kc, vc, step.slots)
-            a = decoder.paged_attention(q, kc, vc, step.page_table, step.q_starts, step.kv_lens, max_q=step.max_q, max_kv=step.max_kv)
+            a = decoder.paged_attention(q, kc, vc, step.page_table, step.q_starts, step.kv_lens, max_q=step.max_q, max_kv=step.max_kv,
+                                        window=c.window, sinks=c.sinks)
             h, x = decoder.norm_residual(ly.out.forward(a.view(T, -1)), x, ly.ffn_norm, eps=c.eps)
             f = ops.quantized_matmul(h, ly.gate.weight, ly.gate.scales, ly.gate.biases, True, c.group_size, c.bits, act="swiglu",
                                      up=(ly.up.weight, ly.up.scales, ly.up.biases))
@@ -109,15 +125,57 @@ class Decoder:
         if length > self.config.positions:
             raise ValueError(f"a sequence of {length} tokens: the decoder's table holds {self.config.positions} positions")
 
-    def generate(self, cache: PagedCache, seqs: Sequence[int], tokens: torch.Tensor, new: int) -> torch.Tensor:
-        """Greedy continuation of sequences from their next tokens [B]: [B, new] token ids."""
+    def generate(self, cache: PagedCache, seqs: Sequence[int], tokens: torch.Tensor, new: int, sampling: Optional[Sampling] = None,
+                 u: Optional[torch.Tensor] = None, graph: bool = False) -> torch.Tensor:
+        """Continuation of sequences from their next tokens [B]: [B, new] token ids, the most likely ones or, with
+        ``sampling``, drawn by the random numbers ``u [new, B]`` (float32 in [0, 1); fresh ones if not given).  The pages of
+        all steps are taken at the start, and the steps are issued without waiting for one; with ``graph`` they are
+        one captured graph, replayed."""
         self._fits(max(cache.length(s) for s in seqs) + new)
-        out = []
-        for _ in range(new):
-            logits = self.forward(tokens, cache, cache.step(seqs, [1] * len(seqs)))
-            tokens = logits.argmax(-1)
-            out.append(tokens)
-        return torch.stack(out, 1) if out else tokens.new_empty((len(seqs), 0))
+        if new == 0:
+            return tokens.new_empty((len(seqs), 0))
+        B, dev = len(seqs), self.norm.device
+        if sampling is None:
+            sampling, u = Sampling(temperature=0.0), torch.zeros((new, B), device=dev)
+        elif u is None:
+            u = torch.rand((new, B), device=dev)
+        if u.shape != (new, B):
+            raise ValueError(f"u must be [{new}, {B}], got {list(u.shape)}")
+        u = u.contiguous()
+        out = torch.empty((new, B), dtype=torch.int64, device=dev)
+        at = torch.zeros(1, dtype=torch.int64, device=dev)
+        current = tokens.to(torch.int64, copy=True)
+        ahead, done = cache.ahead(seqs, new), 0
+
+        def step():
+            logits = self.forward(current, cache, ahead.next())
+            current.copy_(sampling.draw(logits, u.index_select(0, at)[0]))
+            out.index_copy_(0, at, current[None])
+            at.add_(1)
+
+        try:
+            step()  # (also what a graph cannot hold: the kernels' first calls)
+            done = 1
+            if graph and new > 1:
+                torch.cuda.current_stream(dev).synchronize()
+                captured = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(captured):
+                    step()
+                for done in range(2, new + 1):
+                    captured.replay()
+            else:
+                for done in range(2, new + 1):
+                    step()
+        finally:
+            ahead.close(done)
+        self._evict(cache, seqs)
+        return out.t().contiguous()
+
+    def _evict(self, cache: PagedCache, seqs: Sequence[int]) -> None:
+        """With a window, the pages behind it go back."""
+        if self.config.window:
+            for s in seqs:
+                cache.evict(s, self.config.window, self.config.sinks)
 
     def prompt(self, cache: PagedCache, seq: int, tokens: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         """Appends a prompt [n] in chunks; returns the last token's logits [1, vocab]."""
@@ -127,6 +185,7 @@ class Decoder:
         for at in range(0, tokens.shape[0], chunk):
             part = tokens[at:at + chunk]
             logits = self.forward(part, cache, cache.step([seq], [part.shape[0]]))
+            self._evict(cache, [seq])
         return logits
 
 
@@ -137,8 +196,15 @@ def main(argv=None) -> None:
     ap.add_argument("--chunk", type=int, default=2048)
     ap.add_argument("--new", type=int, default=64)
     ap.add_argument("--forks", type=int, default=4, help="continuations that share the prompt's pages")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the most likely token")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
+    ap.add_argument("--window", type=int, default=0, help="positions that a token sees (0: all before it)")
+    ap.add_argument("--sinks", type=int, default=0, help="first positions that stay visible beside the window")
+    ap.add_argument("--graph", action="store_true", help="decode steps as replays of one captured graph")
     a = ap.parse_args(argv)
-    model = Decoder.random(Config(layers=a.layers))
+    model = Decoder.random(Config(layers=a.layers, window=a.window, sinks=a.sinks))
     per = -(-(a.prompt + a.new) // 16) + 1
     cache = model.cache(pages=per + a.forks * (a.new // 16 + 2))
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -153,7 +219,7 @@ def main(argv=None) -> None:
     marks[1].record()
     seqs = [seq] + [cache.fork(seq) for _ in range(a.forks - 1)]
     first = logits.topk(len(seqs)).indices[0]  # each continuation starts from another token
-    text = model.generate(cache, seqs, first, a.new)
+    text = model.generate(cache, seqs, first, a.new, Sampling(a.temperature, a.top_k, a.top_p, a.min_p), graph=a.graph)
     marks[2].record()
     torch.cuda.synchronize()
     print(f"prompt of {a.prompt} tokens: {marks[0].elapsed_time(marks[1]):.2f} ms; {a.new} tokens for {len(seqs)} continuations: "
