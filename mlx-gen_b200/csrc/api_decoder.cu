@@ -17,7 +17,6 @@ size_t paged_attention_workspace(int64_t, int, int, int, int64_t, int64_t, int64
 int launch_paged_attention(attn::Params &, int, int, int64_t, void *, cudaStream_t);
 int launch_plan_step(const plank::Params &, cudaStream_t);
 int launch_sample(const samplek::Params &, int, int64_t, cudaStream_t);
-int64_t sample_row_limit();
 
 static int elem_bytes(int dt) { return dt == QL_F32 ? 4 : 2; }
 static bool elem_aligned(const void *p, int dt) { return (reinterpret_cast<uintptr_t>(p) % elem_bytes(dt)) == 0; }
@@ -249,9 +248,8 @@ int ql_sample(const void *logits, int dtype, int64_t row_stride, int64_t B, int6
     if (B < 0 || V < 1 || row_stride < 0)
         return fail(QL_EINVAL_SHAPE, "ql_sample: bad sizes (B=%lld, V=%lld, row stride %lld)", (long long)B, (long long)V,
                     (long long)row_stride);
-    if (V * elem_bytes(dtype) > sample_row_limit())
-        return fail(QL_EUNSUPPORTED, "ql_sample: a row of %lld logits is too long (at most %lld bytes)", (long long)V,
-                    (long long)sample_row_limit());
+    if (V > samplek::MAX_ROW / elem_bytes(dtype))
+        return fail(QL_EUNSUPPORTED, "ql_sample: a row of %lld logits is too long (at most %d bytes)", (long long)V, samplek::MAX_ROW);
     if ((!temperature && !(temperature_all >= 0.0)) || (!top_p && !(top_p_all >= 0.0)) || (!min_p && !(min_p_all >= 0.0 && min_p_all <= 1.0)) ||
         (!top_k && top_k_all < 0))
         return fail(QL_EINVAL_ARG, "ql_sample: temperature, top_k and top_p must not be negative, min_p in [0, 1]");

@@ -11,15 +11,22 @@
 // a hundred.  So each weight is computed in fp64 and held as the whole number
 // W = round(w * 2^S), S = 46 for up to 2^17 tokens, and all sums are of whole numbers: exact, free of
 // any order, so that a row's token does not depend on how the row was divided or on its batch.
-// The exponential (method: table and short polynomial, P. T. P. Tang 1989): 256 y = k + r with whole
-// k and |r| <= 1/2, 2^-y = 2^-(k >> 8) * table[k & 255] * exp(-r ln 2 / 256), whose series ends
-// after the fourth power (the fifth is below 2^-54).
+// The exponential (method: table and short polynomial, P. T. P. Tang 1989): 16 y = k + r with whole
+// k and |r| <= 1/2, 2^-y = 2^-(k >> 4) * table[k & 15] * exp(-r ln 2 / 16), whose series ends after the
+// fifth power (the sixth is below 2^-42: borders move by less than a 10^-12th of the sum).
 //
-// Bound: fp64 instructions (10 of 64 lanes a clock and SM for each logit) for many rows, the chain of
-// cluster barriers for few.  Split: a cluster of CTAs takes a row, each CTA keeps its slice in shared memory,
-// so that the row is read once whatever filters it has.  A threshold is found without sorting: counts
-// (or weights) of the keys in 1024 bins below the largest key, the bin that holds the border divided
-// again, until it holds at most LIST elements, of which every one then counts what precedes it.
+// Bound: for many rows fp64 and integer instructions (9 and about 20 for each logit and pass; 64 and 128 lanes a
+// clock and SM) and the two to four passes that top-p takes; for few rows the chain of passes and cluster barriers, about
+// 1200 cycles each with what is exchanged.  Split: a cluster of up to 16 CTAs takes a row.  Slices that fit stay in shared
+// memory, so that the row is read once whatever filters it has; longer ones are read again by each pass.
+// Nothing is sorted but short lists: top-k takes a bound from the words' largest elements and lists what is above it;
+// top-p counts in 2048 bins and lists a few bins around the border, or all above it where these are few.
+// Scalars travel by stores into the other CTAs' shared memory before a barrier; what every warp would compute for itself is
+// computed by one.
+// Measured (bf16, 128256 logits, a graph's replay): one row greedy 4.3 us, without filter 8.4, top-k 50 11.4, top-p 0.95
+// 16.2; 64 rows 8, 22, 16, 62; 256 rows with top-p 0.98 at temperature 1.5 (half the vocabulary stays) 264.
+#include <string.h>
+
 #include "pdl.cuh"
 
 namespace ql {
@@ -32,7 +39,8 @@ constexpr int WINDOW = 128;       // .. that top-p's border is looked for among
 constexpr int FEW = 128;          // .. up to which each is compared with every other
 constexpr int NEAR = 128;         // bins around a group that are looked at together
 constexpr int MAX_CTAS = 16;      // of a cluster
-constexpr int MAX_SLICE = 160 << 10;  // bytes of a row in one CTA's shared memory
+constexpr int MAX_SLICE = 66 << 10;  // bytes of a row in one CTA's shared memory
+constexpr int MAX_ROW = 1310208;     // bytes of a row: the longest that is tested
 constexpr uint32_t NO_INDEX = 0xffffffffu;
 static_assert(LIST <= THREADS && THREADS == 512 && MAX_CTAS <= WARPS && NEAR == 4 * 32 && GROUPS == 32 && GROUP == 64 && BINS == 4 * THREADS, "the divisions among threads and lanes below");
 
@@ -341,16 +349,33 @@ __device__ __forceinline__ void sync_all() {
     else __syncthreads();
 }
 
-// One row's view: the slice in shared memory as 16-byte words, `words` of them, divided among the
-// warps in order; places outside the slice hold -inf.
-template <typename T, bool CLUSTER>
+// Infinite logits become 0, the others -inf.
+template <typename T>
+__device__ __noinline__ uint4 only_infinite(uint4 v) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4) w[i] = w[i] == 0x7f800000u ? 0u : Type<T>::NONE;
+        else {
+            const uint32_t inf = Type<T>::NONE & 0x7fffu;
+            w[i] = ((w[i] & 0xffffu) == inf ? 0u : Type<T>::NONE & 0xffffu) | ((w[i] >> 16) == inf ? 0u : Type<T>::NONE & 0xffff0000u);
+        }
+    }
+    return v;
+}
+
+// One row's view: the slice as 16-byte words in shared memory or, GLOBAL, where the caller has it (two words of a lane on their
+// way while one is worked on), divided among the warps in order; places outside the slice hold -inf.
+template <typename T, bool CLUSTER, bool GLOBAL>
 struct Row {
     using Ty = Type<T>;
     static constexpr int N = Ty::N, UNIT = Ty::UNIT;
-    uint4 *data;
+    uint4 *data;             // in shared memory
+    const T *src;            // the slice's first token
+    bool infinite;           // GLOBAL: the row holds +inf
     Shared *sh;
     int first, last;         // this warp's words, `per` of them
     int per, tokens;         // .. and the slice's tokens
+    int all_words;           // of the slice
     int skew;                // places before the slice in the first word
     uint32_t base;           // index of the slice's first token
     uint32_t ctas, rank;
@@ -359,14 +384,43 @@ struct Row {
 
     __device__ __forceinline__ uint32_t index(int word, int e) const { return base + (uint32_t)(word * N + e - skew); }
 
+    __device__ __forceinline__ uint4 word(int w) const {
+        uint4 v = make_uint4(Ty::NONE, Ty::NONE, Ty::NONE, Ty::NONE);
+        if (w >= last) return v;
+        if (!GLOBAL) return data[w];
+        const int at = w * N - skew;
+        if (at >= 0 && at + N <= tokens) v = __ldg(reinterpret_cast<const uint4 *>(src + at));
+        else
+#pragma unroll 1
+            for (int e = 0; e < N; ++e)
+                if (at + e >= 0 && at + e < tokens) v = with(v, e, src[at + e]);
+        return infinite ? only_infinite<T>(v) : v;
+    }
+    static __device__ __forceinline__ uint4 with(uint4 v, int e, T x) {
+        uint32_t bits = 0, mask = sizeof(T) == 4 ? 0xffffffffu : 0xffffu;
+        memcpy(&bits, &x, sizeof(T));
+        const int i = e * (int)sizeof(T) / 4, shift = sizeof(T) == 4 ? 0 : (e & 1) * 16;
+        const uint32_t old = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w, now = (old & ~(mask << shift)) | bits << shift;
+        if (i == 0) v.x = now;
+        if (i == 1) v.y = now;
+        if (i == 2) v.z = now;
+        if (i == 3) v.w = now;
+        return v;
+    }
     // f(v, w) of this warp's words in order, 32 at a time, a lane each; -inf past the last
     template <typename F>
     __device__ __forceinline__ void words(F f) const {
         const int lane = threadIdx.x & 31;
-        for (int w0 = first; w0 < last; w0 += 32) {
-            uint4 v = make_uint4(Ty::NONE, Ty::NONE, Ty::NONE, Ty::NONE);
-            if (w0 + lane < last) v = data[w0 + lane];
-            f(v, w0 + lane);
+        if (GLOBAL) {
+            uint4 next = word(first + lane), after = word(first + 32 + lane);
+            for (int w0 = first; w0 < last; w0 += 32) {
+                const uint4 v = next;
+                next = after;
+                after = word(w0 + 64 + lane);
+                f(v, w0 + lane);
+            }
+        } else {
+            for (int w0 = first; w0 < last; w0 += 32) f(word(w0 + lane), w0 + lane);
         }
     }
     // the same without words of which no lane has an element of at least `low`
@@ -496,8 +550,8 @@ struct Row {
 // The token from a list that holds all that may be drawn (at most LIST, in all CTAs' parts): top-k (none where k
 // is 0), top-p by p of the first k's sum -- or by `need`, where that is not 0 --, min-p by `least`, the draw.
 // By one CTA.
-template <typename T, bool CLUSTER>
-__device__ __forceinline__ void finish(const Row<T, CLUSTER> &row, const Weigher &weigh, int which, uint32_t count, uint64_t k, double p,
+template <typename T, bool CLUSTER, bool GLOBAL>
+__device__ __forceinline__ void finish(const Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, int which, uint32_t count, uint64_t k, double p,
                                        uint64_t need, double least, double u, int64_t *token, float *logprob) {
     constexpr int UNIT = Type<T>::UNIT;
     Shared *sh = row.sh;
@@ -550,8 +604,8 @@ __device__ __forceinline__ void finish(const Row<T, CLUSTER> &row, const Weigher
 
 // A value below which nothing is among the k largest: of the 16-byte words' largest elements, from `least` up to
 // `top`, k are at least that large.  -inf if they are not that many.
-template <typename T, bool CLUSTER>
-__device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER> &row, float top, float least, uint64_t k) {
+template <typename T, bool CLUSTER, bool GLOBAL>
+__device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER, GLOBAL> &row, float top, float least, uint64_t k) {
     Shared *sh = row.sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float c = top > least ? (BINS - 1) / (top - least) : 0.f;
@@ -594,8 +648,8 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER> &row, float to
 // with WEIGHT) reaches `need` >= 1, among the elements within `cut` whose keys are from `low` up to `high`.
 // Elements left out by `low` must not be needed.  By histograms of keys, each dividing the bin that
 // holds the border, until it holds at most LIST elements or one value.
-template <bool WEIGHT, typename T, bool CLUSTER>
-__device__ __noinline__ Cut select(Row<T, CLUSTER> &row, const Weigher &weigh, Cut cut, uint32_t high, uint32_t low, uint64_t need) {
+template <bool WEIGHT, typename T, bool CLUSTER, bool GLOBAL>
+__device__ __noinline__ Cut select(Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, Cut cut, uint32_t high, uint32_t low, uint64_t need) {
     constexpr int UNIT = Type<T>::UNIT, LOG = 10;
     constexpr int BINS = 1 << LOG, GROUP = BINS / GROUPS;  // (half of the others': two more words a bin)
     static_assert(GROUP == 32, "one bin a lane");
@@ -732,8 +786,8 @@ __device__ __forceinline__ float bin_at(float at) { return fminf(__fadd_rn(at, B
 // The passes over the logits, each a function of its own: inlined into one kernel they share its registers, and spilled
 // values in their loops tripled their time.
 // Sum of the weights within the cut; elements of at least `low` counted in bins of the width 1 / c below `top`.
-template <bool WHOLE, typename T, bool CLUSTER>
-__device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+template <bool WHOLE, typename T, bool CLUSTER, bool GLOBAL>
+__device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, float top, float low, float c,
                                                uint32_t *count) {
     constexpr int N = Type<T>::N;
     uint32_t *offset = row.sh->offset;
@@ -757,8 +811,8 @@ __device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER> row, const 
     return mine;
 }
 // Sum of the weights within the cut, of at least `low` and before bin `first`; those in bins from that to `last` to the list.
-template <bool WHOLE, typename T, bool CLUSTER>
-__device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+template <bool WHOLE, typename T, bool CLUSTER, bool GLOBAL>
+__device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, float top, float low, float c,
                                               float first, float last) {
     constexpr int N = Type<T>::N;
     uint64_t mine = 0;
@@ -774,18 +828,16 @@ __device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER> row, const W
             listed |= in && bin >= first && bin <= last ? 1u << e : 0u;
         }
         mine -= N * Weigher::BIAS;
-        if (listed) {
-            const T *p = reinterpret_cast<const T *>(row.data + w);
+        if (listed)
 #pragma unroll 1
             for (int e = 0; e < N; ++e)
-                if (listed & (1u << e)) row.append(1, (float)p[e], w, e);
-        }
+                if (listed & (1u << e)) row.append(1, (float)(GLOBAL ? row.src[w * N - row.skew + e] : reinterpret_cast<const T *>(row.data + w)[e]), w, e);
     });
     return mine;
 }
 // Sum of the weights within the cut, of at least `least`.
-template <bool PLAIN, typename T, bool CLUSTER>
-__device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, double least) {
+template <bool PLAIN, typename T, bool CLUSTER, bool GLOBAL>
+__device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, double least) {
     constexpr int N = Type<T>::N;
     uint64_t mine = 0;
     row.words_from(cut.value, [&](const uint4 &v, int w) {
@@ -799,8 +851,8 @@ __device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER> row, const Weigh
 }
 // One warp's elements within the cut and of at least `least`, `at` the sum of those before: the one at which it passes
 // `target` is the token.
-template <typename T, bool CLUSTER>
-__device__ __noinline__ void draw(const Row<T, CLUSTER> row, const Weigher weigh, const Cut cut, double least, uint64_t at, uint64_t target,
+template <typename T, bool CLUSTER, bool GLOBAL>
+__device__ __noinline__ void draw(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, double least, uint64_t at, uint64_t target,
                                   uint64_t sum, int64_t *token, float *logprob) {
     constexpr int N = Type<T>::N;
     row.words_from(cut.value, [&](const uint4 &v, int w) {
@@ -835,8 +887,8 @@ enum Outcome { LISTED, CUT, CUT_AND_SUM };
 // length in `listed`.  Else a pass over the elements above a few bins around the border sums them exactly and lists
 // those in the bins; where the border is not among these after all, the sum tells by how much the
 // estimate is off.  `cut` is then the one after the prefix.
-template <typename T, bool CLUSTER>
-__device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER> &row, const Weigher &weigh, Cut &cut, float top, double p, double reach, uint64_t &need,
+template <typename T, bool CLUSTER, bool GLOBAL>
+__device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, Cut &cut, float top, double p, double reach, uint64_t &need,
                                            uint32_t &listed, uint64_t &sum, uint64_t &before) {
     constexpr int UNIT = Type<T>::UNIT, N = Type<T>::N;
     Shared *sh = row.sh;
@@ -1001,7 +1053,7 @@ __device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER> &row, const Weigher &
             return LISTED;
         }
         if (n > LIST) {  // a bin of many elements, likely equal ones
-            Row<T, CLUSTER> other = row;
+            Row<T, CLUSTER, GLOBAL> other = row;
             cut = select<true>(other, weigh, cut, key_of<UNIT>(top), key_of<UNIT>(low), need);
             row.turn = other.turn, row.sums = other.sums;
             return CUT;
@@ -1032,7 +1084,7 @@ __device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER> &row, const Weigher &
     }
 }
 
-template <typename T, bool CLUSTER>
+template <typename T, bool CLUSTER, bool GLOBAL>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     using Ty = Type<T>;
     constexpr int N = Ty::N, UNIT = Ty::UNIT;
@@ -1041,7 +1093,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     pdl_trigger();
     if (CLUSTER) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     pdl_wait();
-    Row<T, CLUSTER> row;
+    Row<T, CLUSTER, GLOBAL> row;
     row.sh = sh;
     row.data = reinterpret_cast<uint4 *>(smem + (sizeof(Shared) + 15) / 16 * 16);
     row.ctas = CLUSTER ? gridDim.x : 1;
@@ -1051,13 +1103,15 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const int64_t b = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // ---- the slice: whole words by asynchronous copies, the ends one by one
+    // ---- the slice: to shared memory, whole words by asynchronous copies, the ends one by one
     row.base = row.rank * (uint32_t)p.slice;
     const int n = max(0, min(p.slice, p.V - (int)min(row.base, (uint32_t)p.V)));
     const T *src = reinterpret_cast<const T *>(p.logits) + b * p.stride + row.base;
     row.skew = (int)((reinterpret_cast<uintptr_t>(src) & 15u) / sizeof(T));
     const int words = n ? (n + row.skew + N - 1) / N : 0;
-    for (int w = tid; w < words; w += THREADS) {
+    row.src = src;
+    row.infinite = false;
+    for (int w = tid; !GLOBAL && w < words; w += THREADS) {
         const int at = w * N - row.skew;
         if (at >= 0 && at + N <= n) {
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(row.data + w)), "l"(src + at) : "memory");
@@ -1083,6 +1137,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     row.tokens = n;
+    row.all_words = words;
     row.per = (words + THREADS - 1) / THREADS * 32;
     row.first = min(words, warp * row.per);
     row.last = min(words, row.first + row.per);
@@ -1132,12 +1187,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         logprob = 0.f;
     } else {
         if (top == key_of<UNIT>(INFINITY)) {
-            // infinite logits share everything: they are 0 in the slice from here on, the others -inf
-            for (int w = row.first + lane; w < row.last; w += 32) {
-                T *x = reinterpret_cast<T *>(row.data + w);
-#pragma unroll 1
-                for (int e = 0; e < N; ++e) x[e] = (float)x[e] == INFINITY ? T(0.f) : T(-INFINITY);
-            }
+            // infinite logits share everything: they are 0 from here on, the others -inf
+            row.infinite = true;
+            for (int w = row.first + lane; !GLOBAL && w < row.last; w += 32) row.data[w] = only_infinite<T>(row.data[w]);
             __syncwarp();
             top = bottom = key_of<UNIT>(0.f);
         }
@@ -1157,7 +1209,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
                 k = (uint64_t)top_k;
             }
             if (!in_list) {
-                Row<T, CLUSTER> other = row;
+                Row<T, CLUSTER, GLOBAL> other = row;
                 cut = select<false>(other, weigh, cut, top, low > -INFINITY ? max(none + 1, key_of<UNIT>(low)) : none + 1, (uint64_t)top_k);
                 row.turn = other.turn, row.sums = other.sums;
                 k = 0;
@@ -1180,10 +1232,23 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             }
             const double place = fmax((double)u, 0.0) * (double)sum;
             const uint64_t target = place < (double)sum ? min((uint64_t)place, sum - 1) : sum - 1;
+            // the warp in whose words it is, here or in another CTA; then all warps look through these
             uint64_t at = before;
-            for (int i = 0; i < warp; ++i) at += sh->warp_sum[i];
-            if (at <= target && target < at + sh->warp_sum[warp])
-                draw(row, weigh, cut, least, at, target, sum, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
+            int owner = 0;
+            for (; owner < WARPS && target >= at + sh->warp_sum[owner]; ++owner) at += sh->warp_sum[owner];
+            if (target >= at && owner < WARPS) {
+                Row<T, CLUSTER, GLOBAL> part = row;
+                const int from = min(row.all_words, owner * row.per), words = min(row.per, row.all_words - from);
+                const int each = (words + THREADS - 1) / THREADS * 32;
+                part.first = from + min(words, warp * each);
+                part.last = min(from + words, part.first + each);
+                const uint64_t mine = warp_sum(sum_kept<false>(part, weigh, cut, least));
+                if (lane == 0) sh->scratch[0][warp] = mine;
+                __syncthreads();
+                for (int i = 0; i < warp; ++i) at += sh->scratch[0][i];
+                if (at <= target && target < at + mine)
+                    draw(part, weigh, cut, least, at, target, sum, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
+            }
         }
     }
     if (writer) {
@@ -1198,21 +1263,26 @@ template <typename T>
 static int launch(const Params &q, int64_t B, cudaStream_t st) {
     Params p = q;
     const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T);
+    // CTAs of a row: up to 16, fewer where the rows fill the GPU (two CTAs an SM; some more than that at a time pay
+    // while they are few: 96 rows of 607 KB in 4 CTAs 62 us, in 2 68; 256 rows of 256 KB in 2 90, in 1 84), and
+    // slices of 4 KB at least.
     int ctas = MAX_CTAS;
-    // CTAs of a row: 16 where that leaves SMs idle.  More rows than that: fewer and longer slices, up to 80 KB (two CTAs of
-    // 64 KB an SM; 256 rows of 256 KB without filter in 4 CTAs 90 us, in 8 130, in 2 128; 96 rows of 607 KB in 8 67, in 16
-    // 92).  Short rows: 4 KB at least.
-    while (ctas > 1 && (B * ctas > 148 || bytes / ctas < 4096) && bytes * 2 / ctas <= (80 << 10)) ctas /= 2;
+    while (ctas > 1 && (B * ctas > 400 || bytes / ctas < 4096)) ctas /= 2;
     p.slice = ((p.V + ctas - 1) / ctas + 15) / 16 * 16;
-    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (size_t)p.slice * sizeof(T) + 32;
-    auto kernel = ctas > 1 ? sample_kernel<T, true> : sample_kernel<T, false>;
+    // Slices of which two fit an SM stay in shared memory for all passes (64 rows of 256 KB, top-k 50: 16 us, 23 read again by
+    // each pass); longer ones are read again, from L2 mostly (256 rows: 42 us, 62 in slices of 64 KB).
+    const bool global = (int64_t)p.slice * (int64_t)sizeof(T) > MAX_SLICE;
+    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (global ? 0 : (size_t)p.slice * sizeof(T) + 32);
+    auto kernel = ctas > 1 ? (global ? sample_kernel<T, true, true> : sample_kernel<T, true, false>)
+                           : (global ? sample_kernel<T, false, true> : sample_kernel<T, false, false>);
     static PerDeviceFlag configured;
     const int dev = current_device();
     if (!configured.test(dev)) {
         const int most = (int)((sizeof(Shared) + 15) / 16 * 16 + MAX_SLICE + 32);
-        QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-        QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-        QL_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (auto k : {sample_kernel<T, true, true>, sample_kernel<T, true, false>, sample_kernel<T, false, true>, sample_kernel<T, false, false>}) {
+            QL_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+            QL_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
         configured.set(dev);
     }
     const unsigned gy = (unsigned)(B < 32768 ? B : 32768);
@@ -1233,9 +1303,6 @@ static int launch(const Params &q, int64_t B, cudaStream_t st) {
 }
 
 }  // namespace samplek
-
-// bytes of one row's logits that a call can take
-int64_t sample_row_limit() { return (int64_t)8 * samplek::MAX_SLICE - 16 * 4 * 8; }
 
 int launch_sample(const samplek::Params &p, int dtype, int64_t B, cudaStream_t st) {
     using namespace samplek;
