@@ -284,14 +284,16 @@ __device__ __noinline__ ulonglong2 sum_over_few(Shared *sh, uint32_t count, uint
     return make_ulonglong2(n, s);
 }
 
-// fp32 to fp64 in integer instructions (the conversion has a quarter of the fp64 rate).  Values below 2^-126 keep their
-// sign and some magnitude below 2^-125, infinities become 2^128: neither makes a difference to a weight
-// at the temperatures in use (Weigher).
+// fp32 to fp64 in integer instructions (the conversion has a quarter of the fp64 rate).  Values below 2^-126, zeros among
+// them, keep their sign and some magnitude below 2^-125, infinities become 2^128: neither makes a difference to a
+// weight at the temperatures in use (Weigher).  UNIT: zero bits at the end.
+template <int UNIT>
 __device__ __forceinline__ double widen(float x) {
-    const uint32_t b = __float_as_uint(x + 0.f);  // (-0 as 0)
-    return __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)), (int)(b << 29));
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)), UNIT >= 3 ? 0 : (int)(b << 29));
 }
 
+template <int UNIT>
 struct Weigher {
     static constexpr uint64_t BIAS = 0x4330000000000000ull;  // bits of 2^52
     static constexpr double C = 0.04332169878499658;          // ln 2 / 16
@@ -302,16 +304,16 @@ struct Weigher {
 
     // all but the row's largest logit, which comes later
     __device__ __forceinline__ Weigher(double temperature, int scale_, const double *table_) : max(0.0), scale(scale_), table(table_) {
-        // The temperature is held between 2e-29 and 4e28: beyond, only logits below 1e-26 or above 1e26 could
-        // tell the difference.
+        // The temperature is held between 2e-17 and 4e28: beyond, only logits that differ by less than 1e-14, or above
+        // 1e26, could tell the difference (and -0 and 0, whose distance is 2^-126 here, weigh the same).
         const double limit = 16.0 * (scale + 2);
-        rate = fmin(fmax(23.083120654223414 / temperature, limit * 7.888609052210118e-31), 1.2676506002282294e30);
+        rate = fmin(fmax(23.083120654223414 / temperature, limit * 7.888609052210118e-31), 1.152921504606847e18);
         far = __double2hiint(limit / rate);
     }
-    // w and its factor 2^S in one number; 0 with `keep` false and where w is below 2^-(S + 1)
-    __device__ __forceinline__ void parts(float x, bool keep, double &t, double &e) const {
+    // w and its factor 2^S in one number, of an element d below the largest; 0 with `keep` false and where w is below
+    // 2^-(S + 1)
+    __device__ __forceinline__ void parts(double d, bool keep, double &t, double &e) const {
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
-        double d = max - widen(x);
         const int hi = __double2hiint(d);
         d = __hiloint2double(keep && hi < far ? hi : far, __double2loint(d));
         const double s = fma(d, rate, MAGIC);
@@ -323,25 +325,29 @@ struct Weigher {
     }
     // W + BIAS: sums of n of them are n * BIAS too large (modulo 2^64)
     __device__ __forceinline__ uint64_t biased(float x, bool keep) const {
+        return biased_below(max - widen<UNIT>(x), keep);
+    }
+    __device__ __forceinline__ uint64_t biased_below(double d, bool keep) const {
         double t, e;
-        parts(x, keep, t, e);
+        parts(d, keep, t, e);
         return (uint64_t)__double_as_longlong(fma(t, e, 4503599627370496.0));
     }
     __device__ __forceinline__ uint64_t operator()(float x, bool keep = true) const { return biased(x, keep) - BIAS; }
     // ln(w / sum): w from its distance, the sum without its factor 2^S
     __device__ __noinline__ float logprob(float x, uint64_t sum) const {
-        return (float)((widen(x) - max) * (rate * C) - log((double)sum * exp2(-(double)scale)));
+        return (float)((widen<UNIT>(x) - max) * (rate * C) - log((double)sum * exp2(-(double)scale)));
     }
     // the same, 0 where w 2^S is below `least`
     __device__ __forceinline__ uint64_t at_least(float x, bool keep, double least) const {
         double t, e;
-        parts(x, keep, t, e);
+        parts(max - widen<UNIT>(x), keep, t, e);
         return t * e >= least ? (uint64_t)__double_as_longlong(fma(t, e, 4503599627370496.0)) - BIAS : 0ull;
     }
 };
 
 // One weight, where no loop needs it inlined (most of the kernel's time with few rows is instruction fetches).
-__device__ __noinline__ uint64_t weight_of(const Weigher w, float x, double least) { return w.at_least(x, true, least); }
+template <int UNIT>
+__device__ __noinline__ uint64_t weight_of(const Weigher<UNIT> w, float x, double least) { return w.at_least(x, true, least); }
 
 template <bool CLUSTER>
 __device__ __forceinline__ void sync_all() {
@@ -551,7 +557,7 @@ struct Row {
 // is 0), top-p by p of the first k's sum -- or by `need`, where that is not 0 --, min-p by `least`, the draw.
 // By one CTA.
 template <typename T, bool CLUSTER, bool GLOBAL>
-__device__ __forceinline__ void finish(const Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, int which, uint32_t count, uint64_t k, double p,
+__device__ __forceinline__ void finish(const Row<T, CLUSTER, GLOBAL> &row, const Weigher<Type<T>::UNIT> &weigh, int which, uint32_t count, uint64_t k, double p,
                                        uint64_t need, double least, double u, int64_t *token, float *logprob) {
     constexpr int UNIT = Type<T>::UNIT;
     Shared *sh = row.sh;
@@ -649,7 +655,7 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER, GLOBAL> &row, 
 // Elements left out by `low` must not be needed.  By histograms of keys, each dividing the bin that
 // holds the border, until it holds at most LIST elements or one value.
 template <bool WEIGHT, typename T, bool CLUSTER, bool GLOBAL>
-__device__ __noinline__ Cut select(Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, Cut cut, uint32_t high, uint32_t low, uint64_t need) {
+__device__ __noinline__ Cut select(Row<T, CLUSTER, GLOBAL> &row, const Weigher<Type<T>::UNIT> &weigh, Cut cut, uint32_t high, uint32_t low, uint64_t need) {
     constexpr int UNIT = Type<T>::UNIT, LOG = 10;
     constexpr int BINS = 1 << LOG, GROUP = BINS / GROUPS;  // (half of the others': two more words a bin)
     static_assert(GROUP == 32, "one bin a lane");
@@ -770,7 +776,8 @@ __device__ __noinline__ Cut select(Row<T, CLUSTER, GLOBAL> &row, const Weigher &
 
 // Weights below (1 - p) / (2 V) of the largest (1, so of the sum) sum up to less than (1 - p), so none of them is in
 // top-p's prefix: how far below the largest logit the others may be (with a margin for roundings).
-__device__ __forceinline__ double reach_of(const Weigher &weigh, double p, int V) {
+template <int UNIT>
+__device__ __forceinline__ double reach_of(const Weigher<UNIT> &weigh, double p, int V) {
     const double smallest = fmax(0.5, 0.5 * (1.0 - p) / V * exp2((double)weigh.scale));
     return (weigh.scale - log2(smallest)) * 16.0 / weigh.rate * 1.000001;
 }
@@ -787,17 +794,17 @@ __device__ __forceinline__ float bin_at(float at) { return fminf(__fadd_rn(at, B
 // values in their loops tripled their time.
 // Sum of the weights within the cut; elements of at least `low` counted in bins of the width 1 / c below `top`.
 template <bool WHOLE, typename T, bool CLUSTER, bool GLOBAL>
-__device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+__device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER, GLOBAL> row, const Weigher<Type<T>::UNIT> weigh, const Cut cut, float top, float low, float c,
                                                uint32_t *count) {
     constexpr int N = Type<T>::N;
     uint32_t *offset = row.sh->offset;
     uint64_t mine = 0;
-    row.words_from(cut.value, [&](const uint4 &v, int w) {
+    auto add = [&](const uint4 &v, int w) {
         float x[N];
         Type<T>::load(v, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) mine += weigh.biased(x[e], WHOLE || row.kept(cut, x[e], w, e));
-        mine -= N * Weigher::BIAS;
+        mine -= N * weigh.BIAS;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const bool in = x[e] >= low && (WHOLE || row.kept(cut, x[e], w, e));
@@ -807,12 +814,14 @@ __device__ __noinline__ uint64_t sum_and_count(const Row<T, CLUSTER, GLOBAL> row
             // (where in it, from its lower edge on: 0 to 256)
             add_if(&offset[b], __float_as_uint(fmaf(at - (bin - BIN0), 256.f, BIN0 + 128.f)) - __float_as_uint(BIN0), in);
         }
-    });
+    };
+    if (WHOLE) row.words(add);
+    else row.words_from(cut.value, add);
     return mine;
 }
 // Sum of the weights within the cut, of at least `low` and before bin `first`; those in bins from that to `last` to the list.
 template <bool WHOLE, typename T, bool CLUSTER, bool GLOBAL>
-__device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, float top, float low, float c,
+__device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row, const Weigher<Type<T>::UNIT> weigh, const Cut cut, float top, float low, float c,
                                               float first, float last) {
     constexpr int N = Type<T>::N;
     uint64_t mine = 0;
@@ -827,7 +836,7 @@ __device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row,
             mine += weigh.biased(x[e], in && bin < first);
             listed |= in && bin >= first && bin <= last ? 1u << e : 0u;
         }
-        mine -= N * Weigher::BIAS;
+        mine -= N * weigh.BIAS;
         if (listed)
 #pragma unroll 1
             for (int e = 0; e < N; ++e)
@@ -837,22 +846,24 @@ __device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row,
 }
 // Sum of the weights within the cut, of at least `least`.
 template <bool PLAIN, typename T, bool CLUSTER, bool GLOBAL>
-__device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, double least) {
+__device__ __noinline__ uint64_t sum_kept(const Row<T, CLUSTER, GLOBAL> row, const Weigher<Type<T>::UNIT> weigh, const Cut cut, double least) {
     constexpr int N = Type<T>::N;
     uint64_t mine = 0;
-    row.words_from(cut.value, [&](const uint4 &v, int w) {
+    auto add = [&](const uint4 &v, int w) {
         float x[N];
         Type<T>::load(v, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) mine += PLAIN ? weigh.biased(x[e], true) : weigh.at_least(x[e], row.kept(cut, x[e], w, e), least);
-        if (PLAIN) mine -= N * Weigher::BIAS;
-    });
+        if (PLAIN) mine -= N * weigh.BIAS;
+    };
+    if (PLAIN) row.words(add);
+    else row.words_from(cut.value, add);
     return mine;
 }
 // One warp's elements within the cut and of at least `least`, `at` the sum of those before: the one at which it passes
 // `target` is the token.
 template <typename T, bool CLUSTER, bool GLOBAL>
-__device__ __noinline__ void draw(const Row<T, CLUSTER, GLOBAL> row, const Weigher weigh, const Cut cut, double least, uint64_t at, uint64_t target,
+__device__ __noinline__ void draw(const Row<T, CLUSTER, GLOBAL> row, const Weigher<Type<T>::UNIT> weigh, const Cut cut, double least, uint64_t at, uint64_t target,
                                   uint64_t sum, int64_t *token, float *logprob) {
     constexpr int N = Type<T>::N;
     row.words_from(cut.value, [&](const uint4 &v, int w) {
@@ -888,7 +899,7 @@ enum Outcome { LISTED, CUT, CUT_AND_SUM };
 // those in the bins; where the border is not among these after all, the sum tells by how much the
 // estimate is off.  `cut` is then the one after the prefix.
 template <typename T, bool CLUSTER, bool GLOBAL>
-__device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER, GLOBAL> &row, const Weigher &weigh, Cut &cut, float top, double p, double reach, uint64_t &need,
+__device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER, GLOBAL> &row, const Weigher<Type<T>::UNIT> &weigh, Cut &cut, float top, double p, double reach, uint64_t &need,
                                            uint32_t &listed, uint64_t &sum, uint64_t &before) {
     constexpr int UNIT = Type<T>::UNIT, N = Type<T>::N;
     Shared *sh = row.sh;
@@ -900,7 +911,8 @@ __device__ __forceinline__ Outcome nucleus(Row<T, CLUSTER, GLOBAL> &row, const W
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float middle = (float)offset[q] / (256.f * (float)n[q]) - 0.5f;
-            w[q] = n[q] * weigh(fmaf(-((float)(b + q) + middle), width, top), n[q] != 0);
+            // (by the distance: next to a logit of 10^4 the bins may be narrower than fp32 can tell)
+            w[q] = n[q] * (weigh.biased_below(fmax((double)((float)(b + q) + middle) * (double)width, 0.0), n[q] != 0) - weigh.BIAS);
         }
     };
     uint32_t *count = sh->count[row.turn & 1], *group_count = sh->group_count[row.turn & 1];
@@ -1130,7 +1142,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
     const int64_t top_k = p.top_k ? (int64_t)p.top_k[b] : p.top_k_all;
     const float u = p.u[b];
     // (what takes divisions and functions of fp64, under the copies)
-    Weigher weigh(temperature, p.scale, sh->table);
+    Weigher<UNIT> weigh(temperature, p.scale, sh->table);
     const double least = fmin(fmax(min_p, 0.0), 1.0) * exp2((double)p.scale);
     const double reach = top_p < 1.0 ? reach_of(weigh, top_p, p.V) : 0.0;
     if (tid < 16) sh->table[tid] = exp2(-tid / 16.0);
@@ -1194,7 +1206,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             top = bottom = key_of<UNIT>(0.f);
         }
         const float peak = value_of<UNIT>(top);
-        weigh.max = widen(peak);
+        weigh.max = widen<UNIT>(peak);
         Cut cut{-INFINITY, NO_INDEX};
         // whether all that may be drawn is in the list, its length, which counter, and what is left to do with it
         bool in_list = false;

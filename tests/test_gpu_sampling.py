@@ -122,6 +122,17 @@ def test_many_rows_of_distinct_logits(settings):
     check(x, torch.rand(300, generator=g, device="cuda"), **settings)
 
 
+@pytest.mark.parametrize("far", [0.0, 1e4, -3e6])
+@pytest.mark.parametrize("std", [1e-3, 1.0, 300.0])
+def test_narrow_and_wide_rows_far_from_zero(far, std):
+    """Logits whose spread is small next to their size, or large next to the temperature."""
+    g = gen(70)
+    x = far + torch.randn(20, 20011, generator=g, device="cuda") * std
+    u = torch.rand(20, generator=g, device="cuda")
+    for s in (dict(top_p=0.9), dict(top_k=1500, top_p=0.7), dict(top_k=40, top_p=0.9), dict(top_p=0.5, temperature=max(std, 1e-3)), dict()):
+        check(x, u, **s)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("V", [64, 1000, 16384, 100000])
 def test_equal_logits(dtype, V):
