@@ -23,8 +23,8 @@
 // top-p counts in 2048 bins and lists a few bins around the border, or all above it where these are few.
 // Scalars travel by stores into the other CTAs' shared memory before a barrier; what every warp would compute for itself is
 // computed by one.
-// Measured (bf16, 128256 logits, a graph's replay): one row greedy 4.3 us, without filter 8.4, top-k 50 11.4, top-p 0.95
-// 16.2; 64 rows 8, 22, 16, 62; 256 rows with top-p 0.98 at temperature 1.5 (half the vocabulary stays) 264.
+// Measured (bf16, 128256 logits, a graph's replay): one row greedy 4.3 us, without filter 8.5, top-k 50 11.4, top-p 0.95
+// 16.2; 64 rows 7.8, 22, 16, 61; 256 rows with top-p 0.98 at temperature 1.5 (half the vocabulary stays) 261.
 #include <string.h>
 
 #include "pdl.cuh"
