@@ -299,7 +299,8 @@ int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width,
  *     first top_k stay (0: all), of those the shortest prefix with a sum of at least top_p times
  *     theirs (one token at least; 1: all), of those the ones with w_i >= min_p;
  *     tokens[b] = the first that stays, by index, with (sum up to it) > u (sum of all that stay).
- * temperature 0: the largest logit, the lowest index of equal ones.  Each setting is one number for each row
+ * temperature 0: the largest logit, the lowest index of equal ones; others count as 2e-17 at least and 4e28
+ * at most.  Each setting is one number for each row
  * (a pointer) or for all (NULL and the ..._all argument, kept in 64 bits).  Weights are computed in 64 bits and
  * summed as whole numbers (of 2^-46, for more than 2^17 tokens 2^(ceil(log2 V) - 63)), so that a row's token does not
  * depend on the rest of the batch; a logit of -inf is never drawn, those of +inf share everything.  u is taken as at

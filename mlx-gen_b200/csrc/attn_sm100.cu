@@ -34,7 +34,8 @@
 // TMEM has no room for a third tile's S and O; the 64 columns of S_t that P_t leaves free are unused.
 // Measured (24 / 8 heads of 128): 512 tokens over 16021 positions 101 us = 1013 TFLOP/s in a graph's
 // replay and 115 us = 887 in calls back to back, where the power cap lowers the clock; 4096 tokens causal
-// 114 us = 902 and 123 us = 836; cuBLAS reaches 1644 TFLOP/s in bf16.
+// 114 us = 902 and 123 us = 836; cuBLAS reaches 1644 TFLOP/s in bf16.  With sinks: 1024 tokens over 30011 positions, window 4096
+// and 64 sinks, 79 us; 4096 tokens, window 1024 and 4 sinks, 74 us; 17 chunks of heads of 64, window 256 and 16 sinks, 50 us.
 #include "attn_common.cuh"
 
 namespace ql {

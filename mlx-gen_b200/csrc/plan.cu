@@ -13,6 +13,7 @@
 // at its first position, which is always a new one.  Many tokens: a CTA for each tile.  Where lengths or the count
 // of taken pages are updated in place, a cluster of 8 shares the tiles instead, so that all CTAs have read them (cluster
 // barrier) before one writes them.
+// Measured (a graph's replay): 64 sequences of one token 2.9 us, 203 of 62119 tokens 6.6 us (by the cluster of 8 18.7).
 #include "pdl.cuh"
 
 namespace ql {
