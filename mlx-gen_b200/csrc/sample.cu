@@ -840,7 +840,9 @@ __device__ __noinline__ uint64_t sum_and_list(const Row<T, CLUSTER, GLOBAL> row,
         if (listed)
 #pragma unroll 1
             for (int e = 0; e < N; ++e)
-                if (listed & (1u << e)) row.append(1, (float)(GLOBAL ? row.src[w * N - row.skew + e] : reinterpret_cast<const T *>(row.data + w)[e]), w, e);
+                // (as `words` gives them: an infinite logit is 0)
+                if (listed & (1u << e))
+                    row.append(1, row.infinite ? 0.f : (float)(GLOBAL ? row.src[w * N - row.skew + e] : reinterpret_cast<const T *>(row.data + w)[e]), w, e);
     });
     return mine;
 }
@@ -1173,10 +1175,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         top = __reduce_max_sync(0xffffffffu, lane < row.ctas ? sh->max_of[lane] : 0u);
         bottom = __reduce_min_sync(0xffffffffu, lane < row.ctas ? sh->min_of[lane] : NO_INDEX);
     }
+    // no token, until one is drawn: whichever thread does that has this write behind it by a barrier below
+    if (row.rank == 0 && tid == 0) {
+        p.tokens[b] = -1;
+        if (p.logprobs) p.logprobs[b] = __uint_as_float(0x7fc00000u);
+    }
     const uint32_t none = key_of<UNIT>(-INFINITY);
-    int64_t token = -1;
-    float logprob = __uint_as_float(0x7fc00000u);
-    bool writer = row.rank == 0 && tid == 0;
     // a NaN among the logits or the settings, nothing above -inf, a negative temperature: no token
     const bool bad = top > key_of<UNIT>(INFINITY) || top <= none || !(temperature >= 0.0) || top_p != top_p || min_p != min_p || u != u;
     if (bad) {
@@ -1195,8 +1199,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
         if (warp == 0) row.tell(sh->first_of, sh->first);
         sync_all<CLUSTER>();
         at = __reduce_min_sync(0xffffffffu, lane < row.ctas ? sh->first_of[lane] : NO_INDEX);
-        token = at;
-        logprob = 0.f;
+        if (row.rank == 0 && tid == 0) {
+            p.tokens[b] = at;
+            if (p.logprobs) p.logprobs[b] = 0.f;
+        }
     } else {
         if (top == key_of<UNIT>(INFINITY)) {
             // infinite logits share everything: they are 0 from here on, the others -inf
@@ -1232,7 +1238,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
             in_list = o == LISTED;
             summed = o == CUT_AND_SUM && least == 0.0;
         }
-        writer = false;
         if (in_list) {
             if (row.rank == 0)
                 finish(row, weigh, k ? 0 : 1, listed, k, top_p, need, least, (double)u, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
@@ -1262,10 +1267,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Params p) {
                     draw(part, weigh, cut, least, at, target, sum, p.tokens + b, p.logprobs ? p.logprobs + b : nullptr);
             }
         }
-    }
-    if (writer) {
-        p.tokens[b] = token;
-        if (p.logprobs) p.logprobs[b] = logprob;
     }
     __syncwarp();
     if (CLUSTER) cluster_sync_all();  // no CTA leaves while another reads its shared memory
