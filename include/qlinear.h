@@ -294,6 +294,13 @@ int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width,
                  int64_t num_free, const int32_t *taken, int64_t *positions, int64_t *slots, int32_t *q_starts,
                  int32_t *kv_lens, int32_t *taken_out, void *stream);
 
+/* The same, and a step after which a sequence would hold more than max_kv tokens has no room either: the bound that the
+ * attention behind it was captured with, which a replay too many would pass inside its last page. */
+int ql_plan_step_within(int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                        const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, int64_t max_kv,
+                        const int32_t *free_pages, int64_t num_free, const int32_t *taken, int64_t *positions,
+                        int64_t *slots, int32_t *q_starts, int32_t *kv_lens, int32_t *taken_out, void *stream);
+
 /* One token per row of logits [B, V] (row_stride elements between rows, 0: all the same) from random numbers u [B] in [0, 1):
  *     w_i = exp((x_i - max x) / temperature); in the order of x (descending, equal ones by index) the
  *     first top_k stay (0: all), of those the shortest prefix with a sum of at least top_p times

@@ -218,10 +218,19 @@ int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width,
                  const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, const int32_t *free_pages,
                  int64_t num_free, const int32_t *taken, int64_t *positions, int64_t *slots, int32_t *q_starts,
                  int32_t *kv_lens, int32_t *taken_out, void *stream) {
+    return ql_plan_step_within(page_table, table_stride, table_width, lengths, new_tokens, B, page_size, max_tokens, INT32_MAX,
+                               free_pages, num_free, taken, positions, slots, q_starts, kv_lens, taken_out, stream);
+}
+
+int ql_plan_step_within(int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                        const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, int64_t max_kv,
+                        const int32_t *free_pages, int64_t num_free, const int32_t *taken, int64_t *positions,
+                        int64_t *slots, int32_t *q_starts, int32_t *kv_lens, int32_t *taken_out, void *stream) {
     g_err[0] = 0;
-    if (B < 0 || B > INT32_MAX - 1 || max_tokens < 0 || max_tokens > INT32_MAX || num_free < 0 || num_free > INT32_MAX)
-        return fail(QL_EINVAL_SHAPE, "ql_plan_step: bad sizes (B=%lld, max_tokens=%lld, num_free=%lld)", (long long)B,
-                    (long long)max_tokens, (long long)num_free);
+    if (B < 0 || B > INT32_MAX - 1 || max_tokens < 0 || max_tokens > INT32_MAX || num_free < 0 || num_free > INT32_MAX ||
+        max_kv < 0 || max_kv > INT32_MAX)
+        return fail(QL_EINVAL_SHAPE, "ql_plan_step: bad sizes (B=%lld, max_tokens=%lld, max_kv=%lld, num_free=%lld)", (long long)B,
+                    (long long)max_tokens, (long long)max_kv, (long long)num_free);
     if (!pow2(page_size)) return fail(QL_EUNSUPPORTED, "page size must be a power of two (got %d)", page_size);
     if (table_width < 0 || (B > 1 && table_stride < table_width))
         return fail(QL_EINVAL_SHAPE, "ql_plan_step: the page table's rows overlap (%lld entries, stride %lld)", (long long)table_width,
@@ -234,7 +243,7 @@ int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width,
         if (reinterpret_cast<uintptr_t>(w) % 4) return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(slots) % 8)
         return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
-    const ql::plank::Params p{page_table, table_stride, table_width, lengths, new_tokens, B, max_tokens, log2i(page_size),
+    const ql::plank::Params p{page_table, table_stride, table_width, lengths, new_tokens, B, max_tokens, max_kv, log2i(page_size),
                               free_pages, num_free, taken, positions, slots, q_starts, kv_lens, taken_out};
     return launch_plan_step(p, (cudaStream_t)stream);
 }

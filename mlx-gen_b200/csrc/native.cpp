@@ -34,7 +34,7 @@ decltype(&ql_paged_attention) p_paged_attention;
 decltype(&ql_paged_attention_workspace_size) p_paged_attention_workspace_size;
 decltype(&ql_copy_pages) p_copy_pages;
 decltype(&ql_sink_attention) p_sink_attention;
-decltype(&ql_plan_step) p_plan_step;
+decltype(&ql_plan_step_within) p_plan_step;
 decltype(&ql_sample) p_sample;
 PyObject *g_error;  // QlError(status, message)
 
@@ -317,7 +317,7 @@ at::Tensor given(PyObject *out, int i, const char *name, int64_t n, at::ScalarTy
     return t;
 }
 
-// (page_table, lengths, new_tokens, page_size, max_tokens, free_pages, taken, out) -> (positions, slots, q_starts, kv_lens, taken)
+// (page_table, lengths, new_tokens, page_size, max_tokens, max_kv, free_pages, taken, out) -> (positions, slots, q_starts, kv_lens, taken)
 PyObject *plan_step(PyObject *const *a) {
     const at::Tensor &table = tensor(a[0], "page_table"), &lengths = tensor(a[1], "lengths"), &fresh_tokens = tensor(a[2], "new_tokens");
     const c10::Device dev = on_cuda(table);
@@ -325,36 +325,38 @@ PyObject *plan_step(PyObject *const *a) {
           lengths.sizes(), " and ", table.sizes());
     const int64_t B = lengths.size(0), max_tokens = integer(a[4]);
     VALUE(max_tokens >= 0 && max_tokens <= INT32_MAX, "max_tokens is out of range: ", max_tokens);
+    const int64_t max_kv = a[5] == Py_None ? INT32_MAX : integer(a[5]);
+    VALUE(max_kv >= 0 && max_kv <= INT32_MAX, "max_kv is out of range: ", max_kv);
     VALUE(B <= 1 || table.size(1) == 0 || table.stride(0) >= table.size(1), "page_table's rows overlap");
     const int32_t *lp = counts(lengths, "lengths", B, dev), *np = counts(fresh_tokens, "new_tokens", B, dev);
     index_tensor(table, "page_table", dev);
     const int32_t *fp = nullptr, *tp = nullptr;
     int64_t num_free = 0;
-    const bool grows = a[5] != Py_None;
-    VALUE(grows == (a[6] != Py_None), "free_pages and taken go together");
+    const bool grows = a[6] != Py_None;
+    VALUE(grows == (a[7] != Py_None), "free_pages and taken go together");
     if (grows) {
-        const at::Tensor &pages = tensor(a[5], "free_pages");
+        const at::Tensor &pages = tensor(a[6], "free_pages");
         fp = counts(pages, "free_pages", -1, dev);
-        tp = counts(tensor(a[6], "taken"), "taken", 1, dev);
+        tp = counts(tensor(a[7], "taken"), "taken", 1, dev);
         num_free = pages.size(0);
     }
-    TYPE(a[7] == Py_None || (PyTuple_Check(a[7]) && PyTuple_GET_SIZE(a[7]) == 5), "out must be what a call returned: (positions, slots, q_starts, kv_lens, taken)");
+    TYPE(a[8] == Py_None || (PyTuple_Check(a[8]) && PyTuple_GET_SIZE(a[8]) == 5), "out must be what a call returned: (positions, slots, q_starts, kv_lens, taken)");
     const c10::cuda::CUDAGuard guard(dev);
     at::Tensor positions, slots, starts, lens, taken;
-    if (a[7] == Py_None) {  // five vectors in one allocation
+    if (a[8] == Py_None) {  // five vectors in one allocation
         const at::Tensor whole = fresh({16 * max_tokens + 4 * (2 * B + 2)}, at::kByte, dev);
         positions = part(whole, 0, max_tokens, at::kLong), slots = part(whole, 8 * max_tokens, max_tokens, at::kLong);
         starts = part(whole, 16 * max_tokens, B + 1, at::kInt), lens = part(whole, 16 * max_tokens + 4 * (B + 1), B, at::kInt);
         if (grows) taken = part(whole, 16 * max_tokens + 4 * (2 * B + 1), 1, at::kInt);
     } else {
-        positions = given(a[7], 0, "positions", max_tokens, at::kLong, dev), slots = given(a[7], 1, "slots", max_tokens, at::kLong, dev);
-        starts = given(a[7], 2, "q_starts", B + 1, at::kInt, dev), lens = given(a[7], 3, "kv_lens", B, at::kInt, dev);
-        if (grows) taken = given(a[7], 4, "taken", 1, at::kInt, dev);
+        positions = given(a[8], 0, "positions", max_tokens, at::kLong, dev), slots = given(a[8], 1, "slots", max_tokens, at::kLong, dev);
+        starts = given(a[8], 2, "q_starts", B + 1, at::kInt, dev), lens = given(a[8], 3, "kv_lens", B, at::kInt, dev);
+        if (grows) taken = given(a[8], 4, "taken", 1, at::kInt, dev);
     }
     // (an empty free list has no address of its own)
     if (grows && !fp) fp = tp;
     check(p_plan_step(const_cast<int32_t *>(table.const_data_ptr<int32_t>()), B > 1 ? table.stride(0) : table.size(1), table.size(1), lp, np,
-                      B, int32(a[3], "page_size"), max_tokens, fp, num_free, tp, positions.mutable_data_ptr<int64_t>(),
+                      B, int32(a[3], "page_size"), max_tokens, max_kv, fp, num_free, tp, positions.mutable_data_ptr<int64_t>(),
                       slots.mutable_data_ptr<int64_t>(), starts.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(),
                       grows ? taken.mutable_data_ptr<int32_t>() : nullptr, stream_of(dev)));
     PyObject *last = Py_None;
@@ -492,7 +494,7 @@ PyMethodDef method(const char *name) {
 PyMethodDef g_methods[] = {
     {"init", init, METH_VARARGS, nullptr},  method<norm_residual, 11>("norm_residual"), method<rope, 5>("rope"),
     method<rope_append, 9>("rope_append"),  method<paged_attention, 14>("paged_attention"),
-    method<copy_pages, 3>("copy_pages"),    method<plan_step, 8>("plan_step"), method<sample, 7>("sample"),
+    method<copy_pages, 3>("copy_pages"),    method<plan_step, 9>("plan_step"), method<sample, 7>("sample"),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -25,7 +25,7 @@ struct Params {
     int32_t *table;
     int64_t table_stride, table_width;
     const int32_t *lengths, *new_tokens;
-    int64_t B, max_tokens;
+    int64_t B, max_tokens, max_kv;  // (max_kv: at most INT32_MAX)
     int page_shift;
     const int32_t *free_pages;  // NULL: the tables hold every page already
     int64_t num_free;
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(MAX_THREADS) plan_kernel(const __grid_constant
     bool bad = taken < 0;
     for (int64_t b = b0; b < b1; ++b) {
         const int64_t have = p.lengths[b], n = p.new_tokens[b];
-        bad = bad || have < 0 || n < 0 || have + n > INT32_MAX || pages_of(have + n) > p.table_width;
+        bad = bad || have < 0 || n < 0 || have + n > p.max_kv || pages_of(have + n) > p.table_width;
         tokens += n;
         if (p.free_pages) pages += pages_of(have + n) - pages_of(have);
     }

@@ -52,6 +52,7 @@ EXPORTS = (
     "ql_copy_pages",
     "ql_sink_attention",
     "ql_plan_step",
+    "ql_plan_step_within",
     "ql_sample",
 )
 
@@ -134,10 +135,11 @@ def lib():
         L.ql_sink_attention.argtypes = [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i64, i64, i32, vp, i64, vp, vp,
                                         i64, i64, i64, f32, i64, i64, vp, vp, sz, vp]
         L.ql_plan_step.argtypes = [vp, i64, i64, vp, vp, i64, i32, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
+        L.ql_plan_step_within.argtypes = [vp, i64, i64, vp, vp, i64, i32, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
         L.ql_sample.argtypes = [vp, i32, i64, i64, i64, vp, vp, C.c_double, vp, i64, vp, C.c_double, vp, C.c_double, vp,
                                 vp, vp]
         for f in ("ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention", "ql_copy_pages",
-                  "ql_sink_attention", "ql_plan_step", "ql_sample"):
+                  "ql_sink_attention", "ql_plan_step", "ql_plan_step_within", "ql_sample"):
             getattr(L, f).restype = i32
         for f in ("ql_quantize", "ql_dequantize", "ql_dequantize_rows", "ql_layernorm_modulate", "ql_quantized_matmul",
                   "ql_quantized_matmul_noalloc"):

@@ -240,12 +240,15 @@ class PagedCache:
 class Ahead:
     """Steps of one token for each of some sequences, with their pages reserved and every step's index
     tensors made on the GPU from the lengths of the step before: ``next`` uploads nothing and waits for nothing,
-    and may be captured in a graph and replayed, up to ``steps`` times in all.  ``close`` tells the cache how many steps ran."""
+    and may be captured in a graph and replayed, up to ``steps`` times in all; a replay beyond them has no tokens, and
+    ``device_error()`` tells.  ``close`` tells the cache how many steps ran; a captured step must not be replayed after
+    it (its pages may be another sequence's by then)."""
 
     def __init__(self, cache: PagedCache, seqs: Sequence[int], steps: int):
         if steps < 1:
             raise ValueError(f"at least one step, got {steps}")
         self.cache, self.seqs, self.steps = cache, list(seqs), steps
+        self._called = 0  # steps that `next` itself ran
         need = cache._room(self.seqs, [steps] * len(self.seqs))
         cache._unshare(self.seqs)
         self._free = [cache._take() for _ in range(need)]
@@ -263,9 +266,19 @@ class Ahead:
         self._open = True
 
     def next(self) -> Step:
-        """The next step; its tensors are those of the step before, written again."""
+        """The next step; its tensors are those of the step before, written again.  More calls than steps raise
+        ValueError.  After ``close`` a step has no tokens (slots -1), whatever became of its pages, and ``device_error()`` tells."""
+        B, ps = len(self.seqs), self.cache.page_size
+        if not self._open:  # (counts below 0: no room)
+            positions, slots, starts, lens, _ = decoder.plan_step(
+                self._table, self._lengths, torch.full_like(self._ones, -1), page_size=ps, max_tokens=B)
+            return Step(positions, slots, self._table, starts, lens, 1, self.max_kv)
+        if not torch.cuda.is_current_stream_capturing():
+            if self._called == self.steps:
+                raise ValueError(f"all {self.steps} reserved steps have run")
+            self._called += 1
         positions, slots, starts, lens, _ = decoder.plan_step(
-            self._table, self._lengths, self._ones, page_size=self.cache.page_size, max_tokens=len(self.seqs), free_pages=self._pages,
+            self._table, self._lengths, self._ones, page_size=ps, max_tokens=B, max_kv=self.max_kv, free_pages=self._pages,
             taken=self._out[4], out=self._out)
         return Step(positions, slots, self._table, starts, lens, 1, self.max_kv)
 

@@ -36,7 +36,7 @@ class _Native:
         L = lib()
         m.init(_lib.QlError, *(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
             "ql_last_error", "ql_norm_residual", "ql_rope", "ql_rope_append", "ql_paged_attention",
-            "ql_paged_attention_workspace_size", "ql_copy_pages", "ql_sink_attention", "ql_plan_step", "ql_sample")))
+            "ql_paged_attention_workspace_size", "ql_copy_pages", "ql_sink_attention", "ql_plan_step_within", "ql_sample")))
         for f in ("norm_residual", "rope", "rope_append", "paged_attention", "copy_pages", "plan_step", "sample"):
             setattr(self, f, getattr(m, f))
         return self.__dict__[name]
@@ -200,7 +200,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 # ------------------------------------------------------------------------ from step to step
 
 def plan_step(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor, *, page_size: int, max_tokens: int,
-              free_pages: Optional[torch.Tensor] = None, taken: Optional[torch.Tensor] = None,
+              max_kv: Optional[int] = None, free_pages: Optional[torch.Tensor] = None, taken: Optional[torch.Tensor] = None,
               out: Optional[tuple] = None) -> tuple:
     """The index tensors of a step in which sequence b, ``lengths[b]`` tokens long, gets ``new_tokens[b]``
     more (int32 ``[B]`` both): returns ``(positions, slots, q_starts, kv_lens, taken)`` for ``rope_append`` and
@@ -210,11 +210,11 @@ def plan_step(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: torch
     ``page_table [B, pages]`` (int32).  With a free list -- ``free_pages`` (int32) and ``taken [1]``, the number of its
     entries in use -- pages that the new tokens need are taken from it in the order of the sequences
     and entered in the page table; the returned ``taken`` counts them.  Without, the table holds every page
-    already and ``taken`` is None.  A step that finds too few pages, columns or rows (or counts below 0) has no
-    tokens and changes nothing; ``device_error()`` tells.  ``out``: what an earlier call returned, to be
+    already and ``taken`` is None.  A step that finds too few pages, columns or rows, or after which a sequence would
+    hold more than ``max_kv`` tokens (or with counts below 0) has no tokens and changes nothing; ``device_error()`` tells.  ``out``: what an earlier call returned, to be
     written again; its kv_lens may be ``lengths`` and its taken ``taken``, so that each replay of a captured call
     goes one step on."""
-    return _native.plan_step(page_table, lengths, new_tokens, page_size, max_tokens, free_pages, taken, out)
+    return _native.plan_step(page_table, lengths, new_tokens, page_size, max_tokens, max_kv, free_pages, taken, out)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: bool = False):

@@ -166,6 +166,11 @@ extern "C" {
                         new_tokens: *const i32, b: i64, page_size: c_int, max_tokens: i64, free_pages: *const i32,
                         num_free: i64, taken: *const i32, positions: *mut i64, slots: *mut i64, q_starts: *mut i32,
                         kv_lens: *mut i32, taken_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ql_plan_step_within(page_table: *mut i32, table_stride: i64, table_width: i64, lengths: *const i32,
+                               new_tokens: *const i32, b: i64, page_size: c_int, max_tokens: i64, max_kv: i64,
+                               free_pages: *const i32, num_free: i64, taken: *const i32, positions: *mut i64,
+                               slots: *mut i64, q_starts: *mut i32, kv_lens: *mut i32, taken_out: *mut i32,
+                               stream: *mut c_void) -> c_int;
     pub fn ql_sample(logits: *const c_void, dtype: c_int, row_stride: i64, b: i64, v: i64, u: *const f32,
                      temperature: *const f32, temperature_all: f64, top_k: *const i32, top_k_all: i64,
                      top_p: *const f32, top_p_all: f64, min_p: *const f32, min_p_all: f64, tokens: *mut i64,
