@@ -242,7 +242,9 @@ class Ahead:
     tensors made on the GPU from the lengths of the step before: ``next`` uploads nothing and waits for nothing,
     and may be captured in a graph and replayed, up to ``steps`` times in all; a replay beyond them has no tokens, and
     ``device_error()`` tells.  ``close`` tells the cache how many steps ran; a captured step must not be replayed after
-    it (its pages may be another sequence's by then)."""
+    it (its pages may be another sequence's by then).  One that is dropped without ``close`` closes with no step."""
+
+    _open = False
 
     def __init__(self, cache: PagedCache, seqs: Sequence[int], steps: int):
         if steps < 1:
@@ -255,15 +257,23 @@ class Ahead:
         B, ps, dev = len(self.seqs), cache.page_size, cache.pool.device
         had = [cache._lens[s] for s in self.seqs]
         self.max_kv = max(had) + steps
-        table, width = cache._table(self.seqs, -(-self.max_kv // ps))
-        small = torch.tensor(table + had + [1] * B + self._free + [0], dtype=torch.int32).to(dev, non_blocking=True)
-        self._table = small[:B * width].view(B, width)
-        self._lengths, self._ones, rest = small[B * width:B * width + B], small[B * width + B:B * width + 2 * B], small[B * width + 2 * B:]
-        self._pages, taken = rest[:need], rest[need:]
-        wide = torch.zeros(2 * B, dtype=torch.int64, device=dev)
-        self._out = (wide[:B], wide[B:], torch.zeros(B + 1, dtype=torch.int32, device=dev), self._lengths, taken)
+        try:
+            table, width = cache._table(self.seqs, -(-self.max_kv // ps))
+            small = torch.tensor(table + had + [1] * B + self._free + [0], dtype=torch.int32).to(dev, non_blocking=True)
+            self._table = small[:B * width].view(B, width)
+            self._lengths, self._ones, rest = small[B * width:B * width + B], small[B * width + B:B * width + 2 * B], small[B * width + 2 * B:]
+            self._pages, taken = rest[:need], rest[need:]
+            wide = torch.zeros(2 * B, dtype=torch.int64, device=dev)
+            self._out = (wide[:B], wide[B:], torch.zeros(B + 1, dtype=torch.int32, device=dev), self._lengths, taken)
+        except BaseException:  # (no memory on the device)
+            cache._drop(self._free)
+            raise
         cache._lent.update(self.seqs)
         self._open = True
+
+    def __del__(self):
+        if self._open:
+            self.close(0)
 
     def next(self) -> Step:
         """The next step; its tensors are those of the step before, written again.  More calls than steps raise
