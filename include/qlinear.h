@@ -287,7 +287,8 @@ int ql_sink_attention(const void *q, int dtype, int64_t q_token_stride, int64_t 
  * are not used.  All or nothing: counts below 0, more tokens than max_tokens, pages past table_width or
  * past num_free give a step without tokens (kv_lens = lengths, q_starts 0, nothing taken) and set
  * the device error word; so does a negative table entry, whose tokens get slot -1.  kv_lens may be
- * lengths and taken_out taken: a captured call then advances the sequences at every replay.
+ * lengths and taken_out taken: a captured call then advances the sequences at every replay; any other output over an
+ * input, an output or the page table's rows is refused.
  * page_size: a power of two. */
 int ql_plan_step(int32_t *page_table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
                  const int32_t *new_tokens, int64_t B, int page_size, int64_t max_tokens, const int32_t *free_pages,

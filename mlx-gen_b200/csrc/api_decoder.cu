@@ -28,6 +28,14 @@ static int log2i(int64_t v) {
     return s;
 }
 
+// Whether the n bytes at `a` touch one of the rows of `width` bytes, `stride` >= width apart, from `base` on.
+static bool touches_rows(const void *a, int64_t n, const void *base, int64_t rows, int64_t stride, int64_t width) {
+    if (n <= 0 || rows <= 0 || width <= 0) return false;
+    const int64_t from = (int64_t)(reinterpret_cast<intptr_t>(a) - reinterpret_cast<intptr_t>(base));
+    const int64_t row = from < width ? 0 : rows > 1 ? (from - width) / stride + 1 : 1;  // the first that ends behind a
+    return row < rows && row * stride < from + n;
+}
+
 static int check_attention(int64_t T, int Hq, int Hkv, int D, int64_t B, int64_t max_q, int64_t max_kv) {
     if (T < 0 || T > INT32_MAX || B < 0 || B > 65535)
         return fail(QL_EINVAL_SHAPE, "ql_paged_attention: bad token or sequence count (T=%lld, B=%lld; at most 65535 sequences)",
@@ -243,6 +251,25 @@ int ql_plan_step_within(int32_t *page_table, int64_t table_stride, int64_t table
         if (reinterpret_cast<uintptr_t>(w) % 4) return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(slots) % 8)
         return fail(QL_EINVAL_ARG, "ql_plan_step: pointer not aligned to its dtype");
+    // What is written may not be read or written as something else: CTAs that still read would see it.  (In place is what
+    // the kernel waits for: kv_lens over lengths, taken_out over taken.)
+    struct Range {
+        const void *at;
+        int64_t bytes;
+        bool written;
+    };
+    const Range all[] = {{lengths, 4 * B, false}, {new_tokens, 4 * B, false}, {free_pages, 4 * num_free, false}, {taken, free_pages ? 4 : 0, false},
+                         {positions, 8 * max_tokens, true}, {slots, 8 * max_tokens, true}, {q_starts, 4 * (B + 1), true}, {kv_lens, 4 * B, true},
+                         {taken_out, free_pages ? 4 : 0, true}};
+    for (const Range &w : all) {
+        if ((w.written || free_pages) && touches_rows(w.at, w.bytes, page_table, B, 4 * table_stride, 4 * table_width))
+            return fail(QL_EINVAL_ARG, "ql_plan_step: the page table overlaps another argument");
+        for (const Range &r : all) {
+            const bool in_place = w.at == r.at && ((&w == &all[7] && &r == &all[0]) || (&w == &all[8] && &r == &all[3]));
+            if (w.written && &r != &w && !in_place && touches_rows(r.at, r.bytes, w.at, 1, w.bytes, w.bytes))
+                return fail(QL_EINVAL_ARG, "ql_plan_step: an output overlaps another argument");
+        }
+    }
     const ql::plank::Params p{page_table, table_stride, table_width, lengths, new_tokens, B, max_tokens, max_kv, log2i(page_size),
                               free_pages, num_free, taken, positions, slots, q_starts, kv_lens, taken_out};
     return launch_plan_step(p, (cudaStream_t)stream);

@@ -28,3 +28,24 @@ def test_the_rest_is_refused_as_without_a_bound():
                dict(table=PAGE + 1), dict(slots=PAGE + 4)):
         assert call(**kw) == _lib.QL_EINVAL_ARG, kw
     assert call(ps=12) == _lib.QL_EUNSUPPORTED
+
+
+def at(name, offset=0):
+    return BASE[name] * PAGE + offset
+
+
+@pytest.mark.parametrize("kw", [
+    # an output over an input, whole or in part
+    dict(lens=at("new")), dict(lens=at("new", 4)), dict(lens=at("lengths", 4)), dict(lens=at("lengths", -4)), dict(starts=at("lengths")),
+    dict(starts=at("new", -8)), dict(starts=at("lengths", -8)), dict(positions=at("lengths")), dict(slots=at("new")), dict(lens=at("free", 8)),
+    dict(taken_out=at("lengths", 4)), dict(taken_out=at("free")), dict(taken_out=at("new")), dict(lens=at("taken")), dict(slots=at("free", 8)),
+    # over another output
+    dict(slots=at("positions")), dict(slots=at("positions", 24)), dict(starts=at("lens", 4)), dict(lens=at("starts", 8)), dict(taken_out=at("starts", 8)),
+    dict(lens=at("slots", 28)), dict(lengths=at("lens"), taken_out=at("lens"), B=1),
+    # over the page table's rows, which are written too
+    dict(positions=at("table")), dict(lens=at("table", 60)), dict(starts=at("table", -8)), dict(lengths=at("table", 28)), dict(free=at("table", 32)),
+    dict(taken=at("table", 63 - 3), taken_out=at("table", 63 - 3)), dict(new=at("table", 40), stride=10), dict(lens=at("table", 200), B=7),
+], ids=str)
+def test_outputs_over_other_arguments(kw):
+    assert call(**kw) == _lib.QL_EINVAL_ARG, kw
+    assert b"overlaps" in _lib.lib().ql_last_error()
