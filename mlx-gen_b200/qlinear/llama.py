@@ -161,11 +161,12 @@ class Decoder:
                 captured = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(captured):
                     step()
-                for done in range(2, new + 1):
-                    captured.replay()
+                run = captured.replay
             else:
-                for done in range(2, new + 1):
-                    step()
+                run = step
+            while done < new:
+                run()
+                done += 1  # (only a step that was issued in all its layers counts)
         finally:
             ahead.close(done)
         self._evict(cache, seqs)
