@@ -132,7 +132,7 @@ class Decoder:
         all steps are taken at the start, and the steps are issued without waiting for one; with ``graph`` they are
         one captured graph, replayed."""
         self._fits(max(cache.length(s) for s in seqs) + new)
-        if new == 0:
+        if new <= 0:
             return tokens.new_empty((len(seqs), 0))
         B, dev = len(seqs), self.norm.device
         if sampling is None:

@@ -37,3 +37,12 @@ def test_a_step_that_fails_is_not_counted(small, monkeypatch, fails):  # noqa: F
     p.fails = None
     assert p.model.generate(c, seqs, torch.tensor([0, 4]), 3).tolist() == [[1, 2, 3], [5, 6, 7]]
     assert [c.length(s) for s in seqs] == [17 + fails, 5 + fails]
+
+
+@pytest.mark.parametrize("new", [0, -1, -3])
+def test_no_tokens(small, monkeypatch, new):  # noqa: F811
+    p, c = Passes(monkeypatch), small(4)
+    a = c.new()
+    c.step([a], [5])
+    out = p.model.generate(c, [a], torch.tensor([2]), new)
+    assert out.shape == (1, 0) and out.dtype == torch.int64 and c.length(a) == 5 and p.count == 0
