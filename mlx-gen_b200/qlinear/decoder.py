@@ -217,6 +217,9 @@ def plan_step(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: torch
     return _native.plan_step(page_table, lengths, new_tokens, page_size, max_tokens, max_kv, free_pages, taken, out)
 
 
+MAX_SAMPLE_ROW = 1310208  # bytes of a row of logits that `sample` takes
+
+
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: bool = False):
     """One token per row of ``logits [B, V]`` from the random numbers ``u [B]`` (float32 in [0, 1)): int64 ``[B]``,
     with ``logprobs`` also the logarithms of the probabilities with which they were drawn (float32 ``[B]``)::

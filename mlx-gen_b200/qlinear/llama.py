@@ -128,14 +128,15 @@ class Decoder:
     def generate(self, cache: PagedCache, seqs: Sequence[int], tokens: torch.Tensor, new: int, sampling: Optional[Sampling] = None,
                  u: Optional[torch.Tensor] = None, graph: bool = False) -> torch.Tensor:
         """Continuation of sequences from their next tokens [B]: [B, new] token ids, the most likely ones or, with
-        ``sampling``, drawn by the random numbers ``u [new, B]`` (float32 in [0, 1); fresh ones if not given).  The pages of
-        all steps are taken at the start, and the steps are issued without waiting for one; with ``graph`` they are
-        one captured graph, replayed."""
+        ``sampling``, drawn by the random numbers ``u [new, B]`` (float32 in [0, 1); fresh ones if not given); -1 for
+        a row of logits with a NaN.  The pages of all steps are taken at the start, and the steps are issued without waiting for
+        one; with ``graph`` they are one captured graph, replayed."""
         self._fits(max(cache.length(s) for s in seqs) + new)
         if new <= 0:
             return tokens.new_empty((len(seqs), 0))
         B, dev = len(seqs), self.norm.device
-        if sampling is None:
+        greedy = sampling is None
+        if greedy:
             sampling, u = Sampling(temperature=0.0), torch.zeros((new, B), device=dev)
         elif u is None:
             u = torch.rand((new, B), device=dev)
@@ -149,7 +150,9 @@ class Decoder:
 
         def step():
             logits = self.forward(current, cache, ahead.next())
-            current.copy_(sampling.draw(logits, u.index_select(0, at)[0]))
+            # (a vocabulary longer than sampling's rows has its most likely token all the same)
+            long = greedy and logits.shape[1] * logits.element_size() > decoder.MAX_SAMPLE_ROW
+            current.copy_(logits.argmax(-1) if long else sampling.draw(logits, u.index_select(0, at)[0]))
             out.index_copy_(0, at, current[None])
             at.add_(1)
 

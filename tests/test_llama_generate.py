@@ -46,3 +46,25 @@ def test_no_tokens(small, monkeypatch, new):  # noqa: F811
     c.step([a], [5])
     out = p.model.generate(c, [a], torch.tensor([2]), new)
     assert out.shape == (1, 0) and out.dtype == torch.int64 and c.length(a) == 5 and p.count == 0
+
+
+def test_a_vocabulary_past_the_rows_of_sampling(small, monkeypatch):  # noqa: F811
+    """The most likely token needs no sampling; drawing one is refused as ever."""
+    p, c = Passes(monkeypatch), small(4)
+    logits = torch.zeros(1, llama.decoder.MAX_SAMPLE_ROW // 2 + 1, dtype=torch.bfloat16)
+    logits[0, -1] = 1
+
+    def sample(x, u, **kw):
+        raise ValueError
+
+    monkeypatch.setattr(llama.Decoder, "forward", lambda *a: logits)
+    monkeypatch.setattr(llama.decoder, "sample", sample)
+    a = c.new()
+    c.step([a], [5])
+    assert p.model.generate(c, [a], torch.tensor([2]), 2).tolist() == [[655104, 655104]]
+    with pytest.raises(ValueError):
+        p.model.generate(c, [a], torch.tensor([2]), 2, llama.Sampling())
+    logits = logits[:, 1:]
+    with pytest.raises(ValueError):
+        p.model.generate(c, [a], torch.tensor([2]), 2)
+    assert c.length(a) == 7
