@@ -614,9 +614,7 @@ template <typename T, bool CLUSTER, bool GLOBAL>
 __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER, GLOBAL> &row, float top, float least, uint64_t k) {
     Shared *sh = row.sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // (a range below 6e-36 or that overflows has no bins: the search by keys takes such a row)
-    const float c = (BINS - 1) / (top - least);
-    if (!(c > 0.f && c < INFINITY)) return -INFINITY;
+    const float c = top > least ? (BINS - 1) / (top - least) : 0.f;
     uint32_t *count = sh->count[row.turn & 1], *group = sh->group_count[row.turn & 1];
     ++row.turn;
     *reinterpret_cast<uint4 *>(count + 4 * tid) = make_uint4(0, 0, 0, 0);
@@ -646,7 +644,8 @@ __device__ __forceinline__ float bound_of_largest(Row<T, CLUSTER, GLOBAL> &row, 
     __syncthreads();
     const uint32_t bin = sh->found_bin;
     __syncthreads();
-    if (bin == NO_INDEX) return -INFINITY;
+    // (a range below 6e-36 or one that overflows has no bins: the search by keys takes such a row)
+    if (bin == NO_INDEX || c == 0.f || c == INFINITY) return -INFINITY;
     // the bin's lower edge, less what the roundings of the bin's number may amount to
     const float range = top - least, edge = top - (float)(bin + 1) / c - 1e-5f * range - 1e-6f * fabsf(top);
     return edge > -INFINITY ? edge : -INFINITY;
