@@ -53,7 +53,7 @@ class PagedCache:
         self._lists: Dict[int, List[int]] = {}  # -1: an evicted page
         self._lens: Dict[int, int] = {}
         self._least: Dict[int, int] = {}  # the length that an evicted sequence cannot be truncated below
-        self._lent: set = set()  # sequences whose steps an Ahead plans
+        self._lent: Dict[int, "Ahead"] = {}  # sequences whose steps an Ahead plans
         self._next = 0
 
     # ---- what is there
@@ -180,6 +180,10 @@ class PagedCache:
         the GPU one by one.  Until the returned ``Ahead`` is closed, these sequences belong to it."""
         return Ahead(self, seqs, steps)
 
+    def ahead_of(self, seq: int) -> Optional["Ahead"]:
+        """The open ``Ahead`` that plans the sequence's steps, to be closed by who has lost it; None if there is none."""
+        return self._lent.get(seq)
+
     def _room(self, seqs: Sequence[int], new_tokens: Sequence[int]) -> int:
         """Pages that the tokens need beyond those there, without copies of shared ones."""
         if len(seqs) != len(new_tokens) or len(set(seqs)) != len(seqs) or not seqs:
@@ -242,9 +246,8 @@ class Ahead:
     tensors made on the GPU from the lengths of the step before: ``next`` uploads nothing and waits for nothing,
     and may be captured in a graph and replayed, up to ``steps`` times in all; a replay beyond them has no tokens, and
     ``device_error()`` tells.  ``close`` tells the cache how many steps ran; a captured step must not be replayed after
-    it (its pages may be another sequence's by then).  One that is dropped without ``close`` closes with no step."""
-
-    _open = False
+    it (its pages may be another sequence's by then).  The cache holds it until then (``ahead_of``): one that a program drops
+    may still be captured in its graphs."""
 
     def __init__(self, cache: PagedCache, seqs: Sequence[int], steps: int):
         if steps < 1:
@@ -268,12 +271,8 @@ class Ahead:
         except BaseException:  # (no memory on the device)
             cache._drop(self._free)
             raise
-        cache._lent.update(self.seqs)
+        cache._lent.update(dict.fromkeys(self.seqs, self))
         self._open = True
-
-    def __del__(self):
-        if self._open:
-            self.close(0)
 
     def next(self) -> Step:
         """The next step; its tensors are those of the step before, written again.  More calls than steps raise
@@ -299,7 +298,8 @@ class Ahead:
         if not 0 <= done <= self.steps:
             raise ValueError(f"{self.steps} steps were reserved, {done} cannot have run")
         c = self.cache
-        c._lent.difference_update(self.seqs)
+        for s in self.seqs:
+            del c._lent[s]
         self._open = False
         at = 0
         for _ in range(done):  # pages were taken in the order of the steps, in each of the sequences
