@@ -32,7 +32,8 @@ static int log2i(int64_t v) {
 static bool touches_rows(const void *a, int64_t n, const void *base, int64_t rows, int64_t stride, int64_t width) {
     if (n <= 0 || rows <= 0 || width <= 0) return false;
     const int64_t from = (int64_t)(reinterpret_cast<intptr_t>(a) - reinterpret_cast<intptr_t>(base));
-    const int64_t row = from < width ? 0 : rows > 1 ? (from - width) / stride + 1 : 1;  // the first that ends behind a
+    if (from + n <= 0 || from >= (__int128)(rows - 1) * stride + width) return false;  // (nearly always)
+    const int64_t row = from < width ? 0 : (from - width) / stride + 1;  // the first that ends behind a
     return row < rows && row * stride < from + n;
 }
 
@@ -264,9 +265,10 @@ int ql_plan_step_within(int32_t *page_table, int64_t table_stride, int64_t table
     for (const Range &w : all) {
         if ((w.written || free_pages) && touches_rows(w.at, w.bytes, page_table, B, 4 * table_stride, 4 * table_width))
             return fail(QL_EINVAL_ARG, "ql_plan_step: the page table overlaps another argument");
+        if (!w.written) continue;
         for (const Range &r : all) {
             const bool in_place = w.at == r.at && ((&w == &all[7] && &r == &all[0]) || (&w == &all[8] && &r == &all[3]));
-            if (w.written && &r != &w && !in_place && touches_rows(r.at, r.bytes, w.at, 1, w.bytes, w.bytes))
+            if (&r != &w && !in_place && touches_rows(r.at, r.bytes, w.at, 1, w.bytes, w.bytes))
                 return fail(QL_EINVAL_ARG, "ql_plan_step: an output overlaps another argument");
         }
     }
