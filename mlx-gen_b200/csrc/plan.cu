@@ -4,7 +4,8 @@
 //     table[b][held_b + i] = free[taken + (exclusive sum of fresh_b) + i],  i < fresh_b
 //     token t of sequence b (t = q_starts_b + i): position have_b + i, slot table[b][position /
 //     page_size] * page_size + position % page_size
-// so that a decode step needs nothing from the host and can be captured in a graph and replayed.
+// so that a decode step needs nothing from the host and can be captured in a graph and replayed.  All or nothing: too few
+// pages, columns or rows, or a sequence past max_kv, and the step has no token.
 //
 // Bound: latency (a chain of dependent loads and barriers; 16 bytes a token written).  Split: every
 // CTA sums the counts of all sequences by itself (a thread has B / threads neighbours), then takes

@@ -23,8 +23,10 @@
 // top-p counts in 2048 bins and lists a few bins around the border, or all above it where these are few.
 // Scalars travel by stores into the other CTAs' shared memory before a barrier; what every warp would compute for itself is
 // computed by one.
-// Measured (bf16, 128256 logits, a graph's replay): one row greedy 4.3 us, without filter 8.5, top-k 50 11.4, top-p 0.95
-// 16.2; 64 rows 7.8, 22, 16, 61; 256 rows with top-p 0.98 at temperature 1.5 (half the vocabulary stays) 261.
+// Measured (bf16, 128256 logits from N(0, 2) with 24 likely ones among them, a graph's replay of the same rows): one row greedy
+// 4.3 us, without filter 8.4, top-k 50 11.5, top-p 0.95 at temperature 0.8 16.2 (18.7 with log-probabilities and other rows
+// each time); 64 rows 7.8, 22, 16, 62; 256 rows with top-p 0.98 at temperature 1.5 (half the vocabulary stays) 250, without
+// the likely ones 301.
 #include <string.h>
 
 #include "pdl.cuh"
@@ -1277,14 +1279,22 @@ template <typename T>
 static int launch(const Params &q, int64_t B, cudaStream_t st) {
     Params p = q;
     const int64_t bytes = (int64_t)p.V * (int64_t)sizeof(T);
-    // CTAs of a row: up to 16, fewer where the rows fill the GPU (two CTAs an SM; some more than that at a time pay
-    // while they are few: 96 rows of 607 KB in 4 CTAs 62 us, in 2 68; 256 rows of 256 KB in 2 90, in 1 84), and
-    // slices of 4 KB at least.
+    // CTAs of a row: up to 16 while all rows together have at most 400 (296 are resident at a time), slices of 4 KB at least.
+    // 128256 bf16 logits, us without filter / with top-p 0.95 / with settings of each row's own:
+    //      64 rows  4 CTAs 22 / 76 / 79    2 CTAs 38 / 121 / 124  8 CTAs 31 / 100 / 67
+    //      96       4 CTAs 33 / 114 / 87   2 CTAs 40 / 125 / 140  8 CTAs 44 / 149 / 87
+    //     200       2 CTAs 61 / 193 / 158  1 CTA  71 / 221 / 244  4 CTAs 63 / 211 / 120
+    //     256       1 CTA  74 / 246 / 257  2 CTAs 79 / 246 / 173
+    // (96 of 151643 in f32: 4 CTAs 51 / 136 / 100, 2 CTAs 56 / 163 / 149).  The rule knows the number of rows, not the settings, and gives
+    // away most next to where it steps, and for settings of the rows' own, whose CTAs run unequally long:
+    //      24 rows 16 CTAs 22 / 72 / 40    8 CTAs 15 / 51 / 45
+    //     110       2 CTAs 40 / 158 / 135  4 CTAs 43 / 141 / 94
+    //     160       2 CTAs 59 / 186 / 142  4 CTAs 51 / 178 / 102
     int ctas = MAX_CTAS;
     while (ctas > 1 && (B * ctas > 400 || bytes / ctas < 4096)) ctas /= 2;
     p.slice = ((p.V + ctas - 1) / ctas + 15) / 16 * 16;
-    // Slices of which two fit an SM stay in shared memory for all passes (64 rows of 256 KB, top-k 50: 16 us, 23 read again by
-    // each pass); longer ones are read again, from L2 mostly (256 rows: 42 us, 62 in slices of 64 KB).
+    // Slices of which two fit an SM stay in shared memory for all passes (64 rows of 256 KB, top-k 50: 16 us, 19 read again by
+    // each pass); longer ones are read again, from L2 mostly (256 rows: 41 us, 60 in slices of 64 KB).
     const bool global = (int64_t)p.slice * (int64_t)sizeof(T) > MAX_SLICE;
     const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (global ? 0 : (size_t)p.slice * sizeof(T) + 32);
     auto kernel = ctas > 1 ? (global ? sample_kernel<T, true, true> : sample_kernel<T, true, false>)

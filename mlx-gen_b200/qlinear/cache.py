@@ -112,7 +112,7 @@ class PagedCache:
     def evict(self, seq: int, window: int, sinks: int = 0) -> int:
         """Gives back the pages that no further token of the sequence sees, where each sees the last
         ``window`` positions and the first ``sinks`` (``paged_attention``'s window and sinks); returns how many.
-        Their places in the page list say -1; the sequence can no longer be truncated."""
+        Their places in the page list say -1; the sequence can no longer be truncated below its present length."""
         self._keeps(seq)
         if window < 1 or sinks < 0:
             raise ValueError(f"a window must be positive and sinks not negative, got {window} and {sinks}")
