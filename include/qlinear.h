@@ -311,7 +311,7 @@ int ql_plan_step_within(int32_t *page_table, int64_t table_stride, int64_t table
  * at most.  Each setting is one number for each row
  * (a pointer) or for all (NULL and the ..._all argument, kept in 64 bits).  Weights are computed in 64 bits and
  * summed as whole numbers (of 2^-46, for more than 2^17 tokens 2^(ceil(log2 V) - 63)), so that a row's token does not
- * depend on the rest of the batch; a logit of -inf is never drawn, those of +inf share everything.  u is taken as at
+ * depend on the rest of the batch, and one whose weight rounds to 0 is never drawn, not by u = 0 or 1 either; a logit of -inf is never drawn, those of +inf share everything.  u is taken as at
  * least 0, and 1 or more gives the last token that stays.  A row with a NaN (logits, settings or u), a
  * negative temperature or nothing above -inf: token -1, log-probability NaN.  logprobs [B] or
  * NULL: the logarithm of the probability with which the token was drawn (0 for temperature 0).

@@ -231,7 +231,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
 
     Each setting is a number or a tensor ``[B]`` (float32, top_k int32) with each row's own; top_k 0, top_p 1 and
     min_p 0 filter nothing.  temperature 0 takes the largest logit, the lowest index of equal ones.
-    Sums are exact, so a row's token does not depend on the rest of the batch.  Logits of +inf share everything.  A row with a NaN
+    Weights are summed exactly, as multiples of 2^-46 (to 2^-43, for more than 131072 tokens), so a row's token does not depend on the
+    rest of the batch, and one whose weight rounds to 0 is never drawn (not by u = 0 either).  Logits of +inf share everything.  A row with a NaN
     (among the logits or its settings), a negative temperature or no logit above -inf gives token -1 and log-probability NaN."""
     return _native.sample(logits, u, temperature, top_k, top_p, min_p, logprobs)
 
